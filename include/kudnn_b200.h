@@ -44,6 +44,10 @@ extern "C" {
 #define KUDNN_B200_S32 4
 #define KUDNN_B200_S8 5
 #define KUDNN_B200_U8 6
+/* Types beyond the reference's table: 8-bit floating point (sign, 4 bits of exponent, 3 of mantissa, no infinities, largest value 448),
+ * accepted as the operands of kudnn_b200_grouped_* and written by kudnn_b200_quantize_run, and 64-bit integers, accepted as offsets. */
+#define KUDNN_B200_E4M3 7
+#define KUDNN_B200_S64 8
 
 /* Activations: the values of KuDNN::ActivationFunction (src/dnn/include/operations/kudnn_eltwise.hpp:24-54);
  * 0 (UNIMPLEMENTED there) means "no activation" here. */
@@ -208,6 +212,73 @@ KUDNN_B200_API int kudnn_b200_rmsnorm_validate(int64_t rows, int64_t axis, int d
 KUDNN_B200_API int kudnn_b200_rmsnorm_run(const void *src, void *dst, const void *scale, float *variance, int64_t rows,
                                           int64_t axis, int dtype, int flags, int save_stats, float eps,
                                           void *cuda_stream);
+
+/* ---- feed-forward layers in 8-bit floating point, and of experts ---------------------------------------------------
+ * No counterpart in the reference.  Device pointers only; asynchronous on the stream; forward only, as everything here.
+ *
+ * Quantisation: rows of F32 / F16 / BF16 values -> E4M3 with an fp32 scale per block, value = q * scale.
+ *   most  = max(|v| over the block, 1e-30),  scale = most / 448,  q = e4m3(v * (448 / most)), to nearest even
+ * block_rows = 1: a block is 128 columns of one row (activations), scale[r * s_row + (c / 128) * s_col];
+ * block_rows = 128: 128 x 128 (weights), scale[(r / 128) * s_row + (c / 128) * s_col].  The last blocks may be cut by rows and k.
+ * With block_rows = 1, v may be other than row r of x:
+ *   gate = 1       v = silu(x[r, 0:k]) * x[r, k:2k], in fp32 (between the two products of a feed-forward block)
+ *   index != NULL  row r of q is made from row index[r] of x (tokens on their way to several experts); r with an index outside
+ *                  [0, x_rows) becomes zeros
+ * A block with a NaN becomes NaN throughout, scale included; one with infinities gets an infinite scale, zeros for its finite elements
+ * and NaN for the others.  Any alignment is taken; rows of x and q on 16-byte boundaries are read and written 16 bytes at a time. */
+typedef struct kudnn_b200_quantize_desc {
+    int64_t rows, k;       /* of q */
+    int64_t x_rows;        /* rows of x: == rows unless the run gets an index */
+    int64_t x_ld, q_ld;    /* row pitches in elements; columns are contiguous */
+    int64_t s_row, s_col;  /* strides of scale in elements */
+    int32_t x_dtype, gate, block_rows, reserved;
+} kudnn_b200_quantize_desc;
+KUDNN_B200_API int kudnn_b200_quantize_validate(const kudnn_b200_quantize_desc *desc);
+KUDNN_B200_API int kudnn_b200_quantize_run(const kudnn_b200_quantize_desc *desc, const void *x, void *q, float *scale,
+                                           const int32_t *index, void *cuda_stream);
+
+/* Products by group: the rows of a belong, in order, to `groups` weight matrices (experts), and
+ *     c[r, :] = act( a[r, :] . b[g]^T + bias[g] )     for offsets[g] <= r < offsets[g + 1].
+ * offsets: groups + 1 integers (S32 or S64) in DEVICE memory, so that sizes the GPU computed need not come back to the host; empty
+ * groups are fine.  Offsets are brought into [0, rows], and one that is below its predecessor makes an empty group; rows of c that no
+ * group holds (before the first offset, after the last) become zeros.  Without offsets (offsets_dtype = 0, groups = 1) it is one
+ * product of all rows.
+ * ab_dtype F16 / BF16: fp32 sums.  ab_dtype E4M3: both operands carry fp32 scales, a one per row and 128 columns of K, b one per
+ * 128 x 128 block of [n, k], as kudnn_b200_quantize_run writes them: sum over blocks of a_scale * b_scale * (sum within the block).
+ * c_dtype, bias_dtype: F32 / F16 / BF16.  The bias is added and the activation applied in fp32; the result is rounded once.
+ * Tensors are addressed by element strides.  Operands whose rows are K-contiguous, 16-byte aligned and 16 bytes apart or a multiple of
+ * it go to the tensor cores and are read in place; any other layout takes a general kernel that is many times slower.
+ * A handle holds no scratch: its runs may overlap on any streams and be captured into graphs, which it must outlive. */
+typedef struct kudnn_b200_grouped_desc {
+    int64_t rows, n, k;
+    int32_t groups, ab_dtype, c_dtype, bias_dtype;
+    int32_t has_bias, act, offsets_dtype, reserved;
+    float act_alpha, reserved_f;
+    int64_t a_sm, a_sk;
+    int64_t b_sg, b_sn, b_sk;
+    int64_t c_sm, c_sn;
+    int64_t bias_sg, bias_sn;
+    int64_t a_scale_sm, a_scale_sk;               /* per row, per block of K */
+    int64_t b_scale_sg, b_scale_sn, b_scale_sk;   /* per group, per block of N, per block of K */
+} kudnn_b200_grouped_desc;
+typedef struct kudnn_b200_grouped_args {
+    const void *a, *b;
+    void *c;
+    const void *bias;              /* non-NULL iff has_bias */
+    const float *a_scale, *b_scale; /* non-NULL iff ab_dtype is E4M3 */
+    const void *offsets;           /* non-NULL iff offsets_dtype is set */
+} kudnn_b200_grouped_args;
+typedef struct kudnn_b200_grouped_s *kudnn_b200_grouped_t;
+KUDNN_B200_API int kudnn_b200_grouped_validate(const kudnn_b200_grouped_desc *desc);
+KUDNN_B200_API int kudnn_b200_grouped_create(const kudnn_b200_grouped_desc *desc, kudnn_b200_grouped_t *handle);
+KUDNN_B200_API int kudnn_b200_grouped_destroy(kudnn_b200_grouped_t handle);
+KUDNN_B200_API int kudnn_b200_grouped_run(kudnn_b200_grouped_t handle, const kudnn_b200_grouped_args *args, void *cuda_stream);
+/* As kudnn_b200_linear_check / _force_kernel (SIMT or TC) / _last_kernel / kudnn_b200_debug_set_wait: every CTA leaves out the loads of
+ * the k-blocks from `skip_kblock` on. */
+KUDNN_B200_API int kudnn_b200_grouped_check(kudnn_b200_grouped_t handle, void *cuda_stream);
+KUDNN_B200_API int kudnn_b200_grouped_force_kernel(kudnn_b200_grouped_t handle, int kernel);
+KUDNN_B200_API int kudnn_b200_grouped_last_kernel(kudnn_b200_grouped_t handle);
+KUDNN_B200_API int kudnn_b200_grouped_set_wait(kudnn_b200_grouped_t handle, long long wait_limit_cycles, int skip_kblock);
 
 /* Reads the device-side status word of the handle (bounded waits that gave up) after synchronising the stream. */
 KUDNN_B200_API int kudnn_b200_linear_check(kudnn_b200_linear_t handle, void *cuda_stream);

@@ -6,7 +6,7 @@ this module never touches the data itself.
 import ctypes
 import os
 
-F32, F16, BF16, S32, S8, U8 = 1, 2, 3, 4, 5, 6
+F32, F16, BF16, S32, S8, U8, E4M3, S64 = 1, 2, 3, 4, 5, 6, 7, 8
 ACT_NONE, ACT_RELU, ACT_TANH, ACT_SIGMOID, ACT_GELU_TANH, ACT_SWISH, ACT_GELU_ERF = 0, 5, 9, 10, 20, 25, 27
 RES_NONE, RES_EXT, RES_IDENTICAL, RES_ELTWISE_MUL = 0, 1, 2, 3
 KERNEL_AUTO, KERNEL_SIMT, KERNEL_GEMV_FMA, KERNEL_GEMV_MMA, KERNEL_TC = 0, 1, 2, 3, 4
@@ -56,6 +56,40 @@ class LinearArgs(ctypes.Structure):
     ]
 
 
+class QuantizeDesc(ctypes.Structure):
+    """kudnn_b200_quantize_desc."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("k", ctypes.c_int64), ("x_rows", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64), ("q_ld", ctypes.c_int64), ("s_row", ctypes.c_int64), ("s_col", ctypes.c_int64),
+        ("x_dtype", ctypes.c_int32), ("gate", ctypes.c_int32), ("block_rows", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class GroupedDesc(ctypes.Structure):
+    """kudnn_b200_grouped_desc."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+        ("groups", ctypes.c_int32), ("ab_dtype", ctypes.c_int32), ("c_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+        ("has_bias", ctypes.c_int32), ("act", ctypes.c_int32), ("offsets_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("act_alpha", ctypes.c_float), ("reserved_f", ctypes.c_float),
+        ("a_sm", ctypes.c_int64), ("a_sk", ctypes.c_int64),
+        ("b_sg", ctypes.c_int64), ("b_sn", ctypes.c_int64), ("b_sk", ctypes.c_int64),
+        ("c_sm", ctypes.c_int64), ("c_sn", ctypes.c_int64),
+        ("bias_sg", ctypes.c_int64), ("bias_sn", ctypes.c_int64),
+        ("a_scale_sm", ctypes.c_int64), ("a_scale_sk", ctypes.c_int64),
+        ("b_scale_sg", ctypes.c_int64), ("b_scale_sn", ctypes.c_int64), ("b_scale_sk", ctypes.c_int64),
+    ]
+
+
+class GroupedArgs(ctypes.Structure):
+    """kudnn_b200_grouped_args."""
+
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("c", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("a_scale", ctypes.c_void_p), ("b_scale", ctypes.c_void_p), ("offsets", ctypes.c_void_p)]
+
+
 EXPORTS = [
     "kudnn_b200_linear_validate", "kudnn_b200_linear_create", "kudnn_b200_linear_clone", "kudnn_b200_linear_destroy",
     "kudnn_b200_linear_prepack", "kudnn_b200_linear_run", "kudnn_b200_linear_run_host", "kudnn_b200_linear_check",
@@ -67,6 +101,9 @@ EXPORTS = [
     "kudnn_b200_linear_unpack", "kudnn_b200_debug_set_wait", "kudnn_b200_debug_fail_allocation",
     "kudnn_b200_linear_run_sharded", "kudnn_b200_activation_validate", "kudnn_b200_activation_run", "kudnn_b200_rmsnorm_validate", "kudnn_b200_rmsnorm_run",
     "kudnn_b200_linear_set_multicast", "kudnn_b200_linear_graphs",
+    "kudnn_b200_quantize_validate", "kudnn_b200_quantize_run", "kudnn_b200_grouped_validate", "kudnn_b200_grouped_create",
+    "kudnn_b200_grouped_destroy", "kudnn_b200_grouped_run", "kudnn_b200_grouped_check", "kudnn_b200_grouped_force_kernel",
+    "kudnn_b200_grouped_last_kernel", "kudnn_b200_grouped_set_wait",
 ]
 
 _lib = None
@@ -118,6 +155,16 @@ def library():
     lib.kudnn_b200_linear_workspace_bytes.argtypes = [vp]
     lib.kudnn_b200_linear_workspace_bytes.restype = i64
     lib.kudnn_b200_shard_range.argtypes = [i64, i32, i32, i64, ctypes.POINTER(i64), ctypes.POINTER(i64)]
+    lib.kudnn_b200_quantize_validate.argtypes = [ctypes.POINTER(QuantizeDesc)]
+    lib.kudnn_b200_quantize_run.argtypes = [ctypes.POINTER(QuantizeDesc), vp, vp, vp, vp, vp]
+    lib.kudnn_b200_grouped_validate.argtypes = [ctypes.POINTER(GroupedDesc)]
+    lib.kudnn_b200_grouped_create.argtypes = [ctypes.POINTER(GroupedDesc), ctypes.POINTER(vp)]
+    lib.kudnn_b200_grouped_destroy.argtypes = [vp]
+    lib.kudnn_b200_grouped_run.argtypes = [vp, ctypes.POINTER(GroupedArgs), vp]
+    lib.kudnn_b200_grouped_check.argtypes = [vp, vp]
+    lib.kudnn_b200_grouped_force_kernel.argtypes = [vp, i32]
+    lib.kudnn_b200_grouped_last_kernel.argtypes = [vp]
+    lib.kudnn_b200_grouped_set_wait.argtypes = [vp, ctypes.c_longlong, i32]
     lib.kudnn_b200_last_error.restype = ctypes.c_char_p
     lib.kudnn_b200_version.restype = ctypes.c_char_p
     _lib = lib
@@ -226,6 +273,95 @@ def rmsnorm(src, dst, rows, axis, dtype, scale=None, variance=None, flags=0, sav
     """RMS normalisation over the last axis of a dense [rows, axis] tensor; device or host pointers."""
     _check(library().kudnn_b200_rmsnorm_run(_ptr(src), _ptr(dst), _ptr(scale), _ptr(variance), rows, axis, dtype, flags,
                                             1 if save_stats else 0, eps, stream))
+
+
+SCALE_BLOCK = 128
+
+
+def make_quantize_desc(rows, k, dtype, *, gate=False, x_rows=None, block_rows=1, x_ld=None, q_ld=None, scale_strides=None):
+    """Descriptor of q [rows, k] (e4m3) and its scales from x [x_rows, k], or [x_rows, 2 k] with `gate`.  x_rows differs from rows only
+    where runs get an index, which names the row of x for each row of q.
+
+    Defaults: dense x; q at a pitch of k; scale_strides = (row, block of columns) so that the scales of one block of columns lie next to
+    one another (activations, block_rows = 1: what kudnn_b200_grouped_run reads fastest) or row-major (weights, block_rows = 128).
+    """
+    d = QuantizeDesc()
+    d.rows, d.k, d.x_rows = rows, k, rows if x_rows is None else x_rows
+    d.x_ld = x_ld if x_ld is not None else (2 * k if gate else k)
+    d.q_ld = q_ld if q_ld is not None else k
+    d.s_row, d.s_col = scale_strides or ((1, max(rows, 1)) if block_rows == 1 else (-(-k // SCALE_BLOCK), 1))
+    d.x_dtype, d.gate, d.block_rows = dtype, 1 if gate else 0, block_rows
+    return d
+
+
+def quantize(desc, x, q, scale, index=None, stream=None):
+    """x -> q (e4m3) and scale (fp32); device pointers, asynchronous on `stream`."""
+    _check(library().kudnn_b200_quantize_run(ctypes.byref(desc), _ptr(x), _ptr(q), _ptr(scale), _ptr(index), stream))
+
+
+def make_grouped_desc(rows, n, k, dtype, *, groups=1, c_dtype=None, offsets_dtype=0, a_strides=None, b_strides=None, c_strides=None,
+                      a_scale_strides=None, b_scale_strides=None, has_bias=False, bias_dtype=None, bias_strides=None, act=ACT_NONE,
+                      act_alpha=1.0):
+    """Descriptor for c[r] = act(a[r] . b[g]^T + bias[g]), offsets[g] <= r < offsets[g + 1]; one product of all rows without offsets.
+
+    Strides are in elements: a (row, k), b (group, n, k), c (row, n), bias (group, n), a_scale (row, block of k), b_scale (group, block
+    of n, block of k).  Defaults: everything dense, a_scale with the scales of one block of k next to one another; results of E4M3
+    operands are BF16, others of the operands' type.
+    """
+    blocks_n, blocks_k = -(-n // SCALE_BLOCK), -(-k // SCALE_BLOCK)
+    d = GroupedDesc()
+    d.rows, d.n, d.k, d.groups = rows, n, k, groups
+    d.ab_dtype, d.c_dtype = dtype, c_dtype or (BF16 if dtype == E4M3 else dtype)
+    d.has_bias, d.bias_dtype = 1 if has_bias else 0, bias_dtype or d.c_dtype
+    d.act, d.act_alpha, d.offsets_dtype = act, act_alpha, offsets_dtype
+    d.a_sm, d.a_sk = a_strides or (k, 1)
+    d.b_sg, d.b_sn, d.b_sk = b_strides or (n * k, k, 1)
+    d.c_sm, d.c_sn = c_strides or (n, 1)
+    d.bias_sg, d.bias_sn = bias_strides or (n, 1)
+    d.a_scale_sm, d.a_scale_sk = a_scale_strides or (1, max(rows, 1))
+    d.b_scale_sg, d.b_scale_sn, d.b_scale_sk = b_scale_strides or (blocks_n * blocks_k, blocks_k, 1)
+    return d
+
+
+class Grouped:
+    """One created product by group (kudnn_b200_grouped_t); with one group and no offsets a plain product."""
+
+    def __init__(self, desc):
+        self._lib = library()
+        self.desc = desc
+        h = ctypes.c_void_p()
+        _check(self._lib.kudnn_b200_grouped_create(ctypes.byref(desc), ctypes.byref(h)))
+        self._h = h
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._lib.kudnn_b200_grouped_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def run(self, a, b, c, offsets=None, a_scale=None, b_scale=None, bias=None, stream=None):
+        """Device pointers; asynchronous on `stream` (a cudaStream_t value, None = default stream)."""
+        args = GroupedArgs(_ptr(a), _ptr(b), _ptr(c), _ptr(bias), _ptr(a_scale), _ptr(b_scale), _ptr(offsets))
+        _check(self._lib.kudnn_b200_grouped_run(self._h, ctypes.byref(args), stream))
+
+    def check(self, stream=None):
+        _check(self._lib.kudnn_b200_grouped_check(self._h, stream))
+
+    def force_kernel(self, kernel):
+        _check(self._lib.kudnn_b200_grouped_force_kernel(self._h, kernel))
+
+    def set_wait(self, wait_limit_cycles, skip_kblock=-1):
+        """Test hook: limit of the device-side waits in SM cycles, and the k-block from which on no loads are issued."""
+        _check(self._lib.kudnn_b200_grouped_set_wait(self._h, wait_limit_cycles, skip_kblock))
+
+    @property
+    def last_kernel(self):
+        return self._lib.kudnn_b200_grouped_last_kernel(self._h)
 
 
 def debug_fail_allocation(nth):

@@ -45,6 +45,8 @@ struct GemvPlan {
 
 // Records the calling thread's last error text and returns `code`.
 int set_last_error(int code, const char *message);
+// cudaMalloc that also works while the thread captures a stream, and that the allocation test hook can make fail.
+cudaError_t library_malloc(void **ptr, size_t bytes);
 
 cudaError_t launch_simt(const LinearProblem &pr, int sm_count, cudaStream_t stream);
 // 8-bit integer operands (S8 / U8), 32-bit integer result and bias: exact sums

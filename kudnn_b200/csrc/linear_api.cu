@@ -153,6 +153,12 @@ int set_last_error(int code, const char *message)
     return fail(code, "%s", message);
 }
 
+cudaError_t library_malloc(void **ptr, size_t bytes)
+{
+    CaptureRelaxed relaxed;
+    return device_malloc(ptr, bytes);
+}
+
 }  // namespace kb
 
 struct kudnn_b200_linear_s {
