@@ -309,8 +309,14 @@ int kudnn_b200_grouped_run(kudnn_b200_grouped_t h, const kudnn_b200_grouped_args
     p.act = d.act;
     p.act_alpha = d.act_alpha;
     p.offsets_64 = d.offsets_dtype == KUDNN_B200_S64 ? 1 : 0;
-    const cudaError_t e = kb::launch_grouped_simt(p, static_cast<cudaStream_t>(cuda_stream));
-    h->last_kernel = KUDNN_B200_KERNEL_SIMT;
+    const bool takes = kb::grouped_tc_takes(p);
+    if (h->forced_kernel == KUDNN_B200_KERNEL_TC && !takes) {
+        return fail(KUDNN_B200_UNSUPPORTED, "grouped: the tensor cores want rows that are K-contiguous and 16-byte aligned");
+    }
+    const bool tc = takes && h->forced_kernel != KUDNN_B200_KERNEL_SIMT;
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    const cudaError_t e = tc ? kb::launch_grouped_tc(p, h->sm_count, h->status, h->wait_limit, h->skip_kblock, stream) : kb::launch_grouped_simt(p, stream);
+    h->last_kernel = tc ? KUDNN_B200_KERNEL_TC : KUDNN_B200_KERNEL_SIMT;
     return e == cudaSuccess ? KUDNN_B200_OK : fail_cuda(e, "grouped kernel launch");
 }
 

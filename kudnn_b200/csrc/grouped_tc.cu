@@ -1,0 +1,119 @@
+// Host side of the tensor-core kernel for grouped and block-scaled products (grouped_tc.cuh).
+#include "grouped_tc.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace kb {
+
+using namespace grp;
+
+namespace {
+
+// Row pitch and group distance as the tensor maps want them: a single row or group has none of its own.
+long long pitch_of(long long extent, long long stride, long long inner, int es)
+{
+    return extent > 1 ? stride : (inner * es + 15) / 16 * 16 / es;
+}
+
+bool pitch_fits(long long pitch, long long inner, int es)
+{
+    return pitch >= inner && pitch * es % 16 == 0 && pitch * es < (1ll << 40);
+}
+
+template <bool kScaled, int kTN>
+cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bound, int sm_count, const CUtensorMap &ta, const CUtensorMap &tb,
+                         cudaStream_t stream)
+{
+    using S = Shape<kScaled, kTN>;
+    auto kernel = grouped_tc_kernel<kScaled, kTN>;
+    static std::atomic<unsigned long long> prepared{0};  // devices, a bit each
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    if (dev >= 64 || (prepared.load() >> dev & 1ull) == 0) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        if (dev < 64) {
+            prepared.fetch_or(1ull << dev);
+        }
+    }
+    const int fixed = S::kFixedBytes + (g.groups + 1) * 8;
+    p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::kStageBytes);
+    p.splits = 1;
+    if (S::kSplits) {
+        // as many CTAs as there are SMs, two k-blocks each at least
+        while (p.splits < 8 && item_bound * p.splits * 2 <= sm_count && p.num_kb >= p.splits * 4) {
+            p.splits *= 2;
+        }
+        while (p.splits > 1 && (p.splits - 1) * ((p.num_kb + p.splits - 1) / p.splits) >= p.num_kb) {
+            p.splits /= 2;  // every CTA of a cluster has a share
+        }
+    }
+    p.kb_per_split = (p.num_kb + p.splits - 1) / p.splits;
+    const long long ctas = p.splits > 1 ? item_bound * p.splits : std::min<long long>(std::max<long long>(item_bound, 1), sm_count);
+    return launch_chained(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), static_cast<size_t>(fixed + p.stages * S::kStageBytes), stream,
+                          static_cast<unsigned>(p.splits), ta, tb, p);
+}
+
+template <bool kScaled>
+cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &ta, const CUtensorMap &tb, cudaStream_t stream)
+{
+    // the tile that holds twice an average group's rows, since groups are uneven; without offsets the one that holds them all
+    const long long rows = g.offsets == nullptr ? g.rows : 2ll * g.rows / g.groups;
+    const int tn = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    // offsets may leave out rows and make up to min(groups, rows) short tiles
+    const long long tiles = g.offsets == nullptr ? (g.rows + tn - 1) / tn : std::min(g.groups, g.rows) + g.rows / tn;
+    const long long bound = tiles * p.tiles_n;
+    switch (tn) {
+        case 32: return launch_shape<kScaled, 32>(g, p, bound, sm_count, ta, tb, stream);
+        case 64: return launch_shape<kScaled, 64>(g, p, bound, sm_count, ta, tb, stream);
+        case 128: return launch_shape<kScaled, 128>(g, p, bound, sm_count, ta, tb, stream);
+        default: return launch_shape<kScaled, 256>(g, p, bound, sm_count, ta, tb, stream);
+    }
+}
+
+}  // namespace
+
+bool grouped_tc_takes(const GroupedParams &p)
+{
+    const int es = p.ab_dtype == KUDNN_B200_E4M3 ? 1 : 2;
+    const long long ld_a = pitch_of(p.rows, p.a_sm, p.k, es), ld_b = pitch_of(p.n, p.b_sn, p.k, es);
+    return tc_available() && (p.a_sk == 1 || p.k == 1) && (p.b_sk == 1 || p.k == 1) &&
+           ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15u) == 0 && pitch_fits(ld_a, p.k, es) &&
+           pitch_fits(ld_b, p.k, es) && (p.groups == 1 || pitch_fits(p.b_sg, p.k, es));
+}
+
+cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus *status, long long wait_limit_cycles, int skip_kblock,
+                              cudaStream_t stream)
+{
+    const bool scaled = g.ab_dtype == KUDNN_B200_E4M3;
+    const int es = scaled ? 1 : 2, c_size = dtype_size(g.c_dtype);
+    const long long ld_b = pitch_of(g.n, g.b_sn, g.k, es);
+    CUtensorMap ta, tb;
+    cudaError_t e = tc_encode_groups(&ta, g.a, g.ab_dtype, 1, g.rows, g.k, pitch_of(1, 0, g.k, es), pitch_of(g.rows, g.a_sm, g.k, es), kBoxRows);
+    if (e == cudaSuccess) {
+        e = tc_encode_groups(&tb, g.b, g.ab_dtype, g.groups, g.n, g.k, g.groups > 1 ? g.b_sg : pitch_of(1, 0, g.k, es), ld_b, kTileN);
+    }
+    if (e != cudaSuccess) {
+        return e;
+    }
+    TcParams p;
+    p.g = g;
+    p.kb_elems = 128 / es;
+    p.num_kb = (g.k + p.kb_elems - 1) / p.kb_elems;
+    p.tiles_n = (g.n + kTileN - 1) / kTileN;
+    p.band = 8;
+    p.vec = (g.c_sn == 1 || g.n == 1) && (g.rows == 1 || g.c_sm * c_size % 16 == 0) && (reinterpret_cast<uintptr_t>(g.c) & 15u) == 0 ? 1 : 0;
+    p.idesc = make_idesc(g.ab_dtype == KUDNN_B200_BF16 ? KUDNN_B200_BF16 : KUDNN_B200_F16, 0, kTileN);  // e4m3 and fp16 have the same code, 0
+    p.load_kb = skip_kblock >= 0 ? std::min(skip_kblock, p.num_kb) : p.num_kb;
+    p.status = status;
+    p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimitCycles;
+    return scaled ? launch_kind<true>(g, p, sm_count, ta, tb, stream) : launch_kind<false>(g, p, sm_count, ta, tb, stream);
+}
+
+}  // namespace kb

@@ -98,6 +98,10 @@ const char *tc_unavailable_reason();
 // boxes of 128 bytes of K x box_rows rows with the 128-byte swizzle; rows and columns out of range read as zero.
 cudaError_t tc_encode_kmajor(void *map128, const void *base, int kind, long long rows, long long k_total, long long ld_elems,
                              int box_rows);
+// Tensor map of [groups][rows][k] matrices of F16, BF16 or 8-bit elements (any other code), row pitch ld_elems, group_elems apart, for
+// boxes of 128 bytes of K x box_rows rows of one group with the 128-byte swizzle; what is out of range reads as zero.
+cudaError_t tc_encode_groups(void *map128, const void *base, int dtype, long long groups, long long rows, long long k, long long group_elems,
+                             long long ld_elems, int box_rows);
 // How many CTA pairs with this much shared memory run at a time, as many as the GPU's partitions let; 0 if the driver does not say.
 int tc_pair_clusters(int kind, size_t smem_bytes);
 // with_staging: the launch writes output mirrors and needs the epilogue's row staging in shared memory

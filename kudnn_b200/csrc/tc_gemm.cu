@@ -100,6 +100,30 @@ cudaError_t tc_encode_kmajor(void *map128, const void *base, int kind, long long
     return e;
 }
 
+cudaError_t tc_encode_groups(void *map128, const void *base, int dtype, long long groups, long long rows, long long k, long long group_elems,
+                             long long ld_elems, int box_rows)
+{
+    if (!tc_available()) {
+        return cudaErrorNotSupported;
+    }
+    const int es = dtype == KUDNN_B200_F16 || dtype == KUDNN_B200_BF16 ? 2 : 1;
+    const CUtensorMapDataType dt = dtype == KUDNN_B200_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : dtype == KUDNN_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(groups)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld_elems) * es, static_cast<cuuint64_t>(group_elems) * es};
+    cuuint32_t box[3] = {static_cast<cuuint32_t>(kStageRowBytes / es), static_cast<cuuint32_t>(box_rows), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUtensorMap m;
+    CUresult r = g_encode(&m, dt, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        return cudaErrorInvalidValue;
+    }
+    std::memcpy(map128, &m, sizeof(m));
+    return cudaSuccess;
+}
+
 namespace {
 
 int env_choice(const char *name)

@@ -128,8 +128,14 @@ class Problem:
                 tol[lo:hi] += 2.0 ** -18 * r.abs() + 2.0 ** -20 * v.abs()
         return y, tol
 
+    def aligned(self):
+        size = 1 if self.dtype == "e4m3" else 2
+        return all(s * size % 16 == 0 for s in (self.a.stride(0), self.b_strides[0], self.b_strides[1])) and (self.b_strides[2] == 1 or self.k == 1)
+
     def check(self, kernel=kb.KERNEL_AUTO, stream=None):
         self.run(kernel, stream)
+        if self.aligned() and kernel == kb.KERNEL_AUTO:
+            assert self.kernel == kb.KERNEL_TC
         y, tol = self.exact()
         got = self.c.double()
         off = (got - y).abs()
@@ -296,6 +302,33 @@ def test_out_of_device_memory(cuda_device):
     finally:
         kb.debug_fail_allocation(-1)
     p.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("m", [1, 40, 100, 500])
+def test_a_wait_that_runs_out(cuda_device, dtype, m):
+    """Loads that never come: the kernel gives up, reports it and leaves the device usable."""
+    p = Problem(m, 256, 2048, dtype)
+    op = kb.Grouped(p.desc)
+    op.set_wait(20_000_000, 3)
+    op.run(p.a, p.b, p.c, a_scale=p.a_scale, b_scale=p.b_scale)
+    with pytest.raises(kb.KudnnError) as e:
+        op.check()
+    assert e.value.status == 5
+    op.set_wait(0)
+    op.run(p.a, p.b, p.c, a_scale=p.a_scale, b_scale=p.b_scale)
+    op.check()
+    y, tol = p.exact()
+    assert bool(((p.c.double() - y).abs() <= tol).all())
+
+
+@gpu
+def test_forced_tensor_cores_refuse_what_they_do_not_take(cuda_device):
+    p = Problem(20, 64, 100, "bf16", a_ld=101)
+    with pytest.raises(kb.KudnnError) as e:
+        p.run(kb.KERNEL_TC)
+    assert e.value.status == 1
 
 
 def small(**more):
