@@ -22,10 +22,10 @@ bool pitch_fits(long long pitch, long long inner, int es)
 }
 
 template <bool kScaled, int kTN>
-cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bound, int sm_count, const CUtensorMap &ta, const CUtensorMap &tb,
-                         cudaStream_t stream)
+cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bound, int sm_count, const CUtensorMap &tb, cudaStream_t stream)
 {
     using S = Shape<kScaled, kTN>;
+    constexpr int es = kScaled ? 1 : 2;
     auto kernel = grouped_tc_kernel<kScaled, kTN>;
     static std::atomic<unsigned long long> prepared{0};  // devices, a bit each
     int dev = 0;
@@ -42,6 +42,11 @@ cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bou
             prepared.fetch_or(1ull << dev);
         }
     }
+    CUtensorMap ta;
+    e = tc_encode_groups(&ta, g.a, g.ab_dtype, 1, g.rows, g.k, pitch_of(1, 0, g.k, es), pitch_of(g.rows, g.a_sm, g.k, es), S::kBoxRows);
+    if (e != cudaSuccess) {
+        return e;
+    }
     const int fixed = S::kFixedBytes + (g.groups + 1) * 8;
     p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::kStageBytes);
     p.splits = 1;
@@ -55,25 +60,32 @@ cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bou
         }
     }
     p.kb_per_split = (p.num_kb + p.splits - 1) / p.splits;
-    const long long ctas = p.splits > 1 ? item_bound * p.splits : std::min<long long>(std::max<long long>(item_bound, 1), sm_count);
-    return launch_chained(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), static_cast<size_t>(fixed + p.stages * S::kStageBytes), stream,
-                          static_cast<unsigned>(p.splits), ta, tb, p);
+    const size_t smem = static_cast<size_t>(fixed + p.stages * S::kStageBytes);
+    long long ctas = p.splits > 1 ? item_bound * p.splits : std::min<long long>(std::max<long long>(item_bound, 1), sm_count);
+    if (S::kPair) {
+        // as many pairs as the GPU's partitions hold
+        const int pairs = tc_pair_clusters(KUDNN_B200_F16, kSmemLimit);
+        ctas = 2 * std::min<long long>(std::max<long long>(item_bound, 1), pairs > 0 ? pairs : sm_count / 2);
+    }
+    return launch_chained(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, static_cast<unsigned>(S::kPair ? 2 : p.splits), ta, tb, p);
 }
 
 template <bool kScaled>
-cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &ta, const CUtensorMap &tb, cudaStream_t stream)
+cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &tb, cudaStream_t stream)
 {
     // the tile that holds twice an average group's rows, since groups are uneven; without offsets the one that holds them all
     const long long rows = g.offsets == nullptr ? g.rows : 2ll * g.rows / g.groups;
     const int tn = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     // offsets may leave out rows and make up to min(groups, rows) short tiles
     const long long tiles = g.offsets == nullptr ? (g.rows + tn - 1) / tn : std::min(g.groups, g.rows) + g.rows / tn;
+    p.tiles_n = tn == 256 ? (g.n + 2 * kTileN - 1) / (2 * kTileN) : (g.n + kTileN - 1) / kTileN;
+    p.idesc = make_idesc(g.ab_dtype == KUDNN_B200_BF16 ? KUDNN_B200_BF16 : KUDNN_B200_F16, 0, tn == 256 ? 2 * kTileN : kTileN);  // e4m3 and fp16: code 0
     const long long bound = tiles * p.tiles_n;
     switch (tn) {
-        case 32: return launch_shape<kScaled, 32>(g, p, bound, sm_count, ta, tb, stream);
-        case 64: return launch_shape<kScaled, 64>(g, p, bound, sm_count, ta, tb, stream);
-        case 128: return launch_shape<kScaled, 128>(g, p, bound, sm_count, ta, tb, stream);
-        default: return launch_shape<kScaled, 256>(g, p, bound, sm_count, ta, tb, stream);
+        case 32: return launch_shape<kScaled, 32>(g, p, bound, sm_count, tb, stream);
+        case 64: return launch_shape<kScaled, 64>(g, p, bound, sm_count, tb, stream);
+        case 128: return launch_shape<kScaled, 128>(g, p, bound, sm_count, tb, stream);
+        default: return launch_shape<kScaled, 256>(g, p, bound, sm_count, tb, stream);
     }
 }
 
@@ -94,11 +106,8 @@ cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus
     const bool scaled = g.ab_dtype == KUDNN_B200_E4M3;
     const int es = scaled ? 1 : 2, c_size = dtype_size(g.c_dtype);
     const long long ld_b = pitch_of(g.n, g.b_sn, g.k, es);
-    CUtensorMap ta, tb;
-    cudaError_t e = tc_encode_groups(&ta, g.a, g.ab_dtype, 1, g.rows, g.k, pitch_of(1, 0, g.k, es), pitch_of(g.rows, g.a_sm, g.k, es), kBoxRows);
-    if (e == cudaSuccess) {
-        e = tc_encode_groups(&tb, g.b, g.ab_dtype, g.groups, g.n, g.k, g.groups > 1 ? g.b_sg : pitch_of(1, 0, g.k, es), ld_b, kTileN);
-    }
+    CUtensorMap tb;
+    const cudaError_t e = tc_encode_groups(&tb, g.b, g.ab_dtype, g.groups, g.n, g.k, g.groups > 1 ? g.b_sg : pitch_of(1, 0, g.k, es), ld_b, kTileN);
     if (e != cudaSuccess) {
         return e;
     }
@@ -106,14 +115,14 @@ cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus
     p.g = g;
     p.kb_elems = 128 / es;
     p.num_kb = (g.k + p.kb_elems - 1) / p.kb_elems;
-    p.tiles_n = (g.n + kTileN - 1) / kTileN;
     p.band = 8;
-    p.vec = (g.c_sn == 1 || g.n == 1) && (g.rows == 1 || g.c_sm * c_size % 16 == 0) && (reinterpret_cast<uintptr_t>(g.c) & 15u) == 0 ? 1 : 0;
-    p.idesc = make_idesc(g.ab_dtype == KUDNN_B200_BF16 ? KUDNN_B200_BF16 : KUDNN_B200_F16, 0, kTileN);  // e4m3 and fp16 have the same code, 0
+    const bool short_act = g.act == KUDNN_B200_ACT_NONE || g.act == KUDNN_B200_ACT_RELU || g.act == KUDNN_B200_ACT_SWISH ||
+                           (g.act == KUDNN_B200_ACT_GELU_TANH && g.c_dtype != KUDNN_B200_F32);
+    p.vec = short_act && (g.c_sn == 1 || g.n == 1) && (g.rows == 1 || g.c_sm % 4 == 0) && reinterpret_cast<uintptr_t>(g.c) % (4 * c_size) == 0 ? 1 : 0;
     p.load_kb = skip_kblock >= 0 ? std::min(skip_kblock, p.num_kb) : p.num_kb;
     p.status = status;
     p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimitCycles;
-    return scaled ? launch_kind<true>(g, p, sm_count, ta, tb, stream) : launch_kind<false>(g, p, sm_count, ta, tb, stream);
+    return scaled ? launch_kind<true>(g, p, sm_count, tb, stream) : launch_kind<false>(g, p, sm_count, tb, stream);
 }
 
 }  // namespace kb

@@ -4,19 +4,26 @@
 // a group pads its last tile to 16 rows instead of 128, its weights are read once for as many rows as fit (few rows: bound by the
 // weights' bytes; many: by the tensor pipe), and 128 weight rows share one scale per block of K.
 //
+// Tiles of 256 rows run on CTA pairs (cta_group::2, 256 weight rows, each CTA loads 128 of them and half of the group's rows): a CTA
+// alone would need 48 KiB per block of K, a pair needs 32, and 148 SMs that take 48 KiB every 512 cycles are more than L2 delivers.
+//
 // Roles (384 threads): warp 0 loads (TMA), warp 1 issues MMAs, warp 2 fetches the scales, warps 4-11 take the accumulators: a warp
 // owns 32 TMEM lanes (weight rows) and every other chunk of columns (rows of the group).  CTAs are persistent; work item = (group, rows
-// tile, 128 weight rows), found by a search in the groups' running item counts, which every CTA builds from the offsets.
+// tile, weight rows), found by a search in the groups' running item counts, which every CTA builds from the offsets.
 //
 // Scales.  The accumulator of a block of 128 k leaves tensor memory by itself (two to four buffers take turns) and is added to fp32
-// registers with the product of its scales, two elements per fma.rn.f32x2.  Tensor memory is read as 16 lanes x 256 bits, so that a thread
-// holds few columns (2 of 8) of many rows and needs few scales: two columns' scales serve 4 rows, one 16-byte read of shared memory 16 FMAs.
+// registers with the product of its scales.  Tensor memory is read as 16 lanes x 128 bits, so that a thread holds every fourth column and
+// needs a fourth of the scales: one 16-byte read of shared memory serves 16 FMAs.  Measured alone, cycles per 128 x 256 accumulator,
+// loads and FMAs of 8 warps: 16 x 128 bits 494, 16 x 256 bits 659 (its loads alone 377, against 269), 32 x 32 bits with every column's
+// scale read by every thread 589; the MMAs of a block take 512.
 //
 // Few items: clusters of up to 8 CTAs cut K, exchange their partial sums through distributed shared memory and add them in rank order.
 #pragma once
 
 #include "grouped.cuh"
 #include "sm100_ptx.cuh"
+
+#include <type_traits>
 
 namespace kb {
 
@@ -26,11 +33,10 @@ constexpr int kThreads = 384;
 constexpr int kSumWarps = 8;
 constexpr int kTileN = 128;             // weight rows per CTA
 constexpr int kWeightBytes = kTileN * 128;
-constexpr int kBoxRows = 32;            // rows of a per copy
 constexpr int kMaxStages = 12;
 constexpr int kMaxBuffers = 4;
 constexpr int kScaleSlots = 8;
-constexpr int kUnitPitch = 36;          // floats between the columns of a staged unit of 16 columns x 32 rows: conflict-free both ways
+constexpr int kUnitPitch = 40;          // floats between the columns of a staged unit of 16 columns x 32 rows: conflict-free both ways
 constexpr int kUnitBytes = 16 * kUnitPitch * 4;
 constexpr int kSmemLimit = 232448;
 // registers per thread where a warp's sums take 128 of them: 4 control warps and 8 that sum share what the launch has, 168 each
@@ -40,11 +46,15 @@ constexpr int kBarrierBytes = (2 * kMaxStages + 2 * kMaxBuffers + 2 * kScaleSlot
 
 template <bool kScaled, int kTN>
 struct Shape {
+    static constexpr bool kPair = kTN == 256;
     static constexpr int kBuffers = kScaled ? (kTN == 256 ? 2 : 4) : 2;
     static constexpr int kTmemCols = kBuffers * kTN;
+    static constexpr int kRound = kPair ? 32 : 16;            // N of an MMA is a multiple of this
+    static constexpr int kLoadRows = kPair ? kTN / 2 : kTN;   // rows of a that one CTA loads, at most
+    static constexpr int kBoxRows = kTN >= 128 ? 64 : 32;     // of them in one copy
     static constexpr int kChunk = kTN >= 128 ? 32 : 16;       // columns a warp takes at a time; the two warps of a lane quarter take turns
     static constexpr int kChunks = kTN / kChunk / 2;          // per warp
-    static constexpr int kStageBytes = kWeightBytes + kTN * 128;
+    static constexpr int kStageBytes = kWeightBytes + kLoadRows * 128;
     static constexpr bool kSplits = kTN <= 64;                // whether launches may cut K (the partial sums have to fit)
     static constexpr int kUnits = kSplits && kTN / 16 * 4 > kSumWarps ? kTN / 16 * 4 : kSumWarps;
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kTN * 4 : 0;
@@ -55,11 +65,11 @@ struct TcParams {
     GroupedParams g;
     int num_kb;        // blocks of 128 bytes of K
     int kb_elems;      // elements in one
-    int tiles_n;
+    int tiles_n;       // of 128 weight rows, 256 for pairs
     int splits, kb_per_split;
     int stages;
     int band;          // row tiles that share the weight tiles of a raster band
-    int vec;           // rows of c begin on 16-byte boundaries and are contiguous
+    int vec;           // rows of c are contiguous, four of their elements aligned, and finish_unit knows the activation
     unsigned idesc;    // without N
     int load_kb;       // k-blocks from this one on are not loaded (test hook)
     DeviceStatus *status;
@@ -67,7 +77,7 @@ struct TcParams {
 };
 
 struct Item {
-    int group, row0, count, cols, n0;  // cols: count rounded up to 16
+    int group, row0, count, cols, n0;  // cols: count rounded up to what an MMA takes
 };
 
 template <int kTN>
@@ -84,46 +94,69 @@ __device__ __forceinline__ Item find_item(const TcParams &p, const int *begins, 
     }
     const int local = item - items[lo], begin = begins[lo], rows = begins[lo + 1] - begin;
     const int tiles = (rows + kTN - 1) / kTN;
-    const int tall = ((rows + tiles - 1) / tiles + 15) & ~15;  // rows of a tile: the group cut evenly
+    constexpr int kRound = Shape<false, kTN>::kRound;
+    const int tall = ((rows + tiles - 1) / tiles + kRound - 1) / kRound * kRound;  // rows of a tile: the group cut evenly
     const int per_band = p.band * p.tiles_n;
     const int first = local / per_band * p.band;
     const int wide = tiles - first < p.band ? tiles - first : p.band;
     const int in_band = local % per_band;
     Item w;
     w.group = lo;
-    w.n0 = in_band / wide * kTileN;
+    w.n0 = in_band / wide * (Shape<false, kTN>::kPair ? 2 * kTileN : kTileN);
     w.row0 = begin + (first + in_band % wide) * tall;
     const int left = begin + rows - w.row0;
     w.count = left < tall ? left : tall;
-    w.cols = (w.count + 15) & ~15;
+    w.cols = (w.count + kRound - 1) / kRound * kRound;
     return w;
 }
 
+template <bool kPair>
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
 {
+    if (kPair) {
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+            "}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+            "}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+
+// Tile load of one CTA of a pair into its own shared memory, counted on the leader's barrier (a cluster address).
+__device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorMap *tmap, uint32_t leader_bar, int x, int y, int z)
+{
     asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-        "}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(smem_dst)),
+        "l"(tmap), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
-// 16 lanes x 32 columns: registers 4g + 2h + e hold lane (thread / 4) + 8h, column 8g + 2 (thread % 4) + e
-__device__ __forceinline__ void tmem_load_16x32(uint32_t taddr, uint32_t (&r)[16])
+// 16 lanes x 32 columns: register 2j + h holds lane (thread / 4) + 8h, column 4j + thread % 4
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16])
 {
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        "tcgen05.ld.sync.aligned.16x128b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 // the same, 16 columns
-__device__ __forceinline__ void tmem_load_16x16(uint32_t taddr, uint32_t (&r)[8])
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[8])
 {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
@@ -139,35 +172,7 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[8])
 {
     tmem_load_wait(r);
 }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16])
-{
-    tmem_load_16x32(taddr, r);
-}
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[8])
-{
-    tmem_load_16x16(taddr, r);
-}
 
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi)
-{
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ void load_shared_2x64(uint32_t at, uint64_t &a, uint64_t &b)
-{
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(at));
-}
 __device__ __forceinline__ void load_shared_4(uint32_t at, float *v)
 {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at));
@@ -175,6 +180,30 @@ __device__ __forceinline__ void load_shared_4(uint32_t at, float *v)
 __device__ __forceinline__ void store_shared(uint32_t at, float v)
 {
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// A wait of a whole warp, which gets one answer.  The first look is apart from the bounded loop: an arrival that is there already, the
+// usual case, costs one round trip to shared memory, and several looks that are asked for together cost one.
+__device__ __forceinline__ bool warp_wait(bool there, uint64_t *bar, uint32_t parity, volatile int *abort_flag, DeviceStatus *status, int where,
+                                          long long limit)
+{
+    if (__all_sync(0xffffffffu, there)) {
+        return true;
+    }
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where, limit));
+}
+
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(p));
+    return p != 0u;
 }
 
 __device__ __forceinline__ void cluster_barrier()
@@ -189,89 +218,89 @@ __device__ __forceinline__ uint32_t cluster_rank()
     return r;
 }
 
-template <bool kPrecise>
-__device__ __forceinline__ void activate(float (&v)[8], int act, float alpha)
+template <int kAct, bool kPrecise>
+__device__ __forceinline__ void activate(float (&v)[4][4], float alpha)
 {
-    switch (act) {
-        case KUDNN_B200_ACT_NONE:
-            break;
-        case KUDNN_B200_ACT_RELU:
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = activation<kPrecise>(v[i], KUDNN_B200_ACT_RELU, alpha);
-            }
-            break;
-        case KUDNN_B200_ACT_SWISH:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = activation<kPrecise>(v[i], KUDNN_B200_ACT_SWISH, alpha);
-            }
-            break;
-        case KUDNN_B200_ACT_GELU_TANH:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = kPrecise ? activation<true>(v[i], KUDNN_B200_ACT_GELU_TANH, alpha) : gelu_tanh_sigmoid(v[i]);
-            }
-            break;
-        default:
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-                const float x = i < 4 ? (i < 2 ? (i == 0 ? v[0] : v[1]) : (i == 2 ? v[2] : v[3])) : (i < 6 ? (i == 4 ? v[4] : v[5]) : (i == 6 ? v[6] : v[7]));
-                const float y = activation_any(x, act, alpha, kPrecise ? 1 : 0);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[j] = i == j ? y : v[j];
-                }
-            }
-            break;
+    for (int i = 0; i < 16; ++i) {
+        float &x = v[i / 4][i % 4];
+        x = kAct == KUDNN_B200_ACT_GELU_TANH && !kPrecise ? gelu_tanh_sigmoid(x) : activation<kPrecise>(x, kAct, alpha);
     }
 }
 
-// Eight neighbouring results of one row of c: bias, activation, rounding, store.
-__device__ __forceinline__ void finish_8(const TcParams &p, int row, int n, float (&v)[8], uint32_t bias_at)
+// A staged unit: 16 rows of c x 32 neighbouring columns, the rows kUnitPitch floats apart.  finish_unit takes it where the columns are
+// inside of c, aligned and contiguous and the activation is a short one: a lane takes 4 columns of every fourth row, straight
+// through.  finish_unit_any takes the rest, element by element.  The epilogues of a tile are one loop over its units with one copy of this
+// code: unrolled, with the cases inside, a tile of 128 x 256 took 27 thousand cycles to finish.
+__device__ __forceinline__ void finish_unit(const GroupedParams &g, int row0, int count, int n, const float (&bias)[4], float (&v)[4][4], int lane)
 {
-    const GroupedParams &g = p.g;
-    if (g.has_bias != 0) {
-        float b[8];
-        load_shared_4(bias_at, b);
-        load_shared_4(bias_at + 16, b + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] += b[i];
-        }
+    for (int i = 0; i < 16; ++i) {
+        v[i / 4][i % 4] += bias[i % 4];
     }
-    if (g.c_dtype == KUDNN_B200_F32) {
-        activate<true>(v, g.act, g.act_alpha);
-    } else {
-        activate<false>(v, g.act, g.act_alpha);
-    }
-    const long long at = row * g.c_sm + n * g.c_sn;
-    if (p.vec != 0 && n + 8 <= g.n) {
-        if (g.c_dtype == KUDNN_B200_F32) {
-            float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(g.c) + at);
-            to[0] = make_float4(v[0], v[1], v[2], v[3]);
-            to[1] = make_float4(v[4], v[5], v[6], v[7]);
+    const bool precise = g.c_dtype == KUDNN_B200_F32;
+    if (g.act != KUDNN_B200_ACT_NONE) {
+        if (g.act == KUDNN_B200_ACT_RELU) {
+            activate<KUDNN_B200_ACT_RELU, true>(v, g.act_alpha);
+        } else if (g.act == KUDNN_B200_ACT_GELU_TANH) {
+            activate<KUDNN_B200_ACT_GELU_TANH, false>(v, g.act_alpha);
+        } else if (precise) {
+            activate<KUDNN_B200_ACT_SWISH, true>(v, g.act_alpha);
         } else {
-            uint32_t w[4];
+            activate<KUDNN_B200_ACT_SWISH, false>(v, g.act_alpha);
+        }
+    }
+    const int first = lane / 8;
+    char *to = static_cast<char *>(g.c) + ((row0 + first) * g.c_sm + n) * (precise ? 4 : 2);
+    const long long step = 4 * g.c_sm * (precise ? 4 : 2);
+    if (precise) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (g.c_dtype == KUDNN_B200_F16) {
-                    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                } else {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                }
+        for (int i = 0; i < 4; ++i) {
+            if (first + 4 * i < count) {
+                *reinterpret_cast<float4 *>(to + i * step) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
             }
-            *reinterpret_cast<uint4 *>(static_cast<unsigned short *>(g.c) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return;
+    }
+    uint2 w[4];
+    if (g.c_dtype == KUDNN_B200_F16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 lo = __floats2half2_rn(v[i][0], v[i][1]), hi = __floats2half2_rn(v[i][2], v[i][3]);
+            w[i] = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (n + i < g.n) {
-                store_exact(g.c, g.c_dtype, at + i * g.c_sn, round_rne(v[i], g.c_dtype));
-            }
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(v[i][0], v[i][1]), hi = __floats2bfloat162_rn(v[i][2], v[i][3]);
+            w[i] = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (first + 4 * i < count) {
+            *reinterpret_cast<uint2 *>(to + i * step) = w[i];
+        }
+    }
+}
+
+// bias_at: 32 floats of shared memory
+static __device__ __noinline__ void finish_unit_any(const GroupedParams &g, int row0, int count, int n0, uint32_t bias_at, uint32_t unit_at, int lane)
+{
+    if (n0 + lane >= g.n) {
+        return;
+    }
+    float bias;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(bias) : "r"(bias_at + static_cast<uint32_t>(lane * 4)));
+#pragma unroll 1
+    for (int r = 0; r < 16 && r < count; ++r) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(unit_at + static_cast<uint32_t>((r * kUnitPitch + lane) * 4)));
+        v += bias;
+        if (g.act != KUDNN_B200_ACT_NONE) {
+            v = activation_any(v, g.act, g.act_alpha, g.c_dtype == KUDNN_B200_F32 ? 1 : 0);
+        }
+        store_exact(g.c, g.c_dtype, (row0 + r) * g.c_sm + (n0 + lane) * g.c_sn, round_rne(v, g.c_dtype));
     }
 }
 
@@ -296,7 +325,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int *begins = reinterpret_cast<int *>(tmem_slot + 4);  // first row of each group, then the end of the last
     int *items = begins + p.g.groups + 1;                  // work items before each group, then all
 
-    const int warp = threadIdx.x >> 5;
+    // (from a shuffle, so that the compiler knows it to be the same in all lanes and keeps the roles' addresses in uniform registers)
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     if ((smem_u32(smem) & 1023u) != 0) {  // never: the declaration asks for the alignment
         if (threadIdx.x == 0) {
@@ -311,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < kMaxBuffers; ++s) {
             mbar_init(tmem_full + s, 1);
-            mbar_init(tmem_empty + s, kSumWarps);
+            mbar_init(tmem_empty + s, S::kPair ? 2 * kSumWarps : kSumWarps);  // pair: the sums of both CTAs
         }
         for (int s = 0; s < kScaleSlots; ++s) {
             mbar_init(scale_full + s, 1);
@@ -322,9 +352,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(S::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (S::kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(S::kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(S::kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     if (warp == 0 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_a) : "memory");
@@ -332,6 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if (S::kPair) {
+        cluster_barrier();  // the peer's barriers are initialised before anything is signalled on them
+    }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     pdl_launch_dependents();  // only now that this CTA holds its tensor memory
@@ -380,12 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     const int num_items = items[p.g.groups];
-    const int first_item = p.splits > 1 ? static_cast<int>(blockIdx.x) / p.splits : static_cast<int>(blockIdx.x);
+    const int rank = S::kPair || p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
     // launches that cut K have a cluster for every item that there can be
-    const int stride = p.splits > 1 ? num_items + 1 : static_cast<int>(gridDim.x);
-    const int rank = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int kb_begin = rank * p.kb_per_split;
+    const int first_item = S::kPair ? static_cast<int>(blockIdx.x >> 1) : p.splits > 1 ? static_cast<int>(blockIdx.x) / p.splits : static_cast<int>(blockIdx.x);
+    const int stride = S::kPair ? static_cast<int>(gridDim.x >> 1) : p.splits > 1 ? num_items + 1 : static_cast<int>(gridDim.x);
+    const int kb_begin = S::kPair ? 0 : rank * p.kb_per_split;
     const int kb_end = kb_begin + p.kb_per_split < p.num_kb ? kb_begin + p.kb_per_split : p.num_kb;
+    const int my_n = S::kPair ? rank * kTileN : 0;  // of a pair's 256 weight rows, the CTA's begin here
 
     // rows that no group holds
     const int outside_first = begins[0], outside = p.g.rows - (begins[p.g.groups] - begins[0]);
@@ -401,48 +441,66 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (kScaled && kTN == 256) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
         }
-        if (warp == 0 && lane == 0) {
+        // The whole warp runs a role's loop and one lane issues: what an instruction needs then lies in uniform registers.
+        if (warp == 0) {
             // ------------------------------------------------------------------ loads
             int stage = 0;
             uint32_t phase = 0;
             bool alive = true;
             for (int item = first_item; alive && item < num_items; item += stride) {
                 const Item w = find_item<kTN>(p, begins, items, item);
-                const int boxes = (w.cols + kBoxRows - 1) / kBoxRows;
-                const uint32_t bytes = static_cast<uint32_t>(kWeightBytes + boxes * kBoxRows * 128);
+                const int mine = S::kPair ? w.cols / 2 : w.cols, row0 = w.row0 + (S::kPair ? rank * mine : 0);
+                const int boxes = (mine + S::kBoxRows - 1) / S::kBoxRows;
+                const uint32_t bytes = static_cast<uint32_t>(kWeightBytes + boxes * S::kBoxRows * 128) * (S::kPair ? 2u : 1u);
                 const int end = kb_end < p.load_kb ? kb_end : p.load_kb;
                 for (int kb = kb_begin; kb < end; ++kb) {
-                    if (!mbar_wait(empty_bar + stage, phase ^ 1u, abort_flag, p.status, 1, p.wait_limit)) {
-                        alive = false;
+                    alive = warp_wait(mbar_try_wait(empty_bar + stage, phase ^ 1u), empty_bar + stage, phase ^ 1u, abort_flag, p.status, 1, p.wait_limit);
+                    if (!alive) {
                         break;
                     }
                     unsigned char *at = smem + stage * S::kStageBytes;
                     const int x = kb * p.kb_elems;
-                    mbar_expect_tx(full_bar + stage, bytes);
-                    tma_load_3d(at, &tmap_b, full_bar + stage, x, w.n0, w.group);
-                    for (int i = 0; i < boxes; ++i) {
-                        tma_load_3d(at + kWeightBytes + i * kBoxRows * 128, &tmap_a, full_bar + stage, x, w.row0 + i * kBoxRows, 0);
+                    if (elect_one()) {
+                        if (S::kPair) {
+                            // the leader's barriers count both CTAs' bytes; only the leader announces them
+                            const uint32_t bar = map_to_rank(smem_u32(full_bar + stage), 0u);
+                            if (rank == 0) {
+                                mbar_expect_tx(full_bar + stage, bytes);
+                            }
+                            tma_load_3d_pair(at, &tmap_b, bar, x, w.n0 + my_n, w.group);
+                            for (int i = 0; i < boxes; ++i) {
+                                tma_load_3d_pair(at + kWeightBytes + i * S::kBoxRows * 128, &tmap_a, bar, x, row0 + i * S::kBoxRows, 0);
+                            }
+                        } else {
+                            mbar_expect_tx(full_bar + stage, bytes);
+                            tma_load_3d(at, &tmap_b, full_bar + stage, x, w.n0, w.group);
+                            for (int i = 0; i < boxes; ++i) {
+                                tma_load_3d(at + kWeightBytes + i * S::kBoxRows * 128, &tmap_a, full_bar + stage, x, row0 + i * S::kBoxRows, 0);
+                            }
+                        }
                     }
+                    __syncwarp();
                     if (++stage == p.stages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
-        } else if (warp == 1 && lane == 0) {
-            // ------------------------------------------------------------------ MMAs
+        } else if (warp == 1 && (!S::kPair || rank == 0)) {
+            // ------------------------------------------------------------------ MMAs, of a pair by its leader
             int stage = 0, buffer = 0;
             uint32_t phase = 0, buffer_phase = 0;
             bool alive = true;
+            bool loaded = mbar_try_wait(full_bar, 0);  // looked up one k-block ahead, so that the answer is there when it is needed
             for (int item = first_item; alive && item < num_items; item += stride) {
                 const Item w = find_item<kTN>(p, begins, items, item);
                 const uint32_t idesc = p.idesc | static_cast<uint32_t>(w.cols >> 3) << 17;
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
                     if (kScaled || kb == kb_begin) {
-                        alive = mbar_wait(tmem_empty + buffer, buffer_phase ^ 1u, abort_flag, p.status, 2, p.wait_limit);
-                        tc_fence_after();
+                        alive = warp_wait(mbar_try_wait(tmem_empty + buffer, buffer_phase ^ 1u), tmem_empty + buffer, buffer_phase ^ 1u, abort_flag,
+                                          p.status, 2, p.wait_limit);
                     }
-                    alive = alive && mbar_wait(full_bar + stage, phase, abort_flag, p.status, 3, p.wait_limit);
+                    alive = alive && warp_wait(loaded, full_bar + stage, phase, abort_flag, p.status, 3, p.wait_limit);
                     if (!alive) {
                         break;
                     }
@@ -450,26 +508,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(stage * S::kStageBytes);
                     const uint64_t wdesc = make_smem_desc(at), xdesc = make_smem_desc(at + kWeightBytes);
                     const uint32_t to = tmem_base + static_cast<uint32_t>(buffer * kTN);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint64_t d = static_cast<uint64_t>(2 * ks);
-                        if (kScaled) {
-                            umma_f8(to, wdesc + d, xdesc + d, idesc, ks != 0 ? 1u : 0u);
-                        } else {
-                            umma<KUDNN_B200_F16>(to, wdesc + d, xdesc + d, idesc, kb != kb_begin || ks != 0 ? 1u : 0u);
-                        }
-                    }
-                    umma_commit(empty_bar + stage);
+                    const bool whole = kScaled || kb + 1 == kb_end;  // the buffer is complete
+                    const int this_stage = stage;
                     if (++stage == p.stages) {
                         stage = 0;
                         phase ^= 1u;
                     }
-                    if (kScaled || kb + 1 == kb_end) {
-                        umma_commit(tmem_full + buffer);
-                        if (++buffer == S::kBuffers) {
-                            buffer = 0;
-                            buffer_phase ^= 1u;
+                    loaded = mbar_try_wait(full_bar + stage, phase);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint64_t d = static_cast<uint64_t>(2 * ks);
+                            const uint32_t more = ks != 0 || (!kScaled && kb != kb_begin) ? 1u : 0u;
+                            if (kScaled) {
+                                umma_f8<S::kPair>(to, wdesc + d, xdesc + d, idesc, more);
+                            } else if (S::kPair) {
+                                umma_pair<KUDNN_B200_F16>(to, wdesc + d, xdesc + d, idesc, more);
+                            } else {
+                                umma<KUDNN_B200_F16>(to, wdesc + d, xdesc + d, idesc, more);
+                            }
                         }
+                        if (S::kPair) {
+                            umma_commit_pair(empty_bar + this_stage);
+                            if (whole) {
+                                umma_commit_pair(tmem_full + buffer);
+                            }
+                        } else {
+                            umma_commit(empty_bar + this_stage);
+                            if (whole) {
+                                umma_commit(tmem_full + buffer);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (whole && ++buffer == S::kBuffers) {
+                        buffer = 0;
+                        buffer_phase ^= 1u;
                     }
                 }
             }
@@ -482,7 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int item = first_item; alive && item < num_items; item += stride) {
                 const Item w = find_item<kTN>(p, begins, items, item);
                 const float *sa = p.g.a_scale + w.row0 * p.g.as_sm;
-                const float *sb = p.g.b_scale + w.group * p.g.bs_sg + w.n0 / kScaleBlock * p.g.bs_sn;
+                const bool held = w.n0 + my_n < p.g.n;  // else this CTA of the pair has no weights
+                const float *sb = p.g.b_scale + w.group * p.g.bs_sg + (held ? (w.n0 + my_n) / kScaleBlock : 0) * p.g.bs_sn;
                 for (int kb0 = kb_begin; alive && kb0 < kb_end; kb0 += kAhead) {
                     float s[kAhead][kPer], t[kAhead];
 #pragma unroll
@@ -498,13 +573,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < kAhead; ++i) {
                         if (alive && kb0 + i < kb_end) {
-                            alive = __all_sync(0xffffffffu, mbar_wait(scale_empty + slot, phase ^ 1u, abort_flag, p.status, 5, p.wait_limit));
+                            alive = warp_wait(mbar_try_wait(scale_empty + slot, phase ^ 1u), scale_empty + slot, phase ^ 1u, abort_flag, p.status, 5,
+                                              p.wait_limit);
                             const uint32_t at = smem_u32(scales) + static_cast<uint32_t>(slot * kTN * 4);
 #pragma unroll
                             for (int j = 0; j < kPer; ++j) {
-                                // column 16u + 8g + 2q + e goes to 16u + 4q + 2g + e, so that a thread's two pairs of a unit are 16 bytes
+                                // column 16u + 4j + q goes to 16u + 4q + j: the columns of a thread lie next to one another
                                 const uint32_t c = static_cast<uint32_t>(j * 32 + lane);
-                                const uint32_t to = (c & ~15u) | (c & 6u) << 1 | (c & 8u) >> 2 | (c & 1u);
+                                const uint32_t to = (c & ~15u) | (c & 3u) << 2 | (c & 12u) >> 2;
                                 store_shared(at + to * 4, s[i][j] * t[i]);
                             }
                             __syncwarp();
@@ -525,34 +601,52 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         }
         // ---------------------------------------------------------------------- sums and results
-        constexpr int kRegs = S::kChunk / 2;  // 32-bit registers of 16 lanes x a chunk of columns
+        constexpr int kRegs = S::kChunk / 2;  // registers of 16 lanes x a chunk of columns
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t my_bias = smem_u32(bias_area) + static_cast<uint32_t>((warp - 4) * 128);
         const uint32_t lanes_at = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t drained = S::kPair ? map_to_rank(smem_u32(tmem_empty), 0u) : 0u;
         int buffer = 0, slot = 0;
         uint32_t buffer_phase = 0, slot_phase = 0;
+        auto release = [&]() {  // the MMAs may have the buffer again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (S::kPair) {
+                    mbar_arrive_cluster(drained + static_cast<uint32_t>(buffer * 8));
+                } else {
+                    mbar_arrive(tmem_empty + buffer);
+                }
+            }
+            if (++buffer == S::kBuffers) {
+                buffer = 0;
+                buffer_phase ^= 1u;
+            }
+        };
         for (int item = first_item; item < num_items; item += stride) {
             const Item w = find_item<kTN>(p, begins, items, item);
-            const int n_warp = w.n0 + quarter * 32;
-            float bias = 0.0f;
+            const int n_warp = w.n0 + my_n + quarter * 32;
+            float bias_lane = 0.0f;
             if (p.g.has_bias != 0 && n_warp + lane < p.g.n) {
-                bias = load_as_f32(p.g.bias, p.g.bias_dtype, w.group * p.g.bias_sg + (n_warp + lane) * p.g.bias_sn);
+                bias_lane = load_as_f32(p.g.bias, p.g.bias_dtype, w.group * p.g.bias_sg + (n_warp + lane) * p.g.bias_sn);
             }
             bool alive = true;
-            uint64_t sum[S::kChunks][2][kRegs / 2];  // 16 lanes at a time; in pairs of neighbouring columns
+            float sum[kScaled ? S::kChunks : 1][2][kRegs];  // 16 lanes each
             if (kScaled) {
 #pragma unroll
                 for (int i = 0; i < S::kChunks; ++i) {
 #pragma unroll
-                    for (int j = 0; j < kRegs / 2; ++j) {
-                        sum[i][0][j] = 0;
-                        sum[i][1][j] = 0;
+                    for (int j = 0; j < kRegs; ++j) {
+                        sum[i][0][j] = 0.0f;
+                        sum[i][1][j] = 0.0f;
                     }
                 }
+#pragma unroll 1
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
-                    alive = mbar_wait(scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit) &&
-                            mbar_wait(tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
-                    alive = __all_sync(0xffffffffu, alive);
+                    const bool scales_there = mbar_try_wait(scale_full + slot, slot_phase);
+                    const bool sums_there = mbar_try_wait(tmem_full + buffer, buffer_phase);
+                    alive = warp_wait(scales_there, scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit) &&
+                            warp_wait(sums_there, tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
                     if (!alive) {
                         break;
                     }
@@ -562,33 +656,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < S::kChunks; ++i) {
                         const int c0 = (2 * i + half) * S::kChunk;
-                        if (c0 < w.cols) {
-                            uint32_t lo[kRegs], hi[kRegs];
-                            tmem_load(from + static_cast<uint32_t>(c0), lo);
-                            tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
-                            uint64_t s[S::kChunk / 8];
+                        if (c0 >= w.cols) {
+                            break;
+                        }
+                        uint32_t lo[kRegs], hi[kRegs];
+                        tmem_load(from + static_cast<uint32_t>(c0), lo);
+                        tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
+                        float s[S::kChunk / 4];
 #pragma unroll
-                            for (int u = 0; u < S::kChunk / 16; ++u) {
-                                load_shared_2x64(scale_at + static_cast<uint32_t>((c0 + u * 16) * 4), s[2 * u], s[2 * u + 1]);
-                            }
-                            tmem_wait(lo);
-                            tmem_wait(hi);
+                        for (int u = 0; u < S::kChunk / 16; ++u) {
+                            load_shared_4(scale_at + static_cast<uint32_t>((c0 + u * 16) * 4), s + 4 * u);
+                        }
+                        tmem_wait(lo);
+                        tmem_wait(hi);
 #pragma unroll
-                            for (int j = 0; j < kRegs / 2; ++j) {  // pair j: group of 8 columns j / 2, lane half j % 2
-                                sum[i][0][j] = fma2(pack2(lo[2 * j], lo[2 * j + 1]), s[j / 2], sum[i][0][j]);
-                                sum[i][1][j] = fma2(pack2(hi[2 * j], hi[2 * j + 1]), s[j / 2], sum[i][1][j]);
-                            }
+                        for (int j = 0; j < kRegs; ++j) {
+                            sum[i][0][j] = fmaf(__uint_as_float(lo[j]), s[j / 2], sum[i][0][j]);
+                            sum[i][1][j] = fmaf(__uint_as_float(hi[j]), s[j / 2], sum[i][1][j]);
                         }
                     }
-                    tc_fence_before();
-                    __syncwarp();
+                    release();
                     if (lane == 0) {
-                        mbar_arrive(tmem_empty + buffer);
                         mbar_arrive(scale_empty + slot);
-                    }
-                    if (++buffer == S::kBuffers) {
-                        buffer = 0;
-                        buffer_phase ^= 1u;
                     }
                     if (++slot == kScaleSlots) {
                         slot = 0;
@@ -596,72 +685,80 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             } else {
-                alive = __all_sync(0xffffffffu, mbar_wait(tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit));
+                alive = warp_wait(mbar_try_wait(tmem_full + buffer, buffer_phase), tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
                 tc_fence_after();
             }
             if (!alive) {
                 break;
             }
-            store_shared(my_bias + static_cast<uint32_t>(lane * 4), bias);
+            store_shared(my_bias + static_cast<uint32_t>(lane * 4), bias_lane);
+            __syncwarp();
+            float bias[4];
+            load_shared_4(my_bias + static_cast<uint32_t>((lane & 7) * 16), bias);
             const uint32_t from = tmem_base + lanes_at + static_cast<uint32_t>(buffer * kTN);
+            constexpr int kUnitsPerChunk = S::kChunk / 16;
+#pragma unroll 1
+            for (int u = 0; u < S::kChunks * kUnitsPerChunk; ++u) {
+                const int c0 = (2 * (u / kUnitsPerChunk) + half) * S::kChunk + u % kUnitsPerChunk * 16;
+                if (c0 >= w.cols) {
+                    break;
+                }
+                const int unit = p.splits > 1 ? c0 / 16 * 4 + quarter : warp - 4;
+                const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
+                // column 4j + lane % 4, row lane / 4 (+ 8 and 16)
+                const uint32_t put_at = unit_at + static_cast<uint32_t>(((lane & 3) * kUnitPitch + lane / 4) * 4);
+                if (kScaled) {
+                    __syncwarp();
+                    auto put = [&](auto which) {
+                        constexpr int v = decltype(which)::value;
+                        if constexpr (v < S::kChunks * kUnitsPerChunk) {
 #pragma unroll
-            for (int i = 0; i < S::kChunks; ++i) {
-                const int c0 = (2 * i + half) * S::kChunk;
-                if (c0 < w.cols) {
-                    if (!kScaled) {
-                        uint32_t lo[kRegs], hi[kRegs];
-                        tmem_load(from + static_cast<uint32_t>(c0), lo);
-                        tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
-                        tmem_wait(lo);
-                        tmem_wait(hi);
-#pragma unroll
-                        for (int j = 0; j < kRegs / 2; ++j) {
-                            sum[i][0][j] = pack2(lo[2 * j], lo[2 * j + 1]);
-                            sum[i][1][j] = pack2(hi[2 * j], hi[2 * j + 1]);
+                            for (int j = 0; j < 16; ++j) {  // j: lanes' half, column / 4, lanes' eight
+                                store_shared(put_at + static_cast<uint32_t>(((j >> 1 & 3) * 4 * kUnitPitch + (j >> 3) * 16 + (j & 1) * 8) * 4),
+                                             sum[v / kUnitsPerChunk][j >> 3][v % kUnitsPerChunk * 8 + (j & 7)]);
+                            }
                         }
+                    };
+                    switch (u) {  // the registers' numbers are fixed
+                        case 0: put(std::integral_constant<int, 0>()); break;
+                        case 1: put(std::integral_constant<int, 1>()); break;
+                        case 2: put(std::integral_constant<int, 2>()); break;
+                        case 3: put(std::integral_constant<int, 3>()); break;
+                        case 4: put(std::integral_constant<int, 4>()); break;
+                        case 5: put(std::integral_constant<int, 5>()); break;
+                        case 6: put(std::integral_constant<int, 6>()); break;
+                        default: put(std::integral_constant<int, 7>()); break;
                     }
+                } else {
+                    uint32_t lo[8], hi[8];
+                    tmem_load(from + static_cast<uint32_t>(c0), lo);
+                    tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
+                    tmem_wait(lo);
+                    tmem_wait(hi);
+                    __syncwarp();
 #pragma unroll
-                    for (int u = 0; u < S::kChunk / 16; ++u) {
-                        const int unit = p.splits > 1 ? (c0 / 16 + u) * 4 + quarter : warp - 4;
-                        const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
-                        __syncwarp();
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t to = put_at + static_cast<uint32_t>(((j >> 1) * 4 * kUnitPitch + (j & 1) * 8) * 4);
+                        store_shared(to, __uint_as_float(lo[j]));
+                        store_shared(to + 64, __uint_as_float(hi[j]));
+                    }
+                }
+                __syncwarp();
+                if (p.splits == 1) {
+                    if (p.vec != 0 && n_warp + 32 <= p.g.n) {
+                        float v[4][4];
 #pragma unroll
-                        for (int hl = 0; hl < 2; ++hl) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                float x, y;
-                                unpack2(sum[i][hl][4 * u + j], x, y);
-                                const int col = (j / 2) * 8 + 2 * (lane & 3), row = hl * 16 + (j & 1) * 8 + lane / 4;
-                                store_shared(unit_at + static_cast<uint32_t>((col * kUnitPitch + row) * 4), x);
-                                store_shared(unit_at + static_cast<uint32_t>(((col + 1) * kUnitPitch + row) * 4), y);
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            load_shared_4(unit_at + static_cast<uint32_t>(((lane / 8 + 4 * i) * kUnitPitch + (lane & 7) * 4) * 4), v[i]);
                         }
-                        __syncwarp();
-                        if (p.splits == 1) {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const int col = j * 8 + lane / 4, n8 = (lane & 3) * 8;
-                                float v[8];
-                                load_shared_4(unit_at + static_cast<uint32_t>((col * kUnitPitch + n8) * 4), v);
-                                load_shared_4(unit_at + static_cast<uint32_t>((col * kUnitPitch + n8 + 4) * 4), v + 4);
-                                if (c0 + u * 16 + col < w.count && n_warp + n8 < p.g.n) {
-                                    finish_8(p, w.row0 + c0 + u * 16 + col, n_warp + n8, v, my_bias + static_cast<uint32_t>(n8 * 4));
-                                }
-                            }
-                        }
+                        finish_unit(p.g, w.row0 + c0, w.count - c0, n_warp + (lane & 7) * 4, bias, v, lane);
+                    } else {
+                        finish_unit_any(p.g, w.row0 + c0, w.count - c0, n_warp, my_bias, unit_at, lane);
                     }
                 }
             }
             if (!kScaled) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(tmem_empty + buffer);
-                }
-                if (++buffer == S::kBuffers) {
-                    buffer = 0;
-                    buffer_phase ^= 1u;
-                }
+                release();
             }
         }
     }
@@ -671,32 +768,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         cluster_barrier();
         if (warp >= 4 && first_item < num_items && *abort_flag == 0) {
+            unsigned char *whole = smem;  // the ring's copies have all been consumed
             const Item w = find_item<kTN>(p, begins, items, first_item);
             for (int unit = rank + (warp - 4) * p.splits; unit < w.cols / 16 * 4; unit += kSumWarps * p.splits) {
-                const int c0 = unit / 4 * 16, quarter = unit & 3;
+                const int c0 = unit / 4 * 16, quarter = unit & 3, n0 = w.n0 + quarter * 32;
                 const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
+                float v[4][4] = {};
+                for (int r = 0; r < p.splits; ++r) {
+                    const uint32_t from = map_to_rank(unit_at + static_cast<uint32_t>((lane / 8 * kUnitPitch + (lane & 7) * 4) * 4), static_cast<uint32_t>(r));
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int col = j * 8 + lane / 4, n8 = (lane & 3) * 8, n = w.n0 + quarter * 32 + n8;
-                    if (c0 + col < w.count && n < p.g.n) {
-                        float v[8] = {};
-                        for (int r = 0; r < p.splits; ++r) {
-                            const uint32_t at = map_to_rank(unit_at + static_cast<uint32_t>((col * kUnitPitch + n8) * 4), static_cast<uint32_t>(r));
-                            float x[8];
-                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                         : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
-                                         : "r"(at));
-                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                         : "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
-                                         : "r"(at + 16));
+                    for (int i = 0; i < 4; ++i) {
+                        float x[4];
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                                     : "r"(from + static_cast<uint32_t>(4 * i * kUnitPitch * 4)));
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                v[i] += x[i];
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            v[i][j] += x[j];
                         }
-                        // the bias of this warp's own quarter lies in its area; another quarter's in the area of that quarter's warp
-                        finish_8(p, w.row0 + c0 + col, n, v, smem_u32(bias_area) + static_cast<uint32_t>(quarter * 128 + n8 * 4));
                     }
+                }
+                const uint32_t bias_at = smem_u32(bias_area) + static_cast<uint32_t>(quarter * 128);  // of the first warp that owns the quarter
+                if (p.vec != 0 && n0 + 32 <= p.g.n) {
+                    float bias[4];
+                    load_shared_4(bias_at + static_cast<uint32_t>((lane & 7) * 16), bias);
+                    finish_unit(p.g, w.row0 + c0, w.count - c0, n0 + (lane & 7) * 4, bias, v, lane);
+                } else {
+                    // not over the partial sums, which other CTAs may still have to read
+                    const uint32_t whole_at = smem_u32(whole) + static_cast<uint32_t>((warp - 4) * kUnitBytes);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                         whole_at + static_cast<uint32_t>(((lane / 8 + 4 * i) * kUnitPitch + (lane & 7) * 4) * 4)),
+                                     "f"(v[i][0]), "f"(v[i][1]), "f"(v[i][2]), "f"(v[i][3])
+                                     : "memory");
+                    }
+                    __syncwarp();
+                    finish_unit_any(p.g, w.row0 + c0, w.count - c0, n0, bias_at, whole_at, lane);
                 }
             }
         }
@@ -717,7 +826,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncthreads();
     }
-    if (warp == 1) {
+    if (S::kPair) {
+        cluster_barrier();  // neither CTA leaves while the other's MMAs or arrivals may still reach it
+    }
+    if (warp == 1 && S::kPair) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+    } else if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
     }
 }
