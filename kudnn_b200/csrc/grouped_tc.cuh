@@ -17,6 +17,11 @@
 // loads and FMAs of 8 warps: 16 x 128 bits 494, 16 x 256 bits 659 (its loads alone 377, against 269), 32 x 32 bits with every column's
 // scale read by every thread 589; the MMAs of a block take 512.
 //
+// Scaled products of tall tiles stand the other way round: rows on the M side, 256 weight rows on the N side.  A lane then holds a row
+// and a warp the columns of one scale, so that an accumulator element costs one FMA with a scalar of the thread (327 cycles per 128 x 256)
+// and rows are stored straight from registers; a group's last tile is padded to 256 rows instead of 32.  Measured in the kernel, cycles
+// per block of K: weights on the M side 1170, of which the sums 760.
+//
 // Few items: clusters of up to 8 CTAs cut K, exchange their partial sums through distributed shared memory and add them in rank order.
 #pragma once
 
@@ -44,8 +49,10 @@ constexpr int kControlRegs = 88, kSumRegs = 208;
 static_assert(128 * kControlRegs + 256 * kSumRegs <= kThreads * 168, "register split");
 constexpr int kBarrierBytes = (2 * kMaxStages + 2 * kMaxBuffers + 2 * kScaleSlots) * 8 + 16;
 
-template <bool kScaled, int kTN>
+// kRows: the rows of the group on the M side (see above)
+template <bool kScaled, int kTN, bool kRows>
 struct Shape {
+    static_assert(!kRows || (kScaled && kTN == 256), "rows on the M side: scaled products of tall tiles");
     static constexpr bool kPair = kTN == 256;
     static constexpr int kBuffers = kScaled ? (kTN == 256 ? 2 : 4) : 2;
     static constexpr int kTmemCols = kBuffers * kTN;
@@ -57,8 +64,9 @@ struct Shape {
     static constexpr int kStageBytes = kWeightBytes + kLoadRows * 128;
     static constexpr bool kSplits = kTN <= 64;                // whether launches may cut K (the partial sums have to fit)
     static constexpr int kUnits = kSplits && kTN / 16 * 4 > kSumWarps ? kTN / 16 * 4 : kSumWarps;
-    static constexpr int kScaleBytes = kScaled ? kScaleSlots * kTN * 4 : 0;
-    static constexpr int kFixedBytes = kUnits * kUnitBytes + kSumWarps * 128 + kScaleBytes + kBarrierBytes;
+    static constexpr int kScaleBytes = kScaled && !kRows ? kScaleSlots * kTN * 4 : 0;
+    static constexpr int kBiasBytes = kSumWarps * (kRows ? 512 : 128);
+    static constexpr int kFixedBytes = kUnits * kUnitBytes + kBiasBytes + kScaleBytes + kBarrierBytes;
 };
 
 struct TcParams {
@@ -77,10 +85,10 @@ struct TcParams {
 };
 
 struct Item {
-    int group, row0, count, cols, n0;  // cols: count rounded up to what an MMA takes
+    int group, row0, count, cols, n0;  // cols: N of the MMAs; count rounded up to what they take, or 256 weight rows
 };
 
-template <int kTN>
+template <int kTN, bool kRows>
 __device__ __forceinline__ Item find_item(const TcParams &p, const int *begins, const int *items, int item)
 {
     int lo = 0, hi = p.g.groups;
@@ -94,19 +102,20 @@ __device__ __forceinline__ Item find_item(const TcParams &p, const int *begins, 
     }
     const int local = item - items[lo], begin = begins[lo], rows = begins[lo + 1] - begin;
     const int tiles = (rows + kTN - 1) / kTN;
-    constexpr int kRound = Shape<false, kTN>::kRound;
-    const int tall = ((rows + tiles - 1) / tiles + kRound - 1) / kRound * kRound;  // rows of a tile: the group cut evenly
+    constexpr int kRound = kTN == 256 ? 32 : 16;
+    // rows of a tile: the group cut evenly, or what the M side holds
+    const int tall = kRows ? kTN : ((rows + tiles - 1) / tiles + kRound - 1) / kRound * kRound;
     const int per_band = p.band * p.tiles_n;
     const int first = local / per_band * p.band;
     const int wide = tiles - first < p.band ? tiles - first : p.band;
     const int in_band = local % per_band;
     Item w;
     w.group = lo;
-    w.n0 = in_band / wide * (Shape<false, kTN>::kPair ? 2 * kTileN : kTileN);
+    w.n0 = in_band / wide * (kTN == 256 ? 2 * kTileN : kTileN);
     w.row0 = begin + (first + in_band % wide) * tall;
     const int left = begin + rows - w.row0;
     w.count = left < tall ? left : tall;
-    w.cols = (w.count + kRound - 1) / kRound * kRound;
+    w.cols = kRows ? 256 : (w.count + kRound - 1) / kRound * kRound;
     return w;
 }
 
@@ -304,15 +313,246 @@ static __device__ __noinline__ void finish_unit_any(const GroupedParams &g, int 
     }
 }
 
-template <bool kScaled, int kTN>
+// ---- rows on the M side: a lane holds a row, and its 128 columns of a warp share one scale
+
+template <int kAct, bool kPrecise>
+__device__ __forceinline__ void activate_32(float *v, float alpha)
+{
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        v[i] = kAct == KUDNN_B200_ACT_GELU_TANH && !kPrecise ? gelu_tanh_sigmoid(v[i]) : activation<kPrecise>(v[i], kAct, alpha);
+    }
+}
+
+__device__ __forceinline__ void tmem_load_32x16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void store_32_bytes(void *to, const uint32_t *w)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// The scale of this lane's row times that of the warp's 128 weight rows, for one block of K; 0 where there is no such row or column.
+struct ScaleSource {
+    const float *row, *weights;
+    bool inside;
+};
+__device__ __forceinline__ ScaleSource scale_source(const GroupedParams &g, const Item &w, int row_in_tile, int n)
+{
+    ScaleSource s;
+    s.inside = row_in_tile < w.count && n < g.n;
+    s.row = g.a_scale + (s.inside ? (w.row0 + row_in_tile) * g.as_sm : 0);
+    s.weights = g.b_scale + w.group * g.bs_sg + (s.inside ? n / kScaleBlock * g.bs_sn : 0);
+    return s;
+}
+
+__device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, const int *items, int num_items, int first_item, int stride, int rank,
+                                         int warp, int lane, uint32_t tmem_base, uint64_t *tmem_full, uint64_t *tmem_empty, uint32_t units_at,
+                                         uint32_t bias_at, volatile int *abort_flag)
+{
+    constexpr int kBuffers = Shape<true, 256, true>::kBuffers;
+    const GroupedParams &g = p.g;
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int row_in_tile = rank * 128 + quarter * 32 + lane;
+    const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
+    const uint32_t drained = map_to_rank(smem_u32(tmem_empty), 0u);
+    const uint32_t my_unit = units_at + static_cast<uint32_t>((warp - 4) * kUnitBytes);
+    const uint32_t my_bias = bias_at + static_cast<uint32_t>((warp - 4) * 512);  // 128 floats
+    int buffer = 0;
+    uint32_t phase = 0;
+    Item w;
+    ScaleSource s;
+    float row_next = 0.0f, weights_next = 0.0f, row_after = 0.0f, weights_after = 0.0f;  // of the next two blocks
+    auto begin_item = [&](int item) {
+        w = find_item<256, true>(p, begins, items, item);
+        s = scale_source(g, w, row_in_tile, w.n0 + half * 128);
+        if (s.inside) {
+            row_next = s.row[0];
+            weights_next = s.weights[0];
+            if (p.num_kb > 1) {
+                row_after = s.row[g.as_sk];
+                weights_after = s.weights[g.bs_sk];
+            }
+        } else {
+            row_next = weights_next = row_after = weights_after = 0.0f;
+        }
+    };
+    if (first_item < num_items) {
+        begin_item(first_item);
+    }
+    for (int item = first_item; item < num_items; item += stride) {
+        const Item mine = w;
+        const int n_half = mine.n0 + half * 128;
+        float bias[4] = {};
+        if (g.has_bias != 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = n_half + i * 32 + lane;
+                bias[i] = n < g.n ? load_as_f32(g.bias, g.bias_dtype, mine.group * g.bias_sg + n * g.bias_sn) : 0.0f;
+            }
+        }
+        float sum[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) {
+            sum[j] = 0.0f;
+        }
+        bool alive = true;
+#pragma unroll 1
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+            const float scale = row_next * weights_next;
+            row_next = row_after;
+            weights_next = weights_after;
+            if (kb + 2 < p.num_kb && s.inside) {
+                row_after = s.row[(kb + 2) * g.as_sk];
+                weights_after = s.weights[(kb + 2) * g.bs_sk];
+            }
+            alive = warp_wait(mbar_try_wait(tmem_full + buffer, phase), tmem_full + buffer, phase, abort_flag, p.status, 4, p.wait_limit);
+            if (!alive) {
+                break;
+            }
+            tc_fence_after();
+            const uint32_t from = my_tmem + static_cast<uint32_t>(buffer * 256);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t a[16], b[16];
+                tmem_load_32x16(from + static_cast<uint32_t>(c * 32), a);
+                tmem_load_32x16(from + static_cast<uint32_t>(c * 32 + 16), b);
+                tmem_wait(a);
+                tmem_wait(b);
+                if (c == 3) {  // everything is in registers: the MMAs may have the buffer again
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive_cluster(drained + static_cast<uint32_t>(buffer * 8));
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    sum[c * 32 + j] = fmaf(__uint_as_float(a[j]), scale, sum[c * 32 + j]);
+                    sum[c * 32 + 16 + j] = fmaf(__uint_as_float(b[j]), scale, sum[c * 32 + 16 + j]);
+                }
+            }
+            if (++buffer == kBuffers) {
+                buffer = 0;
+                phase ^= 1u;
+            }
+        }
+        if (!alive) {
+            return;
+        }
+        if (item + stride < num_items) {
+            begin_item(item + stride);  // the next item's first scales are on their way while this one is finished
+        }
+        if (g.has_bias != 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                store_shared(my_bias + static_cast<uint32_t>((i * 32 + lane) * 4), bias[i]);
+            }
+            __syncwarp();
+        }
+        const int row = mine.row0 + row_in_tile;
+        const bool precise = g.c_dtype == KUDNN_B200_F32;
+#pragma unroll 1
+        for (int c0 = 0; c0 < 128 && n_half + c0 < g.n; c0 += 32) {
+            if (p.vec != 0 && n_half + c0 + 32 <= g.n) {
+                if (g.has_bias != 0) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        float b[4];
+                        load_shared_4(my_bias + static_cast<uint32_t>((c0 + j) * 4), b);
+                        sum[j] += b[0];
+                        sum[j + 1] += b[1];
+                        sum[j + 2] += b[2];
+                        sum[j + 3] += b[3];
+                    }
+                }
+                if (g.act != KUDNN_B200_ACT_NONE) {
+                    if (g.act == KUDNN_B200_ACT_RELU) {
+                        activate_32<KUDNN_B200_ACT_RELU, true>(sum, g.act_alpha);
+                    } else if (g.act == KUDNN_B200_ACT_GELU_TANH) {
+                        activate_32<KUDNN_B200_ACT_GELU_TANH, false>(sum, g.act_alpha);
+                    } else if (precise) {
+                        activate_32<KUDNN_B200_ACT_SWISH, true>(sum, g.act_alpha);
+                    } else {
+                        activate_32<KUDNN_B200_ACT_SWISH, false>(sum, g.act_alpha);
+                    }
+                }
+                if (row_in_tile < mine.count) {
+                    char *to = static_cast<char *>(g.c) + (row * g.c_sm + n_half + c0) * (precise ? 4 : 2);
+                    if (precise) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t v[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                v[j] = __float_as_uint(sum[i * 8 + j]);
+                            }
+                            store_32_bytes(to + i * 32, v);
+                        }
+                    } else {
+                        uint32_t v[16];
+                        if (g.c_dtype == KUDNN_B200_F16) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const __half2 h = __floats2half2_rn(sum[2 * j], sum[2 * j + 1]);
+                                v[j] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(sum[2 * j], sum[2 * j + 1]);
+                                v[j] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
+                        }
+                        store_32_bytes(to, v);
+                        store_32_bytes(to + 32, v + 8);
+                    }
+                }
+            } else {
+                if (g.has_bias == 0) {
+                    store_shared(my_bias + static_cast<uint32_t>((c0 + lane) * 4), 0.0f);
+                }
+                // 16 rows at a time through shared memory
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {
+                    __syncwarp();
+                    if (lane / 16 == part) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            store_shared(my_unit + static_cast<uint32_t>(((lane & 15) * kUnitPitch + j) * 4), sum[j]);
+                        }
+                    }
+                    __syncwarp();
+                    const int first = rank * 128 + quarter * 32 + part * 16;
+                    finish_unit_any(g, mine.row0 + first, mine.count - first, n_half + c0, my_bias + static_cast<uint32_t>(c0 * 4), my_unit, lane);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 96; ++j) {
+                sum[j] = sum[j + 32];
+            }
+        }
+        __syncwarp();
+    }
+}
+
+template <bool kScaled, int kTN, bool kRows>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ TcParams p)
 {
-    using S = Shape<kScaled, kTN>;
+    using S = Shape<kScaled, kTN, kRows>;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *units = smem + p.stages * S::kStageBytes;
     unsigned char *bias_area = units + S::kUnits * kUnitBytes;
-    unsigned char *scales = bias_area + kSumWarps * 128;
+    unsigned char *scales = bias_area + S::kBiasBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(scales + S::kScaleBytes);
     uint64_t *full_bar = bars;
     uint64_t *empty_bar = full_bar + kMaxStages;
@@ -448,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t phase = 0;
             bool alive = true;
             for (int item = first_item; alive && item < num_items; item += stride) {
-                const Item w = find_item<kTN>(p, begins, items, item);
+                const Item w = find_item<kTN, kRows>(p, begins, items, item);
                 const int mine = S::kPair ? w.cols / 2 : w.cols, row0 = w.row0 + (S::kPair ? rank * mine : 0);
                 const int boxes = (mine + S::kBoxRows - 1) / S::kBoxRows;
                 const uint32_t bytes = static_cast<uint32_t>(kWeightBytes + boxes * S::kBoxRows * 128) * (S::kPair ? 2u : 1u);
@@ -493,8 +733,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool alive = true;
             bool loaded = mbar_try_wait(full_bar, 0);  // looked up one k-block ahead, so that the answer is there when it is needed
             for (int item = first_item; alive && item < num_items; item += stride) {
-                const Item w = find_item<kTN>(p, begins, items, item);
-                const uint32_t idesc = p.idesc | static_cast<uint32_t>(w.cols >> 3) << 17;
+                const Item w = find_item<kTN, kRows>(p, begins, items, item);
+                const uint32_t idesc = p.idesc | (kRows ? 0u : static_cast<uint32_t>(w.cols >> 3) << 17);
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
                     if (kScaled || kb == kb_begin) {
                         alive = warp_wait(mbar_try_wait(tmem_empty + buffer, buffer_phase ^ 1u), tmem_empty + buffer, buffer_phase ^ 1u, abort_flag,
@@ -506,7 +746,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     tc_fence_after();
                     const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(stage * S::kStageBytes);
-                    const uint64_t wdesc = make_smem_desc(at), xdesc = make_smem_desc(at + kWeightBytes);
+                    const uint64_t first = make_smem_desc(at), second = make_smem_desc(at + kWeightBytes);
+                    const uint64_t mdesc = kRows ? second : first, ndesc = kRows ? first : second;
                     const uint32_t to = tmem_base + static_cast<uint32_t>(buffer * kTN);
                     const bool whole = kScaled || kb + 1 == kb_end;  // the buffer is complete
                     const int this_stage = stage;
@@ -521,11 +762,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint64_t d = static_cast<uint64_t>(2 * ks);
                             const uint32_t more = ks != 0 || (!kScaled && kb != kb_begin) ? 1u : 0u;
                             if (kScaled) {
-                                umma_f8<S::kPair>(to, wdesc + d, xdesc + d, idesc, more);
+                                umma_f8<S::kPair>(to, mdesc + d, ndesc + d, idesc, more);
                             } else if (S::kPair) {
-                                umma_pair<KUDNN_B200_F16>(to, wdesc + d, xdesc + d, idesc, more);
+                                umma_pair<KUDNN_B200_F16>(to, mdesc + d, ndesc + d, idesc, more);
                             } else {
-                                umma<KUDNN_B200_F16>(to, wdesc + d, xdesc + d, idesc, more);
+                                umma<KUDNN_B200_F16>(to, mdesc + d, ndesc + d, idesc, more);
                             }
                         }
                         if (S::kPair) {
@@ -547,14 +788,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-        } else if (kScaled && warp == 2) {
+        } else if (kScaled && !kRows && warp == 2) {
             // ------------------------------------------------------------------ scales of the rows times the weights' one
             constexpr int kPer = kTN / 32, kAhead = kTN == 256 ? 2 : 8;
             int slot = 0;
             uint32_t phase = 0;
             bool alive = true;
             for (int item = first_item; alive && item < num_items; item += stride) {
-                const Item w = find_item<kTN>(p, begins, items, item);
+                const Item w = find_item<kTN, kRows>(p, begins, items, item);
                 const float *sa = p.g.a_scale + w.row0 * p.g.as_sm;
                 const bool held = w.n0 + my_n < p.g.n;  // else this CTA of the pair has no weights
                 const float *sb = p.g.b_scale + w.group * p.g.bs_sg + (held ? (w.n0 + my_n) / kScaleBlock : 0) * p.g.bs_sn;
@@ -601,6 +842,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         }
         // ---------------------------------------------------------------------- sums and results
+        if constexpr (kRows) {
+            sum_rows(p, begins, items, num_items, first_item, stride, rank, warp, lane, tmem_base, tmem_full, tmem_empty, smem_u32(units),
+                     smem_u32(bias_area), abort_flag);
+        } else {
         constexpr int kRegs = S::kChunk / 2;  // registers of 16 lanes x a chunk of columns
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t my_bias = smem_u32(bias_area) + static_cast<uint32_t>((warp - 4) * 128);
@@ -624,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         };
         for (int item = first_item; item < num_items; item += stride) {
-            const Item w = find_item<kTN>(p, begins, items, item);
+            const Item w = find_item<kTN, kRows>(p, begins, items, item);
             const int n_warp = w.n0 + my_n + quarter * 32;
             float bias_lane = 0.0f;
             if (p.g.has_bias != 0 && n_warp + lane < p.g.n) {
@@ -761,6 +1006,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 release();
             }
         }
+        }
     }
 
     if (S::kSplits && p.splits > 1) {
@@ -769,7 +1015,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         cluster_barrier();
         if (warp >= 4 && first_item < num_items && *abort_flag == 0) {
             unsigned char *whole = smem;  // the ring's copies have all been consumed
-            const Item w = find_item<kTN>(p, begins, items, first_item);
+            const Item w = find_item<kTN, kRows>(p, begins, items, first_item);
             for (int unit = rank + (warp - 4) * p.splits; unit < w.cols / 16 * 4; unit += kSumWarps * p.splits) {
                 const int c0 = unit / 4 * 16, quarter = unit & 3, n0 = w.n0 + quarter * 32;
                 const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
