@@ -48,26 +48,28 @@ cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bou
         return e;
     }
     const int fixed = S::kFixedBytes + (g.groups + 1) * 8;
-    p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::kStageBytes);
+    const int budget = S::kCtas == 1 ? kSmemLimit : kSmemPerSm / S::kCtas - 1024;  // 1 KiB per CTA is the system's
+    p.stages = std::min(kMaxStages, std::max(S::kLeastStages, (budget - fixed) / S::kStageBytes));
+    const long long slots = static_cast<long long>(sm_count) * S::kCtas;
     p.splits = 1;
     if (S::kSplits) {
-        // as many CTAs as there are SMs, two k-blocks each at least
-        while (p.splits < 8 && item_bound * p.splits * 2 <= sm_count && p.num_kb >= p.splits * 4) {
-            p.splits *= 2;
+        // as many CTAs as run at a time, two k-blocks each at least
+        while (p.splits < 8 && item_bound * (p.splits + 1) <= slots && p.num_kb >= (p.splits + 1) * 2) {
+            ++p.splits;
         }
         while (p.splits > 1 && (p.splits - 1) * ((p.num_kb + p.splits - 1) / p.splits) >= p.num_kb) {
-            p.splits /= 2;  // every CTA of a cluster has a share
+            --p.splits;  // every CTA of a cluster has a share
         }
     }
     p.kb_per_split = (p.num_kb + p.splits - 1) / p.splits;
     const size_t smem = static_cast<size_t>(fixed + p.stages * S::kStageBytes);
-    long long ctas = p.splits > 1 ? item_bound * p.splits : std::min<long long>(std::max<long long>(item_bound, 1), sm_count);
+    long long ctas = p.splits > 1 ? item_bound * p.splits : std::min<long long>(std::max<long long>(item_bound, 1), slots);
     if (S::kPair) {
         // as many pairs as the GPU's partitions hold
         const int pairs = tc_pair_clusters(KUDNN_B200_F16, kSmemLimit);
         ctas = 2 * std::min<long long>(std::max<long long>(item_bound, 1), pairs > 0 ? pairs : sm_count / 2);
     }
-    return launch_chained(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, static_cast<unsigned>(S::kPair ? 2 : p.splits), ta, tb, p);
+    return launch_chained(kernel, dim3(static_cast<unsigned>(ctas)), dim3(S::kThreads), smem, stream, static_cast<unsigned>(S::kPair ? 2 : p.splits), ta, tb, p);
 }
 
 template <bool kScaled>

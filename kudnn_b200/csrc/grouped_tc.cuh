@@ -7,8 +7,8 @@
 // Tiles of 256 rows run on CTA pairs (cta_group::2, 256 weight rows, each CTA loads 128 of them and half of the group's rows): a CTA
 // alone would need 48 KiB per block of K, a pair needs 32, and 148 SMs that take 48 KiB every 512 cycles are more than L2 delivers.
 //
-// Roles (384 threads): warp 0 loads (TMA), warp 1 issues MMAs, warp 2 fetches the scales, warps 4-11 take the accumulators: a warp
-// owns 32 TMEM lanes (weight rows) and every other chunk of columns (rows of the group).  CTAs are persistent; work item = (group, rows
+// Roles: warp 0 loads (TMA), warp 1 issues MMAs, warp 2 fetches the scales, warps 4-11 (4-7 for short tiles) take the accumulators: a warp
+// owns 32 TMEM lanes (weight rows) and, where there are eight, every other chunk of columns (rows of the group).  CTAs are persistent; work item = (group, rows
 // tile, weight rows), found by a search in the groups' running item counts, which every CTA builds from the offsets.
 //
 // Scales.  The accumulator of a block of 128 k leaves tensor memory by itself (two to four buffers take turns) and is added to fp32
@@ -34,8 +34,7 @@ namespace kb {
 
 namespace grp {
 
-constexpr int kThreads = 384;
-constexpr int kSumWarps = 8;
+constexpr int kControlThreads = 128;
 constexpr int kTileN = 128;             // weight rows per CTA
 constexpr int kWeightBytes = kTileN * 128;
 constexpr int kMaxStages = 12;
@@ -43,10 +42,11 @@ constexpr int kMaxBuffers = 4;
 constexpr int kScaleSlots = 8;
 constexpr int kUnitPitch = 40;          // floats between the columns of a staged unit of 16 columns x 32 rows: conflict-free both ways
 constexpr int kUnitBytes = 16 * kUnitPitch * 4;
-constexpr int kSmemLimit = 232448;
+constexpr int kSmemLimit = 232448;      // of one CTA
+constexpr int kSmemPerSm = 233472;
 // registers per thread where a warp's sums take 128 of them: 4 control warps and 8 that sum share what the launch has, 168 each
 constexpr int kControlRegs = 88, kSumRegs = 208;
-static_assert(128 * kControlRegs + 256 * kSumRegs <= kThreads * 168, "register split");
+static_assert(128 * kControlRegs + 256 * kSumRegs <= 384 * 168, "register split");
 constexpr int kBarrierBytes = (2 * kMaxStages + 2 * kMaxBuffers + 2 * kScaleSlots) * 8 + 16;
 
 // kRows: the rows of the group on the M side (see above)
@@ -54,19 +54,27 @@ template <bool kScaled, int kTN, bool kRows>
 struct Shape {
     static_assert(!kRows || (kScaled && kTN == 256), "rows on the M side: scaled products of tall tiles");
     static constexpr bool kPair = kTN == 256;
+    // Short tiles are bound by the weights' bytes: small CTAs, of which two or three share an SM, keep many copies in flight and even out
+    // the SMs' shares.
+    static constexpr int kCtas = kTN == 32 ? 3 : kTN == 64 ? 2 : 1;
+    static constexpr int kSumWarps = kTN <= 64 ? 4 : 8;
+    static constexpr int kWays = kSumWarps / 4;               // warps that share a quarter of the lanes: they take chunks in turn
+    static constexpr int kThreads = kControlThreads + 32 * kSumWarps;
     static constexpr int kBuffers = kScaled ? (kTN == 256 ? 2 : 4) : 2;
     static constexpr int kTmemCols = kBuffers * kTN;
+    static constexpr int kChunk = kTN >= 64 ? 32 : 16;        // columns a warp takes at a time
+    static constexpr int kChunks = kTN / kChunk / kWays;      // per warp
     static constexpr int kRound = kPair ? 32 : 16;            // N of an MMA is a multiple of this
     static constexpr int kLoadRows = kPair ? kTN / 2 : kTN;   // rows of a that one CTA loads, at most
-    static constexpr int kBoxRows = kTN >= 128 ? 64 : 32;     // of them in one copy
-    static constexpr int kChunk = kTN >= 128 ? 32 : 16;       // columns a warp takes at a time; the two warps of a lane quarter take turns
-    static constexpr int kChunks = kTN / kChunk / 2;          // per warp
+    static constexpr int kBoxRows = kTN >= 128 ? 64 : kTN / 2;  // of them in one copy
     static constexpr int kStageBytes = kWeightBytes + kLoadRows * 128;
-    static constexpr bool kSplits = kTN <= 64;                // whether launches may cut K (the partial sums have to fit)
-    static constexpr int kUnits = kSplits && kTN / 16 * 4 > kSumWarps ? kTN / 16 * 4 : kSumWarps;
+    static constexpr bool kSplits = kTN <= 64;                // whether launches may cut K
+    static constexpr int kUnits = kTN / 16 * 4;               // of a whole tile; partial sums lie where the ring was
+    static constexpr int kLeastStages = kTN == 32 ? 2 : 3;
+    static_assert(!kSplits || (kUnits + kSumWarps) * kUnitBytes <= kLeastStages * kStageBytes, "room for the partial sums");
     static constexpr int kScaleBytes = kScaled && !kRows ? kScaleSlots * kTN * 4 : 0;
     static constexpr int kBiasBytes = kSumWarps * (kRows ? 512 : 128);
-    static constexpr int kFixedBytes = kUnits * kUnitBytes + kBiasBytes + kScaleBytes + kBarrierBytes;
+    static constexpr int kFixedBytes = kSumWarps * kUnitBytes + kBiasBytes + kScaleBytes + kBarrierBytes;
 };
 
 struct TcParams {
@@ -189,6 +197,22 @@ __device__ __forceinline__ void load_shared_4(uint32_t at, float *v)
 __device__ __forceinline__ void store_shared(uint32_t at, float v)
 {
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// Whether a phase has ended, without waiting (mbarrier.try_wait may hold the thread for microseconds)
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 // A wait of a whole warp, which gets one answer.  The first look is apart from the bounded loop: an arrival that is there already, the
@@ -414,7 +438,7 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
                 row_after = s.row[(kb + 2) * g.as_sk];
                 weights_after = s.weights[(kb + 2) * g.bs_sk];
             }
-            alive = warp_wait(mbar_try_wait(tmem_full + buffer, phase), tmem_full + buffer, phase, abort_flag, p.status, 4, p.wait_limit);
+            alive = warp_wait(mbar_test(tmem_full + buffer, phase), tmem_full + buffer, phase, abort_flag, p.status, 4, p.wait_limit);
             if (!alive) {
                 break;
             }
@@ -545,13 +569,15 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
 }
 
 template <bool kScaled, int kTN, bool kRows>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kScaled, kTN, kRows>::kCtas)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ TcParams p)
 {
     using S = Shape<kScaled, kTN, kRows>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    unsigned char *units = smem + p.stages * S::kStageBytes;
-    unsigned char *bias_area = units + S::kUnits * kUnitBytes;
+    constexpr int kThreads = S::kThreads, kSumWarps = S::kSumWarps;
+    unsigned char *behind_ring = smem + p.stages * S::kStageBytes;
+    unsigned char *units = S::kSplits && p.splits > 1 ? smem : behind_ring;  // staged results; partial sums lie where the ring was
+    unsigned char *bias_area = behind_ring + kSumWarps * kUnitBytes;
     unsigned char *scales = bias_area + S::kBiasBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(scales + S::kScaleBytes);
     uint64_t *full_bar = bars;
@@ -694,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t bytes = static_cast<uint32_t>(kWeightBytes + boxes * S::kBoxRows * 128) * (S::kPair ? 2u : 1u);
                 const int end = kb_end < p.load_kb ? kb_end : p.load_kb;
                 for (int kb = kb_begin; kb < end; ++kb) {
-                    alive = warp_wait(mbar_try_wait(empty_bar + stage, phase ^ 1u), empty_bar + stage, phase ^ 1u, abort_flag, p.status, 1, p.wait_limit);
+                    alive = warp_wait(mbar_test(empty_bar + stage, phase ^ 1u), empty_bar + stage, phase ^ 1u, abort_flag, p.status, 1, p.wait_limit);
                     if (!alive) {
                         break;
                     }
@@ -731,13 +757,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             int stage = 0, buffer = 0;
             uint32_t phase = 0, buffer_phase = 0;
             bool alive = true;
-            bool loaded = mbar_try_wait(full_bar, 0);  // looked up one k-block ahead, so that the answer is there when it is needed
+            bool loaded = mbar_test(full_bar, 0);  // looked up one k-block ahead, so that the answer is there when it is needed
             for (int item = first_item; alive && item < num_items; item += stride) {
                 const Item w = find_item<kTN, kRows>(p, begins, items, item);
                 const uint32_t idesc = p.idesc | (kRows ? 0u : static_cast<uint32_t>(w.cols >> 3) << 17);
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
                     if (kScaled || kb == kb_begin) {
-                        alive = warp_wait(mbar_try_wait(tmem_empty + buffer, buffer_phase ^ 1u), tmem_empty + buffer, buffer_phase ^ 1u, abort_flag,
+                        alive = warp_wait(mbar_test(tmem_empty + buffer, buffer_phase ^ 1u), tmem_empty + buffer, buffer_phase ^ 1u, abort_flag,
                                           p.status, 2, p.wait_limit);
                     }
                     alive = alive && warp_wait(loaded, full_bar + stage, phase, abort_flag, p.status, 3, p.wait_limit);
@@ -755,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         stage = 0;
                         phase ^= 1u;
                     }
-                    loaded = mbar_try_wait(full_bar + stage, phase);
+                    loaded = mbar_test(full_bar + stage, phase);
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
@@ -814,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < kAhead; ++i) {
                         if (alive && kb0 + i < kb_end) {
-                            alive = warp_wait(mbar_try_wait(scale_empty + slot, phase ^ 1u), scale_empty + slot, phase ^ 1u, abort_flag, p.status, 5,
+                            alive = warp_wait(mbar_test(scale_empty + slot, phase ^ 1u), scale_empty + slot, phase ^ 1u, abort_flag, p.status, 5,
                                               p.wait_limit);
                             const uint32_t at = smem_u32(scales) + static_cast<uint32_t>(slot * kTN * 4);
 #pragma unroll
@@ -888,8 +914,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll 1
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
-                    const bool scales_there = mbar_try_wait(scale_full + slot, slot_phase);
-                    const bool sums_there = mbar_try_wait(tmem_full + buffer, buffer_phase);
+                    const bool scales_there = mbar_test(scale_full + slot, slot_phase);
+                    const bool sums_there = mbar_test(tmem_full + buffer, buffer_phase);
                     alive = warp_wait(scales_there, scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit) &&
                             warp_wait(sums_there, tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
                     if (!alive) {
@@ -900,7 +926,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t scale_at = smem_u32(scales) + static_cast<uint32_t>(slot * kTN * 4 + (lane & 3) * 16);
 #pragma unroll
                     for (int i = 0; i < S::kChunks; ++i) {
-                        const int c0 = (2 * i + half) * S::kChunk;
+                        const int c0 = (S::kWays * i + half) * S::kChunk;
                         if (c0 >= w.cols) {
                             break;
                         }
@@ -930,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             } else {
-                alive = warp_wait(mbar_try_wait(tmem_full + buffer, buffer_phase), tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
+                alive = warp_wait(mbar_test(tmem_full + buffer, buffer_phase), tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
                 tc_fence_after();
             }
             if (!alive) {
@@ -944,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int kUnitsPerChunk = S::kChunk / 16;
 #pragma unroll 1
             for (int u = 0; u < S::kChunks * kUnitsPerChunk; ++u) {
-                const int c0 = (2 * (u / kUnitsPerChunk) + half) * S::kChunk + u % kUnitsPerChunk * 16;
+                const int c0 = (S::kWays * (u / kUnitsPerChunk) + half) * S::kChunk + u % kUnitsPerChunk * 16;
                 if (c0 >= w.cols) {
                     break;
                 }
@@ -1014,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         cluster_barrier();
         if (warp >= 4 && first_item < num_items && *abort_flag == 0) {
-            unsigned char *whole = smem;  // the ring's copies have all been consumed
+            unsigned char *whole = smem + S::kUnits * kUnitBytes;
             const Item w = find_item<kTN, kRows>(p, begins, items, first_item);
             for (int unit = rank + (warp - 4) * p.splits; unit < w.cols / 16 * 4; unit += kSumWarps * p.splits) {
                 const int c0 = unit / 4 * 16, quarter = unit & 3, n0 = w.n0 + quarter * 32;
