@@ -59,6 +59,6 @@ struct QuantizeParams {
     int rows, k, x_rows;
     int x_dtype, gate, block_rows;
 };
-cudaError_t launch_quantize(const QuantizeParams &p, int sm_count, cudaStream_t stream);
+cudaError_t launch_quantize(const QuantizeParams &p, cudaStream_t stream);
 
 }  // namespace kb

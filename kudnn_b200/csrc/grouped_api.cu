@@ -164,7 +164,7 @@ int kudnn_b200_quantize_run(const kudnn_b200_quantize_desc *d, const void *x, vo
     p.x_dtype = d->x_dtype;
     p.gate = d->gate != 0 ? 1 : 0;
     p.block_rows = d->block_rows;
-    const cudaError_t e = kb::launch_quantize(p, sms, static_cast<cudaStream_t>(cuda_stream));
+    const cudaError_t e = kb::launch_quantize(p, static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? KUDNN_B200_OK : fail_cuda(e, "quantize kernel launch");
 }
 
