@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 namespace kb {
 
@@ -47,20 +48,24 @@ cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bou
     if (e != cudaSuccess) {
         return e;
     }
-    const int fixed = S::kFixedBytes + (g.groups + 1) * 8;
-    const int budget = S::kCtas == 1 ? kSmemLimit : kSmemPerSm / S::kCtas - 1024;  // 1 KiB per CTA is the system's
-    p.stages = std::min(kMaxStages, std::max(S::kLeastStages, (budget - fixed) / S::kStageBytes));
-    const long long slots = static_cast<long long>(sm_count) * S::kCtas;
+    // Where the items leave SMs idle, two or four CTAs of a cluster cut K, if that fills the SMs better: 86 items of one row, 32 blocks of K:
+    // 11.8 us uncut, 12.2 at two (172 CTAs on 148 SMs), 10.4 at four.  Clusters of 8 and odd ones find no room next to one another.
+    // The CTAs that then share an SM share its memory for their rings.
+    auto filled = [&](long long ctas) { return static_cast<double>(ctas) / sm_count / ((ctas + sm_count - 1) / sm_count); };
     p.splits = 1;
     if (S::kSplits) {
-        // as many CTAs as run at a time, two k-blocks each at least
-        while (p.splits < 8 && item_bound * (p.splits + 1) <= slots && p.num_kb >= (p.splits + 1) * 2) {
-            ++p.splits;
-        }
-        while (p.splits > 1 && (p.splits - 1) * ((p.num_kb + p.splits - 1) / p.splits) >= p.num_kb) {
-            --p.splits;  // every CTA of a cluster has a share
+        for (int s = 2; s <= 4; s *= 2) {
+            if (item_bound * s <= static_cast<long long>(sm_count) * S::kCtas && p.num_kb >= 4 * s &&
+                (s - 1) * ((p.num_kb + s - 1) / s) < p.num_kb && filled(item_bound * s) > 1.05 * filled(item_bound * p.splits)) {
+                p.splits = s;
+            }
         }
     }
+    const int sharing = static_cast<int>(std::clamp<long long>((item_bound * p.splits + sm_count - 1) / sm_count, 1, S::kCtas));
+    const int fixed = S::kFixedBytes + (g.groups + 1) * 8;
+    const int budget = sharing == 1 ? kSmemLimit : kSmemPerSm / sharing - 1024;  // 1 KiB per CTA is the system's
+    p.stages = std::min(kMaxStages, std::max(S::kLeastStages, (budget - fixed) / S::kStageBytes));
+    const long long slots = static_cast<long long>(sm_count) * sharing;
     p.kb_per_split = (p.num_kb + p.splits - 1) / p.splits;
     const size_t smem = static_cast<size_t>(fixed + p.stages * S::kStageBytes);
     long long ctas = p.splits > 1 ? item_bound * p.splits : std::min<long long>(std::max<long long>(item_bound, 1), slots);
@@ -72,23 +77,63 @@ cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bou
     return launch_chained(kernel, dim3(static_cast<unsigned>(ctas)), dim3(S::kThreads), smem, stream, static_cast<unsigned>(S::kPair ? 2 : p.splits), ta, tb, p);
 }
 
+// The width of the tiles: the one with the least time by what a block of K was measured to take an SM (cycles, at 1.9 GHz; a pair of SMs
+// for tiles of 256), times the rounds that the items make.  Short tiles share an SM, so that their rounds need not be whole ones.
+// 333 x 11008 x 4096 in 8 bits: 31.9 / 29.4 / 35.4 us on tiles of 64 / 128 / 256 rows, 512 x 2048 x 4096 14.1 / 16.9 / 19.7,
+// 1024 x 4096 x 4096 32.0 / 29.8 / 21.0.
+struct TileCost {
+    int rows;
+    double alone, shared, finish;  // one CTA on an SM, as many as fit; results of a tile
+};
+constexpr TileCost kScaledCost[4] = {{32, 450, 330, 1000}, {64, 564, 470, 1500}, {128, 757, 757, 2500}, {256, 850, 850, 2500}};
+constexpr TileCost kPlainCost[4] = {{32, 450, 330, 1000}, {64, 500, 400, 1500}, {128, 560, 560, 1000}, {256, 540, 540, 1000}};
+
+int choose_tile(const GroupedParams &g, const TcParams &p, bool scaled, bool tall_on_m, int sm_count)
+{
+    const double busy = std::min(g.groups, g.rows);
+    int best = 256;
+    double least = 0.0;
+    for (int i = 0; i < 4; ++i) {
+        const TileCost &c = scaled ? kScaledCost[i] : kPlainCost[i];
+        const int wide = c.rows == 256 ? 256 : 128;
+        // groups are uneven: half of a group's last tile is empty, on average
+        const double tiles = g.offsets == nullptr ? (g.rows + c.rows - 1) / c.rows : std::max(busy, g.rows / static_cast<double>(c.rows) + 0.5 * busy);
+        const double items = tiles * ((g.n + wide - 1) / wide), fill = std::min(1.0, g.rows / (tiles * c.rows));
+        double cycles;
+        if (c.rows <= 64) {
+            cycles = std::max(c.alone * p.num_kb, c.shared * p.num_kb * items / sm_count) + c.finish;
+        } else {
+            // weights on the M side: a block of K takes less where the tile has fewer rows
+            const double each = c.rows == 128 || tall_on_m ? c.alone : (scaled ? 1170.0 : c.alone) * std::max(0.55, fill);
+            const double rounds = std::ceil(items / (c.rows == 256 ? sm_count / 2 : sm_count));
+            cycles = rounds * (each * p.num_kb + c.finish);
+        }
+        if (i == 0 || cycles < least) {
+            least = cycles;
+            best = c.rows;
+        }
+    }
+    return best;
+}
+
 template <bool kScaled>
 cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &tb, cudaStream_t stream)
 {
-    // the tile that holds twice an average group's rows, since groups are uneven; without offsets the one that holds them all
-    const long long rows = g.offsets == nullptr ? g.rows : 2ll * g.rows / g.groups;
-    const int tn = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    // Tall tiles of scaled products: rows on the M side, unless the groups' last tiles, which that pads to 256 rows, would take more than the
+    // faster sums save (850 against 1170 cycles per block of K).
+    const bool tall_on_m = kScaled && (g.offsets == nullptr || g.rows >= 192ll * g.groups);
+    const int tn = choose_tile(g, p, kScaled, tall_on_m, sm_count);
     // offsets may leave out rows and make up to min(groups, rows) short tiles
     const long long tiles = g.offsets == nullptr ? (g.rows + tn - 1) / tn : std::min(g.groups, g.rows) + g.rows / tn;
     p.tiles_n = tn == 256 ? (g.n + 2 * kTileN - 1) / (2 * kTileN) : (g.n + kTileN - 1) / kTileN;
     p.idesc = make_idesc(g.ab_dtype == KUDNN_B200_BF16 ? KUDNN_B200_BF16 : KUDNN_B200_F16, 0, tn == 256 ? 2 * kTileN : kTileN);  // e4m3 and fp16: code 0
     const long long bound = tiles * p.tiles_n;
     if constexpr (kScaled) {
-        // Tall tiles of scaled products: rows on the M side, unless the groups' last tiles, which that pads to 256 rows, would take more
-        // than the faster sums save (700 against 1170 cycles per block of K: groups of 190 rows on average).
-        if (tn == 256 && (g.offsets == nullptr || g.rows >= 192ll * g.groups)) {
+        if (tn == 256 && tall_on_m) {
             p.idesc |= 256u >> 3 << 17;
-            p.vec = p.vec != 0 && g.c_sm * dtype_size(g.c_dtype) % 32 == 0 && reinterpret_cast<uintptr_t>(g.c) % 32 == 0 ? 1 : 0;
+            if (p.vec != 0 && g.c_sm * dtype_size(g.c_dtype) % 32 == 0 && reinterpret_cast<uintptr_t>(g.c) % 32 == 0) {
+                p.vec = 2;
+            }
             return launch_shape<true, 256, true>(g, p, bound, sm_count, tb, stream);
         }
     }

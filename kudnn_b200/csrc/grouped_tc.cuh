@@ -85,7 +85,7 @@ struct TcParams {
     int splits, kb_per_split;
     int stages;
     int band;          // row tiles that share the weight tiles of a raster band
-    int vec;           // rows of c are contiguous, four of their elements aligned, and finish_unit knows the activation
+    int vec;           // 1: rows of c are contiguous, four of their elements aligned, and finish_unit knows the activation; 2: 32-byte aligned too
     unsigned idesc;    // without N
     int load_kb;       // k-blocks from this one on are not loaded (test hook)
     DeviceStatus *status;
@@ -108,19 +108,24 @@ __device__ __forceinline__ Item find_item(const TcParams &p, const int *begins, 
             hi = mid;
         }
     }
+    constexpr int kRound = kTN == 256 ? 32 : 16, kWide = kTN == 256 ? 2 * kTileN : kTileN;
     const int local = item - items[lo], begin = begins[lo], rows = begins[lo + 1] - begin;
-    const int tiles = (rows + kTN - 1) / kTN;
-    constexpr int kRound = kTN == 256 ? 32 : 16;
-    // rows of a tile: the group cut evenly, or what the M side holds
-    const int tall = kRows ? kTN : ((rows + tiles - 1) / tiles + kRound - 1) / kRound * kRound;
-    const int per_band = p.band * p.tiles_n;
-    const int first = local / per_band * p.band;
-    const int wide = tiles - first < p.band ? tiles - first : p.band;
-    const int in_band = local % per_band;
     Item w;
     w.group = lo;
-    w.n0 = in_band / wide * (kTN == 256 ? 2 * kTileN : kTileN);
-    w.row0 = begin + (first + in_band % wide) * tall;
+    int tall;  // rows of a tile: the group cut evenly, or what the M side holds
+    if (rows <= kTN) {
+        tall = rows;
+        w.n0 = local * kWide;
+        w.row0 = begin;
+    } else {
+        const int tiles = (rows + kTN - 1) / kTN;
+        tall = kRows ? kTN : ((rows + tiles - 1) / tiles + kRound - 1) / kRound * kRound;
+        const int per_band = p.band * p.tiles_n, band = local / per_band, in_band = local - band * per_band;
+        const int first = band * p.band, wide = tiles - first < p.band ? tiles - first : p.band;
+        const int column = in_band / wide;
+        w.n0 = column * kWide;
+        w.row0 = begin + (first + in_band - column * wide) * tall;
+    }
     const int left = begin + rows - w.row0;
     w.count = left < tall ? left : tall;
     w.cols = kRows ? 256 : (w.count + kRound - 1) / kRound * kRound;
@@ -317,23 +322,49 @@ __device__ __forceinline__ void finish_unit(const GroupedParams &g, int row0, in
     }
 }
 
-// bias_at: 32 floats of shared memory
+// bias_at: 32 floats of shared memory.  A lane takes a column, so that the 32 of a row are stored side by side however c is aligned.
 static __device__ __noinline__ void finish_unit_any(const GroupedParams &g, int row0, int count, int n0, uint32_t bias_at, uint32_t unit_at, int lane)
 {
     if (n0 + lane >= g.n) {
         return;
     }
-    float bias;
+    float bias, v[4][4];
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(bias) : "r"(bias_at + static_cast<uint32_t>(lane * 4)));
-#pragma unroll 1
-    for (int r = 0; r < 16 && r < count; ++r) {
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(unit_at + static_cast<uint32_t>((r * kUnitPitch + lane) * 4)));
-        v += bias;
-        if (g.act != KUDNN_B200_ACT_NONE) {
-            v = activation_any(v, g.act, g.act_alpha, g.c_dtype == KUDNN_B200_F32 ? 1 : 0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[r / 4][r % 4]) : "r"(unit_at + static_cast<uint32_t>((r * kUnitPitch + lane) * 4)));
+        v[r / 4][r % 4] += bias;
+    }
+    const bool precise = g.c_dtype == KUDNN_B200_F32;
+    if (g.act == KUDNN_B200_ACT_RELU) {
+        activate<KUDNN_B200_ACT_RELU, true>(v, g.act_alpha);
+    } else if (g.act == KUDNN_B200_ACT_SWISH && !precise) {
+        activate<KUDNN_B200_ACT_SWISH, false>(v, g.act_alpha);
+    } else if (g.act == KUDNN_B200_ACT_GELU_TANH && !precise) {
+        activate<KUDNN_B200_ACT_GELU_TANH, false>(v, g.act_alpha);
+    } else if (g.act != KUDNN_B200_ACT_NONE) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            v[r / 4][r % 4] = activation_any(v[r / 4][r % 4], g.act, g.act_alpha, precise ? 1 : 0);
         }
-        store_exact(g.c, g.c_dtype, (row0 + r) * g.c_sm + (n0 + lane) * g.c_sn, round_rne(v, g.c_dtype));
+    }
+    const long long at = row0 * g.c_sm + (n0 + lane) * g.c_sn;
+    if (precise) {
+        float *to = static_cast<float *>(g.c) + at;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (r < count) {
+                to[r * g.c_sm] = v[r / 4][r % 4];
+            }
+        }
+    } else {
+        unsigned short *to = static_cast<unsigned short *>(g.c) + at;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (r < count) {
+                to[r * g.c_sm] = g.c_dtype == KUDNN_B200_F16 ? f32_to_f16_rne_bits(v[r / 4][r % 4]) : f32_to_bf16_rne_bits(v[r / 4][r % 4]);
+            }
+        }
     }
 }
 
@@ -357,8 +388,15 @@ __device__ __forceinline__ void tmem_load_32x16(uint32_t taddr, uint32_t (&r)[16
         : "r"(taddr));
 }
 
-__device__ __forceinline__ void store_32_bytes(void *to, const uint32_t *w)
+__device__ __forceinline__ void store_32_bytes(void *to, const uint32_t *w, int vec)
 {
+    if (vec == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            reinterpret_cast<uint2 *>(to)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+        }
+        return;
+    }
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
                  "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
@@ -519,7 +557,7 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
                             for (int j = 0; j < 8; ++j) {
                                 v[j] = __float_as_uint(sum[i * 8 + j]);
                             }
-                            store_32_bytes(to + i * 32, v);
+                            store_32_bytes(to + i * 32, v, p.vec);
                         }
                     } else {
                         uint32_t v[16];
@@ -536,8 +574,8 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
                                 v[j] = *reinterpret_cast<const uint32_t *>(&h);
                             }
                         }
-                        store_32_bytes(to, v);
-                        store_32_bytes(to + 32, v + 8);
+                        store_32_bytes(to, v, p.vec);
+                        store_32_bytes(to + 32, v + 8, p.vec);
                     }
                 }
             } else {
@@ -614,6 +652,11 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
             mbar_init(scale_empty + s, kSumWarps);
         }
         *abort_flag = 0;
+        if (p.g.offsets == nullptr) {
+            begins[0] = items[0] = 0;
+            begins[1] = p.g.rows;
+            items[1] = (p.g.rows + kTN - 1) / kTN * p.tiles_n;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -642,48 +685,50 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
     pdl_launch_dependents();  // only now that this CTA holds its tensor memory
     pdl_wait();
 
-    // ---- the groups: offsets made to ascend, and the items before each group
-    for (int i = threadIdx.x; i <= p.g.groups; i += kThreads) {
-        begins[i] = group_offset(p.g, i);
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int most = 0;
-        for (int i0 = 0; i0 <= p.g.groups; i0 += 32) {
-            int v = i0 + lane <= p.g.groups ? begins[i0 + lane] : 0;
+    // ---- the groups: offsets made to ascend, and the items before each group (without offsets thread 0 has written them above)
+    if (p.g.offsets != nullptr) {
+        for (int i = threadIdx.x; i <= p.g.groups; i += kThreads) {
+            begins[i] = group_offset(p.g, i);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int most = 0;
+            for (int i0 = 0; i0 <= p.g.groups; i0 += 32) {
+                int v = i0 + lane <= p.g.groups ? begins[i0 + lane] : 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int before = __shfl_up_sync(0xffffffffu, v, o);
-                v = lane >= o && before > v ? before : v;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int before = __shfl_up_sync(0xffffffffu, v, o);
+                    v = lane >= o && before > v ? before : v;
+                }
+                v = v > most ? v : most;
+                if (i0 + lane <= p.g.groups) {
+                    begins[i0 + lane] = v;
+                }
+                most = __shfl_sync(0xffffffffu, v, 31);
             }
-            v = v > most ? v : most;
-            if (i0 + lane <= p.g.groups) {
-                begins[i0 + lane] = v;
-            }
-            most = __shfl_sync(0xffffffffu, v, 31);
-        }
-        __syncwarp();
-        int all = 0;
-        for (int i0 = 0; i0 < p.g.groups; i0 += 32) {
-            int v = 0;
-            if (i0 + lane < p.g.groups) {
-                v = (begins[i0 + lane + 1] - begins[i0 + lane] + kTN - 1) / kTN * p.tiles_n;
-            }
+            __syncwarp();
+            int all = 0;
+            for (int i0 = 0; i0 < p.g.groups; i0 += 32) {
+                int v = 0;
+                if (i0 + lane < p.g.groups) {
+                    v = (begins[i0 + lane + 1] - begins[i0 + lane] + kTN - 1) / kTN * p.tiles_n;
+                }
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int before = __shfl_up_sync(0xffffffffu, v, o);
-                v += lane >= o ? before : 0;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int before = __shfl_up_sync(0xffffffffu, v, o);
+                    v += lane >= o ? before : 0;
+                }
+                if (i0 + lane < p.g.groups) {
+                    items[i0 + lane + 1] = all + v;
+                }
+                all += __shfl_sync(0xffffffffu, v, 31);
             }
-            if (i0 + lane < p.g.groups) {
-                items[i0 + lane + 1] = all + v;
+            if (lane == 0) {
+                items[0] = 0;
             }
-            all += __shfl_sync(0xffffffffu, v, 31);
         }
-        if (lane == 0) {
-            items[0] = 0;
-        }
+        __syncthreads();
     }
-    __syncthreads();
     const int num_items = items[p.g.groups];
     const int rank = S::kPair || p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
     // launches that cut K have a cluster for every item that there can be
