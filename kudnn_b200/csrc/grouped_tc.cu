@@ -171,7 +171,7 @@ cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus
     p.g = g;
     p.kb_elems = 128 / es;
     p.num_kb = (g.k + p.kb_elems - 1) / p.kb_elems;
-    p.band = 8;
+    p.band = 16;
     const bool short_act = g.act == KUDNN_B200_ACT_NONE || g.act == KUDNN_B200_ACT_RELU || g.act == KUDNN_B200_ACT_SWISH ||
                            (g.act == KUDNN_B200_ACT_GELU_TANH && g.c_dtype != KUDNN_B200_F32);
     p.vec = short_act && (g.c_sn == 1 || g.n == 1) && (g.rows == 1 || g.c_sm % 4 == 0) && reinterpret_cast<uintptr_t>(g.c) % (4 * c_size) == 0 ? 1 : 0;

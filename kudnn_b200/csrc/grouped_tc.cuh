@@ -482,14 +482,14 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
             }
             tc_fence_after();
             const uint32_t from = my_tmem + static_cast<uint32_t>(buffer * 256);
+            uint32_t part[2][16];  // one load ahead of the FMAs
+            tmem_load_32x16(from, part[0]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t a[16], b[16];
-                tmem_load_32x16(from + static_cast<uint32_t>(c * 32), a);
-                tmem_load_32x16(from + static_cast<uint32_t>(c * 32 + 16), b);
-                tmem_wait(a);
-                tmem_wait(b);
-                if (c == 3) {  // everything is in registers: the MMAs may have the buffer again
+            for (int c = 0; c < 8; ++c) {
+                tmem_wait(part[c & 1]);
+                if (c < 7) {
+                    tmem_load_32x16(from + static_cast<uint32_t>((c + 1) * 16), part[(c + 1) & 1]);
+                } else {  // everything is in registers: the MMAs may have the buffer again
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
@@ -498,8 +498,7 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
                 }
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    sum[c * 32 + j] = fmaf(__uint_as_float(a[j]), scale, sum[c * 32 + j]);
-                    sum[c * 32 + 16 + j] = fmaf(__uint_as_float(b[j]), scale, sum[c * 32 + 16 + j]);
+                    sum[c * 16 + j] = fmaf(__uint_as_float(part[c & 1][j]), scale, sum[c * 16 + j]);
                 }
             }
             if (++buffer == kBuffers) {
@@ -841,15 +840,15 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                             }
                         }
                         if (S::kPair) {
-                            umma_commit_pair(empty_bar + this_stage);
                             if (whole) {
                                 umma_commit_pair(tmem_full + buffer);
                             }
+                            umma_commit_pair(empty_bar + this_stage);
                         } else {
-                            umma_commit(empty_bar + this_stage);
                             if (whole) {
                                 umma_commit(tmem_full + buffer);
                             }
+                            umma_commit(empty_bar + this_stage);
                         }
                     }
                     __syncwarp();

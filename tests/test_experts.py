@@ -1,0 +1,168 @@
+"""The torch operators kudnn_b200::quantize and ::grouped, and the feed-forward block of experts that runs them together."""
+import collections
+
+import pytest
+import torch
+
+import kudnn_b200 as kb
+from kudnn_b200 import torch_ops
+
+ops = torch.ops.kudnn_b200
+gpu = pytest.mark.gpu
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_fake_implementations_propagate_shapes_without_a_device():
+    q, s = ops.quantize(meta(5, 300))
+    assert q.shape == (5, 300) and q.dtype == torch.float8_e4m3fn and q.stride() == (304, 1)
+    assert s.shape == (5, 3) and s.dtype == torch.float32 and s.stride() == (1, 5)
+    q, s = ops.quantize(meta(5, 600), True, meta(9, dtype=torch.int32))
+    assert q.shape == (9, 300) and s.shape == (9, 3)
+    q, s = ops.quantize(meta(200, 300), block_rows=128)
+    assert q.shape == (200, 300) and s.shape == (2, 3) and s.stride() == (3, 1)
+    e = meta(7, 300, dtype=torch.float8_e4m3fn)
+    assert ops.grouped(e, meta(4, 64, 300, dtype=torch.float8_e4m3fn)).dtype == torch.bfloat16
+    y = ops.grouped(meta(7, 300), meta(4, 64, 300), out_dtype=torch.float32)
+    assert y.shape == (7, 64) and y.dtype == torch.float32
+
+
+class _Recorded:
+    def __init__(self, desc):
+        self.closed = False
+
+    def close(self):
+        self.closed = True
+
+
+def test_created_products_are_bounded_and_captured_ones_stay(monkeypatch):
+    capturing = [False]
+    monkeypatch.setattr(torch_ops.capi, "Grouped", _Recorded)
+    monkeypatch.setattr(torch_ops, "_GROUPED", collections.OrderedDict())
+    monkeypatch.setattr(torch_ops, "_MAX_GROUPED", 3)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    cuda = torch.device("cuda", 0)
+
+    def handle(key):
+        return torch_ops._grouped_handle(cuda, key, lambda: None)
+
+    capturing[0] = True
+    first = handle("a")
+    capturing[0] = False
+    second = handle("b")
+    assert handle("a") is first and handle("b") is second
+    for key in "cdefg":
+        handle(key)
+        assert len(torch_ops._GROUPED) == 3
+    assert handle("a") is first and handle("b") is not second
+    torch_ops.clear_cache()
+    assert first.closed and not torch_ops._GROUPED
+
+
+@gpu
+def test_operators_against_their_definition(cuda_device):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(37, 520, generator=gen, device="cuda").bfloat16()
+    w = torch.randn(3, 264, 520, generator=gen, device="cuda").bfloat16() * 0.05
+    bias = torch.randn(3, 264, generator=gen, device="cuda")
+    offsets = torch.tensor([0, 10, 10, 37], device="cuda")
+    y = ops.grouped(x, w, offsets, bias=bias, act=kb.ACT_RELU, act_alpha=0.0, out_dtype=torch.float32)
+    for g, (lo, hi) in enumerate(((0, 10), (10, 10), (10, 37))):
+        want = torch.relu(x[lo:hi].double() @ w[g].double().t() + bias[g].double())
+        limit = (520 / 8 + 8) * 2.0 ** -23 * (x[lo:hi].double().abs() @ w[g].double().abs().t() + bias[g].double().abs())
+        assert torch.all((y[lo:hi].double() - want).abs() <= limit)
+    # 8-bit operands of the quantiser's own making, dense
+    q, s = ops.quantize(x)
+    qw, sw = ops.quantize(w[0], block_rows=128)
+    y = ops.grouped(q, qw, None, s, sw, out_dtype=torch.float32)
+    a = q.double() * s.double().repeat_interleave(128, 1)[:, :520]
+    b = qw.double() * sw.double().repeat_interleave(128, 0)[:264].repeat_interleave(128, 1)[:, :520]
+    assert torch.all((y.double() - a @ b.t()).abs() <= (520 / 8 + 8) * 2.0 ** -23 * (a.abs() @ b.abs().t()))
+    # views: rows at a pitch, transposed weights, no rows
+    wide = torch.randn(37, 600, generator=gen, device="cuda").bfloat16()
+    t = w.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.allclose(ops.grouped(wide[:, :520], t, offsets).float(), ops.grouped(wide[:, :520].contiguous(), w, offsets).float(), atol=2e-2, rtol=2e-2)
+    assert ops.grouped(x[:0], w, torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, 264)
+    assert ops.quantize(x[:0])[0].shape == (0, 520)
+
+
+@gpu
+@pytest.mark.parametrize("wrong", [
+    lambda x, w, o: ops.grouped(x.float(), w.float(), o), lambda x, w, o: ops.grouped(x, w.half(), o), lambda x, w, o: ops.grouped(x, w[:, :, :-8], o),
+    lambda x, w, o: ops.grouped(x, w, None), lambda x, w, o: ops.grouped(x, w, o[:-1]), lambda x, w, o: ops.grouped(x, w, o.float()),
+    lambda x, w, o: ops.grouped(x, w, o.cpu()), lambda x, w, o: ops.grouped(x, w, o, x_scale=torch.ones(4, 1, device="cuda")),
+    lambda x, w, o: ops.grouped(x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn), o),
+    lambda x, w, o: ops.grouped(x, w, o, bias=torch.ones(64, device="cuda")), lambda x, w, o: ops.grouped(x, w, o, out_dtype=torch.float64),
+    lambda x, w, o: ops.quantize(x.double()), lambda x, w, o: ops.quantize(x[0]), lambda x, w, o: ops.quantize(x[:, :63], True),
+    lambda x, w, o: ops.quantize(x, False, o.long()), lambda x, w, o: ops.quantize(x, block_rows=64), lambda x, w, o: ops.quantize(x, True, None, 128),
+])
+def test_refusals(cuda_device, wrong):
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(2, 64, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises((TypeError, ValueError)):
+        wrong(x, w, torch.tensor([0, 1, 4], dtype=torch.int32, device="cuda"))
+
+
+def experts64(x, router, gate_up, down, top):
+    tokens = x.reshape(-1, x.shape[-1])
+    p = torch.softmax(tokens.double() @ router.double().t(), dim=1)
+    p, chosen = torch.topk(p, top, dim=1)
+    p = p / p.sum(dim=1, keepdim=True)
+    y = torch.zeros(tokens.shape, dtype=torch.float64, device=x.device)
+    for e in range(router.shape[0]):
+        t, slot = (chosen == e).nonzero(as_tuple=True)
+        h = tokens[t].double() @ gate_up[e].double().t()
+        gate, up = h.chunk(2, dim=1)
+        y.index_add_(0, t, (torch.nn.functional.silu(gate) * up @ down[e].double().t()) * p[t, slot][:, None])
+    return y.view(x.shape)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 7, 300])
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_experts(cuda_device, tokens, eight_bit):
+    """Norm of the error over the norm of the result.  bf16: the values between the products, the gated ones, the second product and the sum
+    are each rounded to 2^-9: 2^-7 in all.  8 bits: the two operands of either product are each off by 2^-4 at most, 3.6 % in the square mean;
+    the first product's error (5.1 %) enters the gated value twice with a slope of up to 1.1, so 7.9 %, and with the second product's two
+    operands 9.4 %."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    hidden, ffn, experts, top = 512, 384, 16, 4
+    x = torch.randn(1, tokens, hidden, generator=gen, device="cuda").bfloat16()
+    router = torch.randn(experts, hidden, generator=gen, device="cuda") * 0.1
+    gate_up = (torch.randn(experts, 2 * ffn, hidden, generator=gen, device="cuda") * hidden ** -0.5).bfloat16()
+    down = (torch.randn(experts, hidden, ffn, generator=gen, device="cuda") * ffn ** -0.5).bfloat16()
+    block = torch_ops.Experts(router, gate_up, down, top, eight_bit=eight_bit)
+    y = block(x)
+    want = experts64(x, router, gate_up, down, top)
+    assert y.shape == x.shape and y.dtype == x.dtype
+    off = torch.linalg.vector_norm(y.double() - want) / torch.linalg.vector_norm(want)
+    assert off <= (0.094 if eight_bit else 2.0 ** -7)
+    assert torch.equal(block(x), y)
+
+
+@gpu
+def test_experts_in_a_graph(cuda_device):
+    """The sizes of the groups stay on the device: one captured graph serves other tokens."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    hidden, ffn, experts, top = 256, 256, 8, 2
+    router = torch.randn(experts, hidden, generator=gen, device="cuda") * 0.2
+    gate_up = (torch.randn(experts, 2 * ffn, hidden, generator=gen, device="cuda") * hidden ** -0.5).bfloat16()
+    down = (torch.randn(experts, hidden, ffn, generator=gen, device="cuda") * ffn ** -0.5).bfloat16()
+    block = torch_ops.Experts(router, gate_up, down, top, eight_bit=True)
+    x = torch.randn(24, hidden, generator=gen, device="cuda").bfloat16()
+    other = torch.randn(24, hidden, generator=gen, device="cuda").bfloat16()
+    want = block(other)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = block(x)
+    x.copy_(other)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
