@@ -216,10 +216,12 @@ def make_desc(m, n, k, dtype, *, a_strides=None, b_strides=None, c_strides=None,
 def _ptr(x):
     if x is None:
         return None
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError("expected an address, a torch tensor or a numpy array")

@@ -71,14 +71,19 @@ int ensure_device(Handle *h)
     if (rc != KUDNN_B200_OK) {
         return rc;
     }
+    // cleared on a stream of its own: the first run may be captured on a stream that the default stream would wait for
     void *status = nullptr;
+    cudaStream_t aside = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    (void)cudaThreadExchangeStreamCaptureMode(&mode);
     cudaError_t e = kb::library_malloc(&status, sizeof(kb::DeviceStatus));
-    if (e == cudaSuccess) {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        (void)cudaThreadExchangeStreamCaptureMode(&mode);
-        e = cudaMemset(status, 0, sizeof(kb::DeviceStatus));
-        (void)cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&aside, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(status, 0, sizeof(kb::DeviceStatus), aside);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(aside);
+    if (aside != nullptr) {
+        cudaStreamDestroy(aside);
     }
+    (void)cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) {
         cudaFree(status);
         return fail_cuda(e, "grouped: status block");

@@ -283,6 +283,38 @@ def test_streams_and_graphs(cuda_device, dtype):
 
 
 @gpu
+def test_the_first_run_of_a_handle_may_be_captured(cuda_device):
+    p = Problem(33, 136, 256, "e4m3", sizes=[3, 30])
+    y, tol = p.exact()
+    op = kb.Grouped(p.desc)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        graph.capture_begin(capture_error_mode="thread_local")
+        op.run(p.a, p.b, p.c, offsets=p.offsets, a_scale=p.a_scale, b_scale=p.b_scale, stream=stream.cuda_stream)
+        graph.capture_end()
+    for _ in range(3):
+        p.c.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool(((p.c.double() - y).abs() <= tol).all())
+    op.check()
+
+
+@gpu
+def test_rows_that_share_memory(cuda_device):
+    """Operands broadcast with a stride of zero."""
+    p = Problem(20, 72, 96, "bf16", sizes=[5, 15])
+    want = p.a[:1].double() @ p.b3[1].double().t()
+    p.desc.a_sm = 0
+    p.run()
+    assert p.kernel == kb.KERNEL_SIMT
+    limit = (96 / 8 + 8) * 2.0 ** -23 * (p.a[:1].double().abs() @ p.b3[1].double().abs().t()) + 2.0 ** -8 * want.abs()
+    assert bool(((p.c[5:].double() - want).abs() <= limit).all())
+
+
+@gpu
 def test_large_offsets(cuda_device):
     """Rows of a and c, and weights, whose elements lie beyond 2^31."""
     p = Problem(3000, 128, 256, "bf16", sizes=[2990, 10], a_ld=1 << 20, c_ld=1 << 20)
