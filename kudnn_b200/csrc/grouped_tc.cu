@@ -22,12 +22,12 @@ bool pitch_fits(long long pitch, long long inner, int es)
     return pitch >= inner && pitch * es % 16 == 0 && pitch * es < (1ll << 40);
 }
 
-template <bool kScaled, int kTN, bool kRows = false>
+template <int kMode, int kTN, bool kRows = false>
 cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bound, int sm_count, const CUtensorMap &tb, cudaStream_t stream)
 {
-    using S = Shape<kScaled, kTN, kRows>;
-    constexpr int es = kScaled ? 1 : 2;
-    auto kernel = grouped_tc_kernel<kScaled, kTN, kRows>;
+    using S = Shape<kMode, kTN, kRows>;
+    constexpr int es = S::kScaled ? 1 : 2;
+    auto kernel = grouped_tc_kernel<kMode, kTN, kRows>;
     static std::atomic<unsigned long long> prepared{0};  // devices, a bit each
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -116,9 +116,10 @@ int choose_tile(const GroupedParams &g, const TcParams &p, bool scaled, bool tal
     return best;
 }
 
-template <bool kScaled>
+template <int kMode>
 cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &tb, cudaStream_t stream)
 {
+    constexpr bool kScaled = kMode == kWithScales;
     // Tall tiles of scaled products: rows on the M side, unless the groups' last tiles, which that pads to 256 rows, would take more than the
     // faster sums save (850 against 1170 cycles per block of K).
     const bool tall_on_m = kScaled && (g.offsets == nullptr || g.rows >= 192ll * g.groups);
@@ -134,14 +135,14 @@ cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const
             if (p.vec != 0 && g.c_sm * dtype_size(g.c_dtype) % 32 == 0 && reinterpret_cast<uintptr_t>(g.c) % 32 == 0) {
                 p.vec = 2;
             }
-            return launch_shape<true, 256, true>(g, p, bound, sm_count, tb, stream);
+            return launch_shape<kWithScales, 256, true>(g, p, bound, sm_count, tb, stream);
         }
     }
     switch (tn) {
-        case 32: return launch_shape<kScaled, 32>(g, p, bound, sm_count, tb, stream);
-        case 64: return launch_shape<kScaled, 64>(g, p, bound, sm_count, tb, stream);
-        case 128: return launch_shape<kScaled, 128>(g, p, bound, sm_count, tb, stream);
-        default: return launch_shape<kScaled, 256>(g, p, bound, sm_count, tb, stream);
+        case 32: return launch_shape<kMode, 32>(g, p, bound, sm_count, tb, stream);
+        case 64: return launch_shape<kMode, 64>(g, p, bound, sm_count, tb, stream);
+        case 128: return launch_shape<kMode, 128>(g, p, bound, sm_count, tb, stream);
+        default: return launch_shape<kMode, 256>(g, p, bound, sm_count, tb, stream);
     }
 }
 
@@ -178,7 +179,12 @@ cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus
     p.load_kb = skip_kblock >= 0 ? std::min(skip_kblock, p.num_kb) : p.num_kb;
     p.status = status;
     p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimitCycles;
-    return scaled ? launch_kind<true>(g, p, sm_count, tb, stream) : launch_kind<false>(g, p, sm_count, tb, stream);
+    p.drain = 4;
+    if (scaled) {
+        return launch_kind<kWithScales>(g, p, sm_count, tb, stream);
+    }
+    return g.c_dtype == KUDNN_B200_F32 && p.num_kb > p.drain ? launch_kind<kDrained>(g, p, sm_count, tb, stream)
+                                                              : launch_kind<kPlain>(g, p, sm_count, tb, stream);
 }
 
 }  // namespace kb

@@ -20,9 +20,13 @@
 // Scaled products of tall tiles stand the other way round: rows on the M side, 256 weight rows on the N side.  A lane then holds a row
 // and a warp the columns of one scale, so that an accumulator element costs one FMA with a scalar of the thread (327 cycles per 128 x 256)
 // and rows are stored straight from registers; a group's last tile is padded to 256 rows instead of 32.  Measured in the kernel, cycles
-// per block of K: weights on the M side 1170, of which the sums 760.
+// per block of K: weights on the M side 1170, of which the sums 760; rows on the M side 860, of which the MMAs 512.
 //
-// Few items: clusters of up to 8 CTAs cut K, exchange their partial sums through distributed shared memory and add them in rank order.
+// What bounds tall scaled tiles (4096 x 11008 x 4096, 171 us in short runs; each part taken out in turn): copies alone 84 us, with the MMAs
+// and the exchange of buffers 121, with the loads from tensor memory 134, with the FMAs 148; the rest is a tile's results, in which the
+// MMAs stand still but for the two blocks that tensor memory holds.  In runs of seconds the board's power cap takes the clock to 1.4 GHz.
+//
+// Few items: clusters of two or four CTAs cut K, exchange their partial sums through distributed shared memory and add them in rank order.
 #pragma once
 
 #include "grouped.cuh"
@@ -49,9 +53,15 @@ constexpr int kControlRegs = 88, kSumRegs = 208;
 static_assert(128 * kControlRegs + 256 * kSumRegs <= 384 * 168, "register split");
 constexpr int kBarrierBytes = (2 * kMaxStages + 2 * kMaxBuffers + 2 * kScaleSlots) * 8 + 16;
 
+// How the blocks of K add up: in tensor memory; in fp32 registers with their scales (e4m3); or there without, p.drain blocks at a time, for
+// fp32 results of 16-bit operands.  The tensor cores cut every addition, always towards zero: 3000 x 1024 x 8192 is 1.0e-5 off in the
+// norm when all of it stays in tensor memory, and 16-bit results do not see that, but fp32 ones do.
+constexpr int kPlain = 0, kWithScales = 1, kDrained = 2;
+
 // kRows: the rows of the group on the M side (see above)
-template <bool kScaled, int kTN, bool kRows>
+template <int kMode, int kTN, bool kRows>
 struct Shape {
+    static constexpr bool kScaled = kMode == kWithScales, kSums = kMode != kPlain;
     static_assert(!kRows || (kScaled && kTN == 256), "rows on the M side: scaled products of tall tiles");
     static constexpr bool kPair = kTN == 256;
     // Short tiles are bound by the weights' bytes: small CTAs, of which two or three share an SM, keep many copies in flight and even out
@@ -60,7 +70,7 @@ struct Shape {
     static constexpr int kSumWarps = kTN <= 64 ? 4 : 8;
     static constexpr int kWays = kSumWarps / 4;               // warps that share a quarter of the lanes: they take chunks in turn
     static constexpr int kThreads = kControlThreads + 32 * kSumWarps;
-    static constexpr int kBuffers = kScaled ? (kTN == 256 ? 2 : 4) : 2;
+    static constexpr int kBuffers = kSums && kTN != 256 ? 4 : 2;
     static constexpr int kTmemCols = kBuffers * kTN;
     static constexpr int kChunk = kTN >= 64 ? 32 : 16;        // columns a warp takes at a time
     static constexpr int kChunks = kTN / kChunk / kWays;      // per warp
@@ -83,6 +93,7 @@ struct TcParams {
     int kb_elems;      // elements in one
     int tiles_n;       // of 128 weight rows, 256 for pairs
     int splits, kb_per_split;
+    int drain;         // kDrained: blocks of K that add up in tensor memory
     int stages;
     int band;          // row tiles that share the weight tiles of a raster band
     int vec;           // 1: rows of c are contiguous, four of their elements aligned, and finish_unit knows the activation; 2: 32-byte aligned too
@@ -420,7 +431,7 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
                                          int warp, int lane, uint32_t tmem_base, uint64_t *tmem_full, uint64_t *tmem_empty, uint32_t units_at,
                                          uint32_t bias_at, volatile int *abort_flag)
 {
-    constexpr int kBuffers = Shape<true, 256, true>::kBuffers;
+    constexpr int kBuffers = Shape<kWithScales, 256, true>::kBuffers;
     const GroupedParams &g = p.g;
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int row_in_tile = rank * 128 + quarter * 32 + lane;
@@ -605,11 +616,12 @@ __device__ __forceinline__ void sum_rows(const TcParams &p, const int *begins, c
     }
 }
 
-template <bool kScaled, int kTN, bool kRows>
-__global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kScaled, kTN, kRows>::kCtas)
+template <int kMode, int kTN, bool kRows>
+__global__ void __launch_bounds__(Shape<kMode, kTN, kRows>::kThreads, Shape<kMode, kTN, kRows>::kCtas)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ TcParams p)
 {
-    using S = Shape<kScaled, kTN, kRows>;
+    using S = Shape<kMode, kTN, kRows>;
+    constexpr bool kScaled = S::kScaled, kSums = S::kSums;
     extern __shared__ __align__(1024) unsigned char smem[];
     constexpr int kThreads = S::kThreads, kSumWarps = S::kSumWarps;
     unsigned char *behind_ring = smem + p.stages * S::kStageBytes;
@@ -748,7 +760,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
     }
 
     if (warp < 4) {
-        if (kScaled && kTN == 256) {
+        if (kSums && kTN == 256) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
         }
         // The whole warp runs a role's loop and one lane issues: what an instruction needs then lies in uniform registers.
@@ -805,8 +817,9 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
             for (int item = first_item; alive && item < num_items; item += stride) {
                 const Item w = find_item<kTN, kRows>(p, begins, items, item);
                 const uint32_t idesc = p.idesc | (kRows ? 0u : static_cast<uint32_t>(w.cols >> 3) << 17);
+                int held = 0;  // blocks that the buffer has added up
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
-                    if (kScaled || kb == kb_begin) {
+                    if (held == 0) {
                         alive = warp_wait(mbar_test(tmem_empty + buffer, buffer_phase ^ 1u), tmem_empty + buffer, buffer_phase ^ 1u, abort_flag,
                                           p.status, 2, p.wait_limit);
                     }
@@ -819,7 +832,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                     const uint64_t first = make_smem_desc(at), second = make_smem_desc(at + kWeightBytes);
                     const uint64_t mdesc = kRows ? second : first, ndesc = kRows ? first : second;
                     const uint32_t to = tmem_base + static_cast<uint32_t>(buffer * kTN);
-                    const bool whole = kScaled || kb + 1 == kb_end;  // the buffer is complete
+                    const bool whole = kScaled || kb + 1 == kb_end || (kSums && held + 1 == p.drain);  // the buffer is complete
                     const int this_stage = stage;
                     if (++stage == p.stages) {
                         stage = 0;
@@ -830,7 +843,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
                             const uint64_t d = static_cast<uint64_t>(2 * ks);
-                            const uint32_t more = ks != 0 || (!kScaled && kb != kb_begin) ? 1u : 0u;
+                            const uint32_t more = ks != 0 || held != 0 ? 1u : 0u;
                             if (kScaled) {
                                 umma_f8<S::kPair>(to, mdesc + d, ndesc + d, idesc, more);
                             } else if (S::kPair) {
@@ -852,6 +865,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                         }
                     }
                     __syncwarp();
+                    held = whole ? 0 : held + 1;
                     if (whole && ++buffer == S::kBuffers) {
                         buffer = 0;
                         buffer_phase ^= 1u;
@@ -908,7 +922,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
             }
         }
     } else {
-        if (kScaled && kTN == 256) {
+        if (kSums && kTN == 256) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         }
         // ---------------------------------------------------------------------- sums and results
@@ -946,8 +960,8 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                 bias_lane = load_as_f32(p.g.bias, p.g.bias_dtype, w.group * p.g.bias_sg + (n_warp + lane) * p.g.bias_sn);
             }
             bool alive = true;
-            float sum[kScaled ? S::kChunks : 1][2][kRegs];  // 16 lanes each
-            if (kScaled) {
+            float sum[kSums ? S::kChunks : 1][2][kRegs];  // 16 lanes each
+            if (kSums) {
 #pragma unroll
                 for (int i = 0; i < S::kChunks; ++i) {
 #pragma unroll
@@ -957,10 +971,10 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                     }
                 }
 #pragma unroll 1
-                for (int kb = kb_begin; kb < kb_end; ++kb) {
-                    const bool scales_there = mbar_test(scale_full + slot, slot_phase);
+                for (int kb = kb_begin; kb < kb_end; kb += kScaled ? 1 : p.drain) {
+                    const bool scales_there = !kScaled || mbar_test(scale_full + slot, slot_phase);
                     const bool sums_there = mbar_test(tmem_full + buffer, buffer_phase);
-                    alive = warp_wait(scales_there, scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit) &&
+                    alive = (!kScaled || warp_wait(scales_there, scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit)) &&
                             warp_wait(sums_there, tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
                     if (!alive) {
                         break;
@@ -979,24 +993,27 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                         tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
                         float s[S::kChunk / 4];
 #pragma unroll
-                        for (int u = 0; u < S::kChunk / 16; ++u) {
+                        for (int u = 0; kScaled && u < S::kChunk / 16; ++u) {
                             load_shared_4(scale_at + static_cast<uint32_t>((c0 + u * 16) * 4), s + 4 * u);
                         }
                         tmem_wait(lo);
                         tmem_wait(hi);
 #pragma unroll
                         for (int j = 0; j < kRegs; ++j) {
-                            sum[i][0][j] = fmaf(__uint_as_float(lo[j]), s[j / 2], sum[i][0][j]);
-                            sum[i][1][j] = fmaf(__uint_as_float(hi[j]), s[j / 2], sum[i][1][j]);
+                            const float scale = kScaled ? s[j / 2] : 1.0f;
+                            sum[i][0][j] = fmaf(__uint_as_float(lo[j]), scale, sum[i][0][j]);
+                            sum[i][1][j] = fmaf(__uint_as_float(hi[j]), scale, sum[i][1][j]);
                         }
                     }
                     release();
-                    if (lane == 0) {
-                        mbar_arrive(scale_empty + slot);
-                    }
-                    if (++slot == kScaleSlots) {
-                        slot = 0;
-                        slot_phase ^= 1u;
+                    if (kScaled) {
+                        if (lane == 0) {
+                            mbar_arrive(scale_empty + slot);
+                        }
+                        if (++slot == kScaleSlots) {
+                            slot = 0;
+                            slot_phase ^= 1u;
+                        }
                     }
                 }
             } else {
@@ -1022,7 +1039,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                 const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
                 // column 4j + lane % 4, row lane / 4 (+ 8 and 16)
                 const uint32_t put_at = unit_at + static_cast<uint32_t>(((lane & 3) * kUnitPitch + lane / 4) * 4);
-                if (kScaled) {
+                if constexpr (kSums) {
                     __syncwarp();
                     auto put = [&](auto which) {
                         constexpr int v = decltype(which)::value;
@@ -1072,7 +1089,7 @@ __global__ void __launch_bounds__(Shape<kScaled, kTN, kRows>::kThreads, Shape<kS
                     }
                 }
             }
-            if (!kScaled) {
+            if (!kSums) {
                 release();
             }
         }

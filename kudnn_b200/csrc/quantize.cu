@@ -86,8 +86,8 @@ __device__ __forceinline__ const void *source_row(const QuantizeParams &p, int r
 
 // Rows on 16-byte boundaries: 8 lanes per block of 128 columns, 16 columns each, everything in registers between one read and one write.
 //
-// Bound by HBM: 2 to 5 bytes read and 1.03 written per element, about twelve instructions per gated one.  8192 x 11008 gated bf16 values
-// take MEASURED_GATE.
+// Bound by HBM: 2 to 8 bytes read and 1.03 written per element, about twelve instructions per gated one.  8192 x 11008 gated bf16 values
+// take 77 us (5.87 TB/s, 0.89 of a copy's rate); read and written element by element 238 us.
 template <typename T, bool kGate>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constant__ QuantizeParams p)
 {
@@ -161,7 +161,9 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
 }
 
 // Rows that begin anywhere: a warp takes four blocks of columns, every lane each 32nd, so that its accesses lie side by side however they
-// are aligned.  9001 rows of 4099 fp16 values, gathered from 1501, take MEASURED_ROUTED.
+// are aligned.  Bound by instructions (the schedulers issue in 74 % of the cycles): 9001 rows of 4099 fp16 values, gathered from 1501, take
+// 25 us; 41 us where every lane divided for every block and each block was reduced by itself, and no less with four neighbouring columns
+// per lane and 4-byte stores.
 template <typename T, bool kGate>
 __global__ void __launch_bounds__(128) quantize_any_kernel(const __grid_constant__ QuantizeParams p)
 {
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(128) quantize_any_kernel(const __grid_constant
     }
 }
 
-// One CTA per 128 x 128 block, for weights: a warp takes 16 rows, a lane 4 columns.
+// One CTA per 128 x 128 block, for weights, once per layer: a warp takes 16 rows, a lane 4 columns.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const __grid_constant__ QuantizeParams p)
 {

@@ -247,6 +247,17 @@ def test_no_rows(cuda_device):
 
 @gpu
 @pytest.mark.parametrize("dtype", OPERANDS)
+@pytest.mark.parametrize("m,k", [(3, 8192), (50, 2000), (100, 8192), (700, 8192), (1, 520)])
+def test_fp32_results_keep_their_bits(cuda_device, dtype, m, k):
+    """256 products at most add up in the tensor cores before fp32 registers take over: 16 cuts of up to 2^-23, half of it on average, of sums
+    that are half of the last one on average, 2^-21 in the norm; as much again for the fp32 additions."""
+    p = Problem(m, 384, k, dtype, sizes=[m - m // 3, m // 3], out="f32").check()
+    y, _ = p.exact()
+    assert torch.linalg.vector_norm(p.c.double() - y) <= 2.0 ** -20 * torch.linalg.vector_norm(y)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", OPERANDS)
 def test_the_same_bits_every_time(cuda_device, dtype):
     p = Problem(16, 512, 4096, dtype)
     first = p.run().c.clone()
