@@ -27,6 +27,8 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi)
     return r;
 }
 
+// silu(gate) * up.  The approximate exponential and reciprocal (about 1e-6 relative) for 16-bit values: in libm grade 8192 x 11008 of them take
+// 110 us instead of 82, and as many end on the other side of one of e4m3's rounding boundaries.
 template <bool kPrecise>
 __device__ __forceinline__ float gated(float gate, float up)
 {
