@@ -8,8 +8,9 @@
 // alone would need 48 KiB per block of K, a pair needs 32, and 148 SMs that take 48 KiB every 512 cycles are more than L2 delivers.
 //
 // Roles: warp 0 loads (TMA), warp 1 issues MMAs, warp 2 fetches the scales, warps 4-11 (4-7 for short tiles) take the accumulators: a warp
-// owns 32 TMEM lanes (weight rows) and, where there are eight, every other chunk of columns (rows of the group).  CTAs are persistent; work item = (group, rows
-// tile, weight rows), found by a search in the groups' running item counts, which every CTA builds from the offsets.
+// owns 32 TMEM lanes (weight rows) and, where there are eight, every other chunk of columns (rows of the group).  CTAs are persistent; a
+// work item = (group, rows tile, weight rows) is found by a search in the groups' running item counts, which every CTA builds from the
+// offsets.
 //
 // Scales.  The accumulator of a block of 128 k leaves tensor memory by itself (two to four buffers take turns) and is added to fp32
 // registers with the product of its scales.  Tensor memory is read as 16 lanes x 128 bits, so that a thread holds every fourth column and
@@ -930,169 +931,169 @@ __global__ void __launch_bounds__(Shape<kMode, kTN, kRows>::kThreads, Shape<kMod
             sum_rows(p, begins, items, num_items, first_item, stride, rank, warp, lane, tmem_base, tmem_full, tmem_empty, smem_u32(units),
                      smem_u32(bias_area), abort_flag);
         } else {
-        constexpr int kRegs = S::kChunk / 2;  // registers of 16 lanes x a chunk of columns
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        const uint32_t my_bias = smem_u32(bias_area) + static_cast<uint32_t>((warp - 4) * 128);
-        const uint32_t lanes_at = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t drained = S::kPair ? map_to_rank(smem_u32(tmem_empty), 0u) : 0u;
-        int buffer = 0, slot = 0;
-        uint32_t buffer_phase = 0, slot_phase = 0;
-        auto release = [&]() {  // the MMAs may have the buffer again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (S::kPair) {
-                    mbar_arrive_cluster(drained + static_cast<uint32_t>(buffer * 8));
-                } else {
-                    mbar_arrive(tmem_empty + buffer);
-                }
-            }
-            if (++buffer == S::kBuffers) {
-                buffer = 0;
-                buffer_phase ^= 1u;
-            }
-        };
-        for (int item = first_item; item < num_items; item += stride) {
-            const Item w = find_item<kTN, kRows>(p, begins, items, item);
-            const int n_warp = w.n0 + my_n + quarter * 32;
-            float bias_lane = 0.0f;
-            if (p.g.has_bias != 0 && n_warp + lane < p.g.n) {
-                bias_lane = load_as_f32(p.g.bias, p.g.bias_dtype, w.group * p.g.bias_sg + (n_warp + lane) * p.g.bias_sn);
-            }
-            bool alive = true;
-            float sum[kSums ? S::kChunks : 1][2][kRegs];  // 16 lanes each
-            if (kSums) {
-#pragma unroll
-                for (int i = 0; i < S::kChunks; ++i) {
-#pragma unroll
-                    for (int j = 0; j < kRegs; ++j) {
-                        sum[i][0][j] = 0.0f;
-                        sum[i][1][j] = 0.0f;
+            constexpr int kRegs = S::kChunk / 2;  // registers of 16 lanes x a chunk of columns
+            const int quarter = warp & 3, half = (warp - 4) >> 2;
+            const uint32_t my_bias = smem_u32(bias_area) + static_cast<uint32_t>((warp - 4) * 128);
+            const uint32_t lanes_at = static_cast<uint32_t>(quarter * 32) << 16;
+            const uint32_t drained = S::kPair ? map_to_rank(smem_u32(tmem_empty), 0u) : 0u;
+            int buffer = 0, slot = 0;
+            uint32_t buffer_phase = 0, slot_phase = 0;
+            auto release = [&]() {  // the MMAs may have the buffer again
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (S::kPair) {
+                        mbar_arrive_cluster(drained + static_cast<uint32_t>(buffer * 8));
+                    } else {
+                        mbar_arrive(tmem_empty + buffer);
                     }
                 }
-#pragma unroll 1
-                for (int kb = kb_begin; kb < kb_end; kb += kScaled ? 1 : p.drain) {
-                    const bool scales_there = !kScaled || mbar_test(scale_full + slot, slot_phase);
-                    const bool sums_there = mbar_test(tmem_full + buffer, buffer_phase);
-                    alive = (!kScaled || warp_wait(scales_there, scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit)) &&
-                            warp_wait(sums_there, tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
-                    if (!alive) {
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t from = tmem_base + lanes_at + static_cast<uint32_t>(buffer * kTN);
-                    const uint32_t scale_at = smem_u32(scales) + static_cast<uint32_t>(slot * kTN * 4 + (lane & 3) * 16);
+                if (++buffer == S::kBuffers) {
+                    buffer = 0;
+                    buffer_phase ^= 1u;
+                }
+            };
+            for (int item = first_item; item < num_items; item += stride) {
+                const Item w = find_item<kTN, kRows>(p, begins, items, item);
+                const int n_warp = w.n0 + my_n + quarter * 32;
+                float bias_lane = 0.0f;
+                if (p.g.has_bias != 0 && n_warp + lane < p.g.n) {
+                    bias_lane = load_as_f32(p.g.bias, p.g.bias_dtype, w.group * p.g.bias_sg + (n_warp + lane) * p.g.bias_sn);
+                }
+                bool alive = true;
+                float sum[kSums ? S::kChunks : 1][2][kRegs];  // 16 lanes each
+                if (kSums) {
 #pragma unroll
                     for (int i = 0; i < S::kChunks; ++i) {
-                        const int c0 = (S::kWays * i + half) * S::kChunk;
-                        if (c0 >= w.cols) {
-                            break;
-                        }
-                        uint32_t lo[kRegs], hi[kRegs];
-                        tmem_load(from + static_cast<uint32_t>(c0), lo);
-                        tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
-                        float s[S::kChunk / 4];
-#pragma unroll
-                        for (int u = 0; kScaled && u < S::kChunk / 16; ++u) {
-                            load_shared_4(scale_at + static_cast<uint32_t>((c0 + u * 16) * 4), s + 4 * u);
-                        }
-                        tmem_wait(lo);
-                        tmem_wait(hi);
 #pragma unroll
                         for (int j = 0; j < kRegs; ++j) {
-                            const float scale = kScaled ? s[j / 2] : 1.0f;
-                            sum[i][0][j] = fmaf(__uint_as_float(lo[j]), scale, sum[i][0][j]);
-                            sum[i][1][j] = fmaf(__uint_as_float(hi[j]), scale, sum[i][1][j]);
+                            sum[i][0][j] = 0.0f;
+                            sum[i][1][j] = 0.0f;
                         }
                     }
-                    release();
-                    if (kScaled) {
-                        if (lane == 0) {
-                            mbar_arrive(scale_empty + slot);
-                        }
-                        if (++slot == kScaleSlots) {
-                            slot = 0;
-                            slot_phase ^= 1u;
-                        }
-                    }
-                }
-            } else {
-                alive = warp_wait(mbar_test(tmem_full + buffer, buffer_phase), tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
-                tc_fence_after();
-            }
-            if (!alive) {
-                break;
-            }
-            store_shared(my_bias + static_cast<uint32_t>(lane * 4), bias_lane);
-            __syncwarp();
-            float bias[4];
-            load_shared_4(my_bias + static_cast<uint32_t>((lane & 7) * 16), bias);
-            const uint32_t from = tmem_base + lanes_at + static_cast<uint32_t>(buffer * kTN);
-            constexpr int kUnitsPerChunk = S::kChunk / 16;
 #pragma unroll 1
-            for (int u = 0; u < S::kChunks * kUnitsPerChunk; ++u) {
-                const int c0 = (S::kWays * (u / kUnitsPerChunk) + half) * S::kChunk + u % kUnitsPerChunk * 16;
-                if (c0 >= w.cols) {
-                    break;
-                }
-                const int unit = p.splits > 1 ? c0 / 16 * 4 + quarter : warp - 4;
-                const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
-                // column 4j + lane % 4, row lane / 4 (+ 8 and 16)
-                const uint32_t put_at = unit_at + static_cast<uint32_t>(((lane & 3) * kUnitPitch + lane / 4) * 4);
-                if constexpr (kSums) {
-                    __syncwarp();
-                    auto put = [&](auto which) {
-                        constexpr int v = decltype(which)::value;
-                        if constexpr (v < S::kChunks * kUnitsPerChunk) {
+                    for (int kb = kb_begin; kb < kb_end; kb += kScaled ? 1 : p.drain) {
+                        const bool scales_there = !kScaled || mbar_test(scale_full + slot, slot_phase);
+                        const bool sums_there = mbar_test(tmem_full + buffer, buffer_phase);
+                        alive = (!kScaled || warp_wait(scales_there, scale_full + slot, slot_phase, abort_flag, p.status, 6, p.wait_limit)) &&
+                                warp_wait(sums_there, tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
+                        if (!alive) {
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t from = tmem_base + lanes_at + static_cast<uint32_t>(buffer * kTN);
+                        const uint32_t scale_at = smem_u32(scales) + static_cast<uint32_t>(slot * kTN * 4 + (lane & 3) * 16);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {  // j: lanes' half, column / 4, lanes' eight
-                                store_shared(put_at + static_cast<uint32_t>(((j >> 1 & 3) * 4 * kUnitPitch + (j >> 3) * 16 + (j & 1) * 8) * 4),
-                                             sum[v / kUnitsPerChunk][j >> 3][v % kUnitsPerChunk * 8 + (j & 7)]);
+                        for (int i = 0; i < S::kChunks; ++i) {
+                            const int c0 = (S::kWays * i + half) * S::kChunk;
+                            if (c0 >= w.cols) {
+                                break;
+                            }
+                            uint32_t lo[kRegs], hi[kRegs];
+                            tmem_load(from + static_cast<uint32_t>(c0), lo);
+                            tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
+                            float s[S::kChunk / 4];
+#pragma unroll
+                            for (int u = 0; kScaled && u < S::kChunk / 16; ++u) {
+                                load_shared_4(scale_at + static_cast<uint32_t>((c0 + u * 16) * 4), s + 4 * u);
+                            }
+                            tmem_wait(lo);
+                            tmem_wait(hi);
+#pragma unroll
+                            for (int j = 0; j < kRegs; ++j) {
+                                const float scale = kScaled ? s[j / 2] : 1.0f;
+                                sum[i][0][j] = fmaf(__uint_as_float(lo[j]), scale, sum[i][0][j]);
+                                sum[i][1][j] = fmaf(__uint_as_float(hi[j]), scale, sum[i][1][j]);
                             }
                         }
-                    };
-                    switch (u) {  // the registers' numbers are fixed
-                        case 0: put(std::integral_constant<int, 0>()); break;
-                        case 1: put(std::integral_constant<int, 1>()); break;
-                        case 2: put(std::integral_constant<int, 2>()); break;
-                        case 3: put(std::integral_constant<int, 3>()); break;
-                        case 4: put(std::integral_constant<int, 4>()); break;
-                        case 5: put(std::integral_constant<int, 5>()); break;
-                        case 6: put(std::integral_constant<int, 6>()); break;
-                        default: put(std::integral_constant<int, 7>()); break;
+                        release();
+                        if (kScaled) {
+                            if (lane == 0) {
+                                mbar_arrive(scale_empty + slot);
+                            }
+                            if (++slot == kScaleSlots) {
+                                slot = 0;
+                                slot_phase ^= 1u;
+                            }
+                        }
                     }
                 } else {
-                    uint32_t lo[8], hi[8];
-                    tmem_load(from + static_cast<uint32_t>(c0), lo);
-                    tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
-                    tmem_wait(lo);
-                    tmem_wait(hi);
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t to = put_at + static_cast<uint32_t>(((j >> 1) * 4 * kUnitPitch + (j & 1) * 8) * 4);
-                        store_shared(to, __uint_as_float(lo[j]));
-                        store_shared(to + 64, __uint_as_float(hi[j]));
-                    }
+                    alive = warp_wait(mbar_test(tmem_full + buffer, buffer_phase), tmem_full + buffer, buffer_phase, abort_flag, p.status, 4, p.wait_limit);
+                    tc_fence_after();
                 }
+                if (!alive) {
+                    break;
+                }
+                store_shared(my_bias + static_cast<uint32_t>(lane * 4), bias_lane);
                 __syncwarp();
-                if (p.splits == 1) {
-                    if (p.vec != 0 && n_warp + 32 <= p.g.n) {
-                        float v[4][4];
+                float bias[4];
+                load_shared_4(my_bias + static_cast<uint32_t>((lane & 7) * 16), bias);
+                const uint32_t from = tmem_base + lanes_at + static_cast<uint32_t>(buffer * kTN);
+                constexpr int kUnitsPerChunk = S::kChunk / 16;
+#pragma unroll 1
+                for (int u = 0; u < S::kChunks * kUnitsPerChunk; ++u) {
+                    const int c0 = (S::kWays * (u / kUnitsPerChunk) + half) * S::kChunk + u % kUnitsPerChunk * 16;
+                    if (c0 >= w.cols) {
+                        break;
+                    }
+                    const int unit = p.splits > 1 ? c0 / 16 * 4 + quarter : warp - 4;
+                    const uint32_t unit_at = smem_u32(units) + static_cast<uint32_t>(unit * kUnitBytes);
+                    // column 4j + lane % 4, row lane / 4 (+ 8 and 16)
+                    const uint32_t put_at = unit_at + static_cast<uint32_t>(((lane & 3) * kUnitPitch + lane / 4) * 4);
+                    if constexpr (kSums) {
+                        __syncwarp();
+                        auto put = [&](auto which) {
+                            constexpr int v = decltype(which)::value;
+                            if constexpr (v < S::kChunks * kUnitsPerChunk) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            load_shared_4(unit_at + static_cast<uint32_t>(((lane / 8 + 4 * i) * kUnitPitch + (lane & 7) * 4) * 4), v[i]);
+                                for (int j = 0; j < 16; ++j) {  // j: lanes' half, column / 4, lanes' eight
+                                    store_shared(put_at + static_cast<uint32_t>(((j >> 1 & 3) * 4 * kUnitPitch + (j >> 3) * 16 + (j & 1) * 8) * 4),
+                                                 sum[v / kUnitsPerChunk][j >> 3][v % kUnitsPerChunk * 8 + (j & 7)]);
+                                }
+                            }
+                        };
+                        switch (u) {  // the registers' numbers are fixed
+                            case 0: put(std::integral_constant<int, 0>()); break;
+                            case 1: put(std::integral_constant<int, 1>()); break;
+                            case 2: put(std::integral_constant<int, 2>()); break;
+                            case 3: put(std::integral_constant<int, 3>()); break;
+                            case 4: put(std::integral_constant<int, 4>()); break;
+                            case 5: put(std::integral_constant<int, 5>()); break;
+                            case 6: put(std::integral_constant<int, 6>()); break;
+                            default: put(std::integral_constant<int, 7>()); break;
                         }
-                        finish_unit(p.g, w.row0 + c0, w.count - c0, n_warp + (lane & 7) * 4, bias, v, lane);
                     } else {
-                        finish_unit_any(p.g, w.row0 + c0, w.count - c0, n_warp, my_bias, unit_at, lane);
+                        uint32_t lo[8], hi[8];
+                        tmem_load(from + static_cast<uint32_t>(c0), lo);
+                        tmem_load(from + (16u << 16) + static_cast<uint32_t>(c0), hi);
+                        tmem_wait(lo);
+                        tmem_wait(hi);
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t to = put_at + static_cast<uint32_t>(((j >> 1) * 4 * kUnitPitch + (j & 1) * 8) * 4);
+                            store_shared(to, __uint_as_float(lo[j]));
+                            store_shared(to + 64, __uint_as_float(hi[j]));
+                        }
+                    }
+                    __syncwarp();
+                    if (p.splits == 1) {
+                        if (p.vec != 0 && n_warp + 32 <= p.g.n) {
+                            float v[4][4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                load_shared_4(unit_at + static_cast<uint32_t>(((lane / 8 + 4 * i) * kUnitPitch + (lane & 7) * 4) * 4), v[i]);
+                            }
+                            finish_unit(p.g, w.row0 + c0, w.count - c0, n_warp + (lane & 7) * 4, bias, v, lane);
+                        } else {
+                            finish_unit_any(p.g, w.row0 + c0, w.count - c0, n_warp, my_bias, unit_at, lane);
+                        }
                     }
                 }
+                if (!kSums) {
+                    release();
+                }
             }
-            if (!kSums) {
-                release();
-            }
-        }
         }
     }
 
