@@ -98,6 +98,22 @@ def test_gate(cuda_device, dtype, rows, k):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [1, 16])
+def test_gate_keeps_the_bits_of_the_scale(cuda_device, dtype, k):
+    """A gate and an up per row, so that the scale is silu(gate) * up / 448.  In units of 2^-24: the exponential 4 (2 in the last place), its
+    product with the gate, the sum with 1, the product with the inverse, that with up and the scale's division 1 each, the inverse 2."""
+    far = 60.0 if dtype == torch.float16 else 87.0  # e^-87 is a normal number, and times up above 1e-30, below which nothing is scaled up
+    gate = torch.linspace(-far, 40.0, 3001, device="cuda").to(dtype)
+    gate = gate[gate != 0]
+    up = torch.full_like(gate, 1e4 if dtype == torch.float16 else 1e36)
+    x = torch.cat([gate[:, None].expand(-1, k), up[:, None].expand(-1, k)], dim=1).contiguous()
+    _, scale = run(x, x.shape[0], k, gate=True)
+    want = (gate.double() * torch.sigmoid(gate.double()) * up.double()).abs() / 448.0
+    assert torch.all((scale[:, 0].double() - want).abs() <= 11 * 2.0 ** -24 * want)
+
+
+@gpu
 @pytest.mark.parametrize("rows,k", [(1, 256), (40, 4099), (77, 640)])
 @pytest.mark.parametrize("gate", [False, True])
 def test_index(cuda_device, rows, k, gate):
