@@ -161,6 +161,16 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+def _quantized(x, rows, k, block_rows):
+    """Uninitialised results of quantize beside x: q at a pitch of 16 bytes; the scales of one block of columns next to one another for
+    activations, as the products read them, row-major for weights."""
+    blocks_k, scale_rows = -(-k // capi.SCALE_BLOCK), -(-rows // block_rows)
+    q = x.new_empty((rows, _pitch(k)), dtype=torch.float8_e4m3fn)[:, :k]
+    if block_rows == 1:
+        return q, x.new_empty((blocks_k, scale_rows), dtype=torch.float32).t()
+    return q, x.new_empty((scale_rows, blocks_k), dtype=torch.float32)
+
+
 @torch.library.custom_op("kudnn_b200::quantize", mutates_args=(), device_types="cuda")
 def quantize(x: torch.Tensor, gate: bool = False, index: Optional[torch.Tensor] = None,
              block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -180,10 +190,7 @@ def quantize(x: torch.Tensor, gate: bool = False, index: Optional[torch.Tensor] 
     if x.stride(1) != 1 and x.shape[1] > 1:
         x = x.contiguous()
     rows, k = x.shape[0] if index is None else index.shape[0], x.shape[1] // 2 if gate else x.shape[1]
-    blocks_k, scale_rows = -(-k // capi.SCALE_BLOCK), -(-rows // block_rows)
-    q = torch.empty((rows, _pitch(k)), dtype=torch.float8_e4m3fn, device=x.device)[:, :k]
-    # the scales of one block of columns lie next to one another for activations, as the products read them; row-major for weights
-    scale = torch.empty((blocks_k, scale_rows), device=x.device).t() if block_rows == 1 else torch.empty((scale_rows, blocks_k), device=x.device)
+    q, scale = _quantized(x, rows, k, block_rows)
     if rows > 0:
         index = None if index is None else index.contiguous()
         desc = capi.make_quantize_desc(rows, k, _DTYPES[x.dtype], gate=gate, x_rows=x.shape[0], block_rows=block_rows,
@@ -196,11 +203,7 @@ def quantize(x: torch.Tensor, gate: bool = False, index: Optional[torch.Tensor] 
 @quantize.register_fake
 def _quantize_fake(x, gate=False, index=None, block_rows=1):
     rows, k = x.shape[0] if index is None else index.shape[0], x.shape[1] // 2 if gate else x.shape[1]
-    blocks_k, scale_rows = -(-k // capi.SCALE_BLOCK), -(-rows // block_rows)
-    q = x.new_empty((rows, _pitch(k)), dtype=torch.float8_e4m3fn)[:, :k]
-    if block_rows == 1:
-        return q, x.new_empty((blocks_k, scale_rows), dtype=torch.float32).t()
-    return q, x.new_empty((scale_rows, blocks_k), dtype=torch.float32)
+    return _quantized(x, rows, k, block_rows)
 
 
 def _grouped_handle(device, key, make):

@@ -29,6 +29,56 @@ def test_fake_implementations_propagate_shapes_without_a_device():
     assert y.shape == (7, 64) and y.dtype == torch.float32
 
 
+@pytest.fixture
+def bfloat16_by_default():
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    yield
+    torch.set_default_dtype(before)
+
+
+@pytest.mark.parametrize("more", [dict(), dict(block_rows=128)])
+def test_scales_hold_32_bits_whatever_the_default_type(bfloat16_by_default, monkeypatch, more):
+    """On the host: what the operator hands to the library, whose kernel writes 4 bytes per scale."""
+    got = {}
+
+    class _Nothing:
+        cuda_stream = 0
+
+        def __init__(self, *args):
+            pass
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *args):
+            pass
+
+    monkeypatch.setattr(torch_ops, "_on", _Nothing)
+    monkeypatch.setattr(torch.cuda, "current_stream", _Nothing)
+    monkeypatch.setattr(torch_ops.capi, "quantize", lambda desc, x, q, scale, index, stream: got.update(desc=desc, q=q, scale=scale))
+    x = torch.zeros(200, 300)
+    q, scale = torch_ops.quantize._init_fn(x, **more)
+    fake = ops.quantize(meta(200, 300), **more)
+    assert got["scale"] is scale and scale.dtype == torch.float32 and scale.numel() * 4 <= scale.untyped_storage().nbytes()
+    for own, other in zip((q, scale), fake):
+        assert (own.dtype, own.shape, own.stride()) == (other.dtype, other.shape, other.stride())
+    assert got["desc"].s_row == scale.stride(0) and got["desc"].s_col == scale.stride(1) and got["desc"].q_ld == q.stride(0)
+
+
+@gpu
+def test_quantize_under_another_default_type(cuda_device, bfloat16_by_default):
+    x = torch.randn(37, 520, device="cuda", dtype=torch.float32)
+    for block_rows in (1, 128):
+        made = torch_ops._quantized(x, 37, 520, block_rows)[1]
+        assert made.dtype == torch.float32 and made.untyped_storage().nbytes() == 4 * made.numel()  # before anything is launched
+        q, scale = ops.quantize(x, block_rows=block_rows)
+        torch.set_default_dtype(torch.float32)
+        q2, scale2 = ops.quantize(x, block_rows=block_rows)
+        torch.set_default_dtype(torch.bfloat16)
+        assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(scale, scale2)
+
+
 class _Recorded:
     def __init__(self, desc):
         self.closed = False
