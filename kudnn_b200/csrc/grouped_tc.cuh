@@ -1097,6 +1097,30 @@ __global__ void __launch_bounds__(Shape<kMode, kTN, kRows>::kThreads, Shape<kMod
         }
     }
 
+    // ---------------------------------------------------------------------- teardown
+    // Tensor memory goes back before a CTA waits for others of its cluster: launches on two streams that share SMs could each hold what
+    // the other's CTAs, and with them its own, wait for.
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*abort_flag != 0) {
+        // give copies and MMAs that were already issued time to land before the memory is handed back
+        const long long t0 = clock64();
+        while (clock64() - t0 < 400000ll) {
+            __nanosleep(1000);
+        }
+        __syncthreads();
+    }
+    if (S::kPair) {
+        cluster_barrier();  // neither CTA leaves while the other's MMAs or arrivals may still reach it
+    }
+    if (warp == 1 && S::kPair) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+    } else if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+    }
+
     if (S::kSplits && p.splits > 1) {
         // ---------------------------------------------------------------------- partial sums of the cluster, in rank order
         __syncwarp();
@@ -1145,28 +1169,6 @@ __global__ void __launch_bounds__(Shape<kMode, kTN, kRows>::kThreads, Shape<kMod
         }
         __syncwarp();
         cluster_barrier();  // no CTA leaves while another still reads its shared memory
-    }
-
-    // ---------------------------------------------------------------------- teardown
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (*abort_flag != 0) {
-        // give copies and MMAs that were already issued time to land before the memory is handed back
-        const long long t0 = clock64();
-        while (clock64() - t0 < 400000ll) {
-            __nanosleep(1000);
-        }
-        __syncthreads();
-    }
-    if (S::kPair) {
-        cluster_barrier();  // neither CTA leaves while the other's MMAs or arrivals may still reach it
-    }
-    if (warp == 1 && S::kPair) {
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
-    } else if (warp == 1) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
     }
 }
 
