@@ -1881,6 +1881,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
 
+    // ---------------------------------------------------------------------- teardown
+    // Tensor memory goes back before a CTA waits for others that cut K with it: launches on two streams that share SMs could each hold
+    // what the other's CTAs, and with them its own, wait for.
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*abort_flag != 0) {
+        // give copies and MMAs that were already issued time to land before the memory is handed back
+        const long long t0 = clock64();
+        while (clock64() - t0 < 400000ll) {
+            __nanosleep(1000);
+        }
+        __syncthreads();
+    }
+    if (kPair) {
+        // neither CTA frees tensor memory or leaves while the other may still signal its barriers or, through the
+        // leader's MMAs, use its shared and tensor memory
+        cluster_sync_all();
+    }
+    if (warp == 1) {
+        if (kPair) {
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+        } else {
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+        }
+    }
+
     if constexpr (kKind != KUDNN_B200_S8) {  // integer launches never split K
         if (p.via_smem != 0) {
             // ------------------------------------------------------------------ finish the tile from shared memory
@@ -1926,32 +1954,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             __syncwarp();
             cluster_sync_all();  // no CTA leaves while another still reads its shared memory
-        }
-    }
-
-    // ---------------------------------------------------------------------- teardown
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (*abort_flag != 0) {
-        // give copies and MMAs that were already issued time to land before the memory is handed back
-        const long long t0 = clock64();
-        while (clock64() - t0 < 400000ll) {
-            __nanosleep(1000);
-        }
-        __syncthreads();
-    }
-    if (kPair) {
-        // neither CTA frees tensor memory or leaves while the other may still signal its barriers or, through the
-        // leader's MMAs, use its shared and tensor memory
-        cluster_sync_all();
-    }
-    if (warp == 1) {
-        if (kPair) {
-            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
-        } else {
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
         }
     }
 }

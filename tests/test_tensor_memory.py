@@ -8,7 +8,7 @@ gpu = pytest.mark.gpu
 
 
 @gpu
-@pytest.mark.parametrize("linears", [1])
+@pytest.mark.parametrize("linears", [1, 2, 4])
 def test_cut_launches_on_several_streams(cuda_device, monkeypatch, capfd, linears):
     """Products by group and linear ones whose CTAs are small enough to share an SM, but not its tensor memory."""
     monkeypatch.setenv("KUDNN_B200_TC_SPLITS", "4")
