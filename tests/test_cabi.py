@@ -108,3 +108,21 @@ def test_shard_range_partitions_exactly():
         assert covered == total
     with pytest.raises(kb.KudnnError):
         kb.shard_range(10, 0, 0)
+
+
+def test_addresses_are_taken_as_they_are():
+    """A call from torch passes up to six addresses: none is looked through for a tensor's or an array's attributes first."""
+    class Address(int):
+        def __getattr__(self, name):
+            raise AssertionError(name)
+
+    class Tensor:
+        def data_ptr(self):
+            return 4096
+
+    at = Address(1 << 40)
+    assert capi._ptr(at) is at and capi._ptr(None) is None and capi._ptr(Tensor()) == 4096
+    array = np.zeros(4)
+    assert capi._ptr(array) == array.ctypes.data
+    with pytest.raises(TypeError):
+        capi._ptr("somewhere")
