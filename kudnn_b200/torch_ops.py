@@ -28,7 +28,8 @@ RESIDUALS = {None: capi.RES_NONE, "none": capi.RES_NONE, "add": capi.RES_IDENTIC
 # pre-packs the weights it first sees and recognises them by pointer).  The weak reference kept beside a primitive holds
 # the storage's identity, not its memory: as long as it exists no other storage has that identity, so weights that are
 # allocated later where freed ones were never meet their packed copy.  Bounded: when full, the primitive used longest ago is
-# dropped, and destroyed when no call of another thread uses it any more; one whose launches a CUDA graph holds stays.
+# dropped, and destroyed when no call of another thread uses it any more and after the lock is free again (that waits for the
+# device); one whose launches a CUDA graph holds stays, however many they are.
 _HANDLES = collections.OrderedDict()
 _MAX_HANDLES = 128
 _LOCK = threading.Lock()
@@ -51,8 +52,7 @@ def _handle(m, n, k, x, weight, bias, act, act_alpha, residual, res_op):
         lin.prepack(weight, stream=torch.cuda.current_stream(x.device).cuda_stream)
         if len(_HANDLES) >= _MAX_HANDLES:
             oldest = next((old for old, (other, _) in _HANDLES.items() if other.graphs == 0), None)
-            if oldest is not None:
-                del _HANDLES[oldest]
+            dropped = None if oldest is None else _HANDLES.pop(oldest)  # noqa: F841  (lives until this function has returned)
         _HANDLES[key] = (lin, StorageWeakRef(storage))
         return lin
 
@@ -61,12 +61,11 @@ def clear_cache():
     """Destroys every cached primitive (and the packed weight copies they own); graphs that hold calls of the operator
     must not be replayed afterwards."""
     with _LOCK:
-        while _HANDLES:
-            _, (lin, _) = _HANDLES.popitem()
-            lin.close()
-        while _GROUPED:
-            _, (op, _) = _GROUPED.popitem()
-            op.close()
+        dropped = [entry[0] for cache in (_HANDLES, _GROUPED) for entry in cache.values()]
+        _HANDLES.clear()
+        _GROUPED.clear()
+    for op in dropped:
+        op.close()
 
 
 def _run(x, x2, weight, bias, act, act_alpha, res2, res_op, gamma, m, n, k, out):
@@ -147,7 +146,8 @@ class Linear(torch.nn.Module):
 _OPERANDS = {torch.float16: capi.F16, torch.bfloat16: capi.BF16, torch.float8_e4m3fn: capi.E4M3}
 _OFFSETS = {torch.int32: capi.S32, torch.int64: capi.S64}
 # Created products by group: descriptors only, no weights and nothing of a call's tensors.  Bounded as _HANDLES; what was called while its
-# stream was captured stays, since the graph must not outlive it.
+# stream was captured stays, since the graph must not outlive it, beyond the bound as well: a shape that graphs hold keeps its status word in
+# device memory until clear_cache().
 _GROUPED = collections.OrderedDict()
 _MAX_GROUPED = 1024
 
@@ -213,8 +213,7 @@ def _grouped_handle(device, key, make):
         if entry is None:
             if len(_GROUPED) >= _MAX_GROUPED:
                 oldest = next((old for old, (_, held) in _GROUPED.items() if not held), None)
-                if oldest is not None:
-                    del _GROUPED[oldest]
+                dropped = None if oldest is None else _GROUPED.pop(oldest)  # noqa: F841  (as in _handle)
             entry = _GROUPED[key] = [capi.Grouped(make()), False]
         else:
             _GROUPED.move_to_end(key)

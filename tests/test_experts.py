@@ -1,5 +1,6 @@
 """The torch operators kudnn_b200::quantize and ::grouped, and the feed-forward block of experts that runs them together."""
 import collections
+import types
 
 import pytest
 import torch
@@ -109,6 +110,39 @@ def test_created_products_are_bounded_and_captured_ones_stay(monkeypatch):
     assert handle("a") is first and handle("b") is not second
     torch_ops.clear_cache()
     assert first.closed and not torch_ops._GROUPED
+
+
+def test_dropped_primitives_are_destroyed_without_the_lock(monkeypatch):
+    """Destroying one waits for the device, and the lock holds up the calls of all other threads."""
+    locked = []
+
+    class Watched:
+        def __init__(self, desc):
+            self.graphs = 0
+
+        def prepack(self, b, stream=None):
+            pass
+
+        def close(self):
+            locked.append(torch_ops._LOCK.locked())
+
+        __del__ = close
+
+    for name in ("Grouped", "Linear"):
+        monkeypatch.setattr(torch_ops.capi, name, Watched)
+    for name in ("_GROUPED", "_HANDLES"):
+        monkeypatch.setattr(torch_ops, name, collections.OrderedDict())
+    monkeypatch.setattr(torch_ops, "_MAX_GROUPED", 2)
+    monkeypatch.setattr(torch_ops, "_MAX_HANDLES", 2)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=1))
+    weight = torch.zeros(8, 16)
+    for m in range(1, 5):
+        torch_ops._grouped_handle(torch.device("cuda", 0), m, lambda: None)
+        torch_ops._handle(m, 8, 16, torch.zeros(m, 16), weight, None, 0, 1.0, None, 0)
+    assert locked == [False] * 4
+    torch_ops.clear_cache()
+    assert not torch_ops._GROUPED and not torch_ops._HANDLES and len(locked) >= 8 and not any(locked)
 
 
 @gpu
