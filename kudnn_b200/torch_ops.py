@@ -336,5 +336,5 @@ class Experts(torch.nn.Module):
             y = ops.grouped((torch.nn.functional.silu(gate) * up).to(x.dtype), self.down, offsets)
         back = torch.empty_like(order)
         back[order] = torch.arange(order.shape[0], device=x.device)
-        y = (y[back].view(count, self.top, -1).float() * p[:, :, None]).sum(dim=1)
+        y = (y[back].view(count, self.top, tokens.shape[1]).float() * p[:, :, None]).sum(dim=1)
         return y.to(x.dtype).view(x.shape)

@@ -189,6 +189,18 @@ def test_refusals(cuda_device, wrong):
         wrong(x, w, torch.tensor([0, 1, 4], dtype=torch.int32, device="cuda"))
 
 
+def meta_experts(eight_bit, hidden=300, ffn=200, experts=6):
+    return torch_ops.Experts(meta(experts, hidden, dtype=torch.float32), meta(experts, 2 * ffn, hidden), meta(experts, hidden, ffn), 2,
+                             eight_bit=eight_bit)
+
+
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("shape", [(0, 300), (2, 0, 300), (5, 300)])
+def test_experts_propagate_shapes_of_any_number_of_tokens(eight_bit, shape):
+    y = meta_experts(eight_bit)(meta(*shape))
+    assert y.shape == shape and y.dtype == torch.bfloat16
+
+
 def experts64(x, router, gate_up, down, top):
     tokens = x.reshape(-1, x.shape[-1])
     p = torch.softmax(tokens.double() @ router.double().t(), dim=1)
@@ -224,6 +236,14 @@ def test_experts(cuda_device, tokens, eight_bit):
     off = torch.linalg.vector_norm(y.double() - want) / torch.linalg.vector_norm(want)
     assert off <= (0.094 if eight_bit else 2.0 ** -7)
     assert torch.equal(block(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_experts_without_tokens(cuda_device, eight_bit):
+    w = torch.ones(4, 64, 32, dtype=torch.bfloat16, device="cuda")
+    block = torch_ops.Experts(torch.ones(4, 32, device="cuda"), w, w.transpose(1, 2)[:, :, :32].contiguous(), 2, eight_bit=eight_bit)
+    assert block(torch.ones(3, 0, 32, dtype=torch.bfloat16, device="cuda")).shape == (3, 0, 32)
 
 
 @gpu
