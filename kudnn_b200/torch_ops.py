@@ -314,6 +314,25 @@ class Experts(torch.nn.Module):
             else:
                 self.register_buffer(name, w)
 
+    def _apply(self, fn, recurse=True):
+        """Moves of the module (``to``, ``cuda``, ``half`` ...): the router, scales and e4m3 weights go along but keep their types, and the
+        weights the pitch that the products read in place."""
+        names = ("router", "gate_up", "gate_up_scale", "down", "down_scale") if self.eight_bit else ("router",)
+        kept = {name: self._buffers[name] for name in names}
+        self._buffers.update(dict.fromkeys(names))
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            e4m3 = t.dtype == torch.float8_e4m3fn
+            if e4m3:  # with the bytes between the rows
+                bits = torch.as_strided(t, t.shape[:2] + (t.stride(1),), t.stride(), t.storage_offset()).view(torch.uint8)
+            else:
+                bits = t.view(torch.int32)
+            moved = fn(bits)
+            if moved.dtype != bits.dtype:
+                moved = bits.to(moved.device)
+            self._buffers[name] = moved.view(t.dtype)[:, :, :t.shape[2]] if e4m3 else moved.view(t.dtype)
+        return self
+
     @torch.no_grad()
     def forward(self, x):
         tokens = x.reshape(-1, x.shape[-1])

@@ -201,6 +201,20 @@ def test_experts_propagate_shapes_of_any_number_of_tokens(eight_bit, shape):
     assert y.shape == shape and y.dtype == torch.bfloat16
 
 
+MOVES = [lambda b: b.half(), lambda b: b.to(torch.bfloat16), lambda b: b.double(), lambda b: b.type(torch.float16)]
+
+
+@pytest.mark.parametrize("move", MOVES)
+def test_casts_of_the_experts_leave_8_bit_weights_scales_and_the_router(move):
+    block = meta_experts(True)
+    before = {name: (t.dtype, t.shape, t.stride()) for name, t in block.named_buffers()}
+    assert before["down"] == (torch.float8_e4m3fn, (6, 300, 200), (300 * 208, 208, 1))
+    move(block)
+    assert {name: (t.dtype, t.shape, t.stride()) for name, t in block.named_buffers()} == before
+    block = move(meta_experts(False))
+    assert block.router.dtype == torch.float32 and block.down.dtype == block.gate_up.dtype != torch.float32
+
+
 def experts64(x, router, gate_up, down, top):
     tokens = x.reshape(-1, x.shape[-1])
     p = torch.softmax(tokens.double() @ router.double().t(), dim=1)
@@ -244,6 +258,19 @@ def test_experts_without_tokens(cuda_device, eight_bit):
     w = torch.ones(4, 64, 32, dtype=torch.bfloat16, device="cuda")
     block = torch_ops.Experts(torch.ones(4, 32, device="cuda"), w, w.transpose(1, 2)[:, :, :32].contiguous(), 2, eight_bit=eight_bit)
     assert block(torch.ones(3, 0, 32, dtype=torch.bfloat16, device="cuda")).shape == (3, 0, 32)
+
+
+@gpu
+def test_experts_keep_their_results_when_they_are_moved(cuda_device):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    gate_up = (torch.randn(6, 400, 300, generator=gen, device="cuda") * 0.05).bfloat16()
+    down = (torch.randn(6, 300, 200, generator=gen, device="cuda") * 0.05).bfloat16()
+    block = torch_ops.Experts(torch.randn(6, 300, generator=gen, device="cuda"), gate_up, down, 2, eight_bit=True)
+    x = torch.randn(9, 300, generator=gen, device="cuda").bfloat16()
+    want = block(x)
+    for move in MOVES + [lambda b: b.cpu().to("cuda"), lambda b: b.to("cuda", torch.bfloat16)]:
+        move(block)
+        assert torch.equal(block(x), want)
 
 
 @gpu
