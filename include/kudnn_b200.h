@@ -214,7 +214,8 @@ KUDNN_B200_API int kudnn_b200_rmsnorm_run(const void *src, void *dst, const void
                                           void *cuda_stream);
 
 /* ---- feed-forward layers in 8-bit floating point, and of experts ---------------------------------------------------
- * No counterpart in the reference.  Device pointers only; asynchronous on the stream; forward only, as everything here.
+ * No counterpart in the reference.  Device pointers only, each a multiple of its elements' size; asynchronous on the stream; forward
+ * only, as everything here.
  *
  * Quantisation: rows of F32 / F16 / BF16 values -> E4M3 with an fp32 scale per block, value = q * scale.
  *   most  = max(|v| over the block, 1e-30),  scale = most / 448,  q = e4m3(v * (448 / most)), to nearest even

@@ -39,6 +39,12 @@ bool float_type(int dt)
     return dt == KUDNN_B200_F32 || dt == KUDNN_B200_F16 || dt == KUDNN_B200_BF16;
 }
 
+// whether some address is not a multiple of its elements' size: a load from it would fault
+bool misaligned(const void *p, int size)
+{
+    return reinterpret_cast<uintptr_t>(p) % size != 0;
+}
+
 constexpr int64_t kMostExtent = 0x7fffffffll - 1024;
 
 int current_device(int *dev, int *sms)
@@ -148,6 +154,9 @@ int kudnn_b200_quantize_run(const kudnn_b200_quantize_desc *d, const void *x, vo
     }
     if ((x == nullptr && d->x_rows != 0) || q == nullptr || scale == nullptr) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "quantize: x, q and scale must not be null");
+    }
+    if (misaligned(x, kb::dtype_size(d->x_dtype)) || misaligned(scale, 4) || misaligned(index, 4)) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "quantize: x, scale or index is not aligned to its elements");
     }
     int dev = 0, sms = 0;
     rc = current_device(&dev, &sms);
@@ -276,6 +285,12 @@ int kudnn_b200_grouped_run(kudnn_b200_grouped_t h, const kudnn_b200_grouped_args
     }
     if (args->a == nullptr || args->b == nullptr || args->c == nullptr) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "grouped: a, b and c must not be null");
+    }
+    const int es = d.ab_dtype == KUDNN_B200_E4M3 ? 1 : 2;
+    if (misaligned(args->a, es) || misaligned(args->b, es) || misaligned(args->c, kb::dtype_size(d.c_dtype)) ||
+        (d.has_bias != 0 && misaligned(args->bias, kb::dtype_size(d.bias_dtype))) || misaligned(args->a_scale, 4) || misaligned(args->b_scale, 4) ||
+        misaligned(args->offsets, d.offsets_dtype == KUDNN_B200_S64 ? 8 : 4)) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "grouped: an operand is not aligned to its elements");
     }
     const int rc = ensure_device(h);
     if (rc != KUDNN_B200_OK) {

@@ -420,3 +420,19 @@ def test_pointers_that_do_not_match_the_descriptor_are_refused():
     empty.run(None, None, None, **every)  # no rows: nothing to do
     assert kb.library().kudnn_b200_grouped_validate(None) == 2
     assert math.isclose(small().act_alpha, 1.0)
+
+
+def test_addresses_between_elements_are_refused():
+    """A load from one would fault."""
+    at = 1 << 20
+    op = kb.Grouped(small(offsets_dtype=kb.S64, has_bias=1, bias_dtype=kb.F16))
+    every = dict(a=at, b=at, c=at, offsets=at, a_scale=at, b_scale=at, bias=at)
+    for name, off in (("c", 1), ("offsets", 4), ("a_scale", 2), ("b_scale", 1), ("bias", 1)):
+        with pytest.raises(kb.KudnnError) as e:
+            op.run(**dict(every, **{name: at + off}))
+        assert e.value.status == 2
+    op = kb.Grouped(small(dtype=kb.BF16))
+    for name, off in (("a", 1), ("b", 1), ("c", 1), ("offsets", 2)):
+        with pytest.raises(kb.KudnnError) as e:
+            op.run(**dict(dict(a=at, b=at, c=at, offsets=at), **{name: at + off}))
+        assert e.value.status == 2

@@ -232,3 +232,11 @@ def test_null_pointers_and_rows_without_index_are_refused():
     d.rows = d.x_rows = 0
     kb.quantize(d, None, None, None)            # no rows: nothing to do
     assert capi.library().kudnn_b200_quantize_validate(None) == 2
+
+
+def test_addresses_between_elements_are_refused():
+    at = 1 << 20
+    for x, scale, index in ((at + 1, at, at), (at, at + 2, at), (at, at, at + 1)):
+        with pytest.raises(kb.KudnnError) as e:
+            kb.quantize(desc(), x, at, scale, index)
+        assert e.value.status == 2
