@@ -4,6 +4,7 @@
 #include <cstdio>
 #include <mutex>
 #include <new>
+#include <numeric>
 
 struct kudnn_b200_grouped_s {
     kudnn_b200_grouped_desc d;
@@ -43,6 +44,13 @@ bool float_type(int dt)
 bool misaligned(const void *p, int size)
 {
     return reinterpret_cast<uintptr_t>(p) % size != 0;
+}
+
+// Whether two elements of a matrix share an address: i * s1 == j * s2 for some i < rows, j < cols, the least of which are s2 / g, s1 / g.
+bool overlaps(int64_t rows, int64_t s1, int64_t cols, int64_t s2)
+{
+    const int64_t g = std::gcd(s1, s2);
+    return g == 0 ? rows > 1 || cols > 1 : s2 / g < rows && s1 / g < cols;
 }
 
 constexpr int64_t kMostExtent = 0x7fffffffll - 1024;
@@ -131,7 +139,7 @@ int kudnn_b200_quantize_validate(const kudnn_b200_quantize_desc *d)
         return fail(KUDNN_B200_BAD_ARGUMENTS, "quantize: rows of q overlap");
     }
     const int64_t scale_rows = (d->rows + d->block_rows - 1) / d->block_rows, scale_cols = (d->k + kb::kScaleBlock - 1) / kb::kScaleBlock;
-    if ((scale_rows > 1 && d->s_row == 0) || (scale_cols > 1 && d->s_col == 0)) {
+    if (overlaps(scale_rows, d->s_row, scale_cols, d->s_col)) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "quantize: scales overlap");
     }
     return KUDNN_B200_OK;
@@ -225,7 +233,7 @@ int kudnn_b200_grouped_validate(const kudnn_b200_grouped_desc *d)
             return fail(KUDNN_B200_BAD_ARGUMENTS, "grouped: negative strides");
         }
     }
-    if ((d->rows > 1 && d->c_sm == 0) || (d->n > 1 && d->c_sn == 0)) {
+    if (overlaps(d->rows, d->c_sm, d->n, d->c_sn)) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "grouped: elements of c overlap");
     }
     return KUDNN_B200_OK;

@@ -436,3 +436,16 @@ def test_addresses_between_elements_are_refused():
         with pytest.raises(kb.KudnnError) as e:
             op.run(**dict(dict(a=at, b=at, c=at, offsets=at), **{name: at + off}))
         assert e.value.status == 2
+
+
+@pytest.mark.parametrize("c_sm,c_sn,status", [
+    (256, 1, 0), (255, 1, 2), (1, 8, 0), (1, 7, 2), (1, 1, 2), (0, 1, 2), (1, 0, 2), (2, 16, 0), (2, 15, 0), (6, 4, 2), (257, 8, 0), (255, 8, 0),
+])
+def test_results_that_share_memory_are_refused(c_sm, c_sn, status):
+    """8 x 256 of them; held against all addresses."""
+    shared = len({r * c_sm + n * c_sn for r in range(8) for n in range(256)}) < 8 * 256
+    assert shared == (status != 0)
+    d = small(c_sm=c_sm, c_sn=c_sn)
+    assert kb.library().kudnn_b200_grouped_validate(ctypes.byref(d)) == status
+    one = small(rows=1, c_sm=0)
+    assert kb.library().kudnn_b200_grouped_validate(ctypes.byref(one)) == 0

@@ -240,3 +240,12 @@ def test_addresses_between_elements_are_refused():
         with pytest.raises(kb.KudnnError) as e:
             kb.quantize(desc(), x, at, scale, index)
         assert e.value.status == 2
+
+
+@pytest.mark.parametrize("strides,status", [((1, 4), 0), ((1, 3), 2), ((1, 1), 2), ((2, 1), 0), ((3, 2), 0), ((1, 2), 2), ((2, 3), 0)])
+def test_scales_that_share_memory_are_refused(strides, status):
+    """4 rows, 2 blocks of columns; held against all addresses."""
+    import ctypes
+    shared = len({r * strides[0] + c * strides[1] for r in range(4) for c in range(2)}) < 8
+    assert shared == (status != 0)
+    assert kb.library().kudnn_b200_quantize_validate(ctypes.byref(desc(scale_strides=strides))) == status
