@@ -79,7 +79,8 @@ struct Shape {
     static constexpr int kLoadRows = kPair ? kTN / 2 : kTN;   // rows of a that one CTA loads, at most
     static constexpr int kBoxRows = kTN >= 128 ? 64 : kTN / 2;  // of them in one copy
     static constexpr int kStageBytes = kWeightBytes + kLoadRows * 128;
-    static constexpr bool kSplits = kTN <= 64;                // whether launches may cut K
+    // Whether launches may cut K.  Not tiles of 64 rows: where they cost less than those of 32, they are more than half of the SMs.
+    static constexpr bool kSplits = kTN == 32;
     static constexpr int kUnits = kTN / 16 * 4;               // of a whole tile; partial sums lie where the ring was
     static constexpr int kLeastStages = kTN == 32 ? 2 : 3;
     static_assert(!kSplits || (kUnits + kSumWarps) * kUnitBytes <= kLeastStages * kStageBytes, "room for the partial sums");
