@@ -280,6 +280,10 @@ KUDNN_B200_API int kudnn_b200_grouped_check(kudnn_b200_grouped_t handle, void *c
 KUDNN_B200_API int kudnn_b200_grouped_force_kernel(kudnn_b200_grouped_t handle, int kernel);
 KUDNN_B200_API int kudnn_b200_grouped_last_kernel(kudnn_b200_grouped_t handle);
 KUDNN_B200_API int kudnn_b200_grouped_set_wait(kudnn_b200_grouped_t handle, long long wait_limit_cycles, int skip_kblock);
+/* Test hooks: rows of the tensor-core kernel's tiles (32, 64, 128 or 256; 0: by the sizes) and whether those of 256 rows of E4M3 operands
+ * stand on the M side of the MMA; the tile of the last run (zeros if it took the general kernel) and how many CTAs cut its K. */
+KUDNN_B200_API int kudnn_b200_grouped_force_tile(kudnn_b200_grouped_t handle, int tile_rows, int rows_on_m);
+KUDNN_B200_API int kudnn_b200_grouped_last_tile(kudnn_b200_grouped_t handle, int *tile_rows, int *rows_on_m, int *splits);
 
 /* Reads the device-side status word of the handle (bounded waits that gave up) after synchronising the stream. */
 KUDNN_B200_API int kudnn_b200_linear_check(kudnn_b200_linear_t handle, void *cuda_stream);

@@ -103,7 +103,7 @@ EXPORTS = [
     "kudnn_b200_linear_set_multicast", "kudnn_b200_linear_graphs",
     "kudnn_b200_quantize_validate", "kudnn_b200_quantize_run", "kudnn_b200_grouped_validate", "kudnn_b200_grouped_create",
     "kudnn_b200_grouped_destroy", "kudnn_b200_grouped_run", "kudnn_b200_grouped_check", "kudnn_b200_grouped_force_kernel",
-    "kudnn_b200_grouped_last_kernel", "kudnn_b200_grouped_set_wait",
+    "kudnn_b200_grouped_last_kernel", "kudnn_b200_grouped_set_wait", "kudnn_b200_grouped_force_tile", "kudnn_b200_grouped_last_tile",
 ]
 
 _lib = None
@@ -165,6 +165,8 @@ def library():
     lib.kudnn_b200_grouped_force_kernel.argtypes = [vp, i32]
     lib.kudnn_b200_grouped_last_kernel.argtypes = [vp]
     lib.kudnn_b200_grouped_set_wait.argtypes = [vp, ctypes.c_longlong, i32]
+    lib.kudnn_b200_grouped_force_tile.argtypes = [vp, i32, i32]
+    lib.kudnn_b200_grouped_last_tile.argtypes = [vp] + [ctypes.POINTER(ctypes.c_int)] * 3
     lib.kudnn_b200_last_error.restype = ctypes.c_char_p
     lib.kudnn_b200_version.restype = ctypes.c_char_p
     _lib = lib
@@ -359,9 +361,20 @@ class Grouped:
         """Test hook: limit of the device-side waits in SM cycles, and the k-block from which on no loads are issued."""
         _check(self._lib.kudnn_b200_grouped_set_wait(self._h, wait_limit_cycles, skip_kblock))
 
+    def force_tile(self, tile_rows, rows_on_m=False):
+        """Test hook: rows of the tensor-core kernel's tiles, 0: by the sizes."""
+        _check(self._lib.kudnn_b200_grouped_force_tile(self._h, tile_rows, 1 if rows_on_m else 0))
+
     @property
     def last_kernel(self):
         return self._lib.kudnn_b200_grouped_last_kernel(self._h)
+
+    @property
+    def last_tile(self):
+        """(rows of a tile, whether they stood on the M side, CTAs that cut K) of the last run."""
+        got = [ctypes.c_int() for _ in range(3)]
+        _check(self._lib.kudnn_b200_grouped_last_tile(self._h, *[ctypes.byref(v) for v in got]))
+        return got[0].value, got[1].value != 0, got[2].value
 
 
 def debug_fail_allocation(nth):

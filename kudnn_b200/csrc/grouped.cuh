@@ -45,8 +45,13 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(unsigned short v)
 
 // Whether the tensor-core kernel (grouped_tc.cuh) takes these operands: rows K-contiguous, 16-byte aligned.
 bool grouped_tc_takes(const GroupedParams &p);
+// rows of its tiles (0: not chosen yet), whether they stand on the M side, CTAs that cut K
+struct GroupedTile {
+    int rows, on_m, splits;
+};
+// Takes the tile that *tile asks for, or chooses one, and says which it was.
 cudaError_t launch_grouped_tc(const GroupedParams &p, int sm_count, DeviceStatus *status, long long wait_limit_cycles, int skip_kblock,
-                              cudaStream_t stream);
+                              GroupedTile *tile, cudaStream_t stream);
 cudaError_t launch_grouped_simt(const GroupedParams &p, cudaStream_t stream);
 
 // x -> e4m3 with a scale per row and 128 columns (block_rows = 1) or per 128 x 128 (block_rows = 128); see quantize.cu

@@ -11,6 +11,7 @@ struct kudnn_b200_grouped_s {
     std::mutex lock;
     int forced_kernel = KUDNN_B200_KERNEL_AUTO;
     int last_kernel = 0;
+    kb::GroupedTile forced_tile = {0, 0, 0}, last_tile = {0, 0, 0};
     int device = -1;
     int sm_count = 0;
     kb::DeviceStatus *status = nullptr;
@@ -343,7 +344,10 @@ int kudnn_b200_grouped_run(kudnn_b200_grouped_t h, const kudnn_b200_grouped_args
     }
     const bool tc = takes && h->forced_kernel != KUDNN_B200_KERNEL_SIMT;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    const cudaError_t e = tc ? kb::launch_grouped_tc(p, h->sm_count, h->status, h->wait_limit, h->skip_kblock, stream) : kb::launch_grouped_simt(p, stream);
+    kb::GroupedTile tile = h->forced_tile;
+    const cudaError_t e = tc ? kb::launch_grouped_tc(p, h->sm_count, h->status, h->wait_limit, h->skip_kblock, &tile, stream)
+                             : kb::launch_grouped_simt(p, stream);
+    h->last_tile = tc ? tile : kb::GroupedTile{0, 0, 0};
     h->last_kernel = tc ? KUDNN_B200_KERNEL_TC : KUDNN_B200_KERNEL_SIMT;
     return e == cudaSuccess ? KUDNN_B200_OK : fail_cuda(e, "grouped kernel launch");
 }
@@ -383,6 +387,29 @@ int kudnn_b200_grouped_force_kernel(kudnn_b200_grouped_t h, int kernel)
 int kudnn_b200_grouped_last_kernel(kudnn_b200_grouped_t h)
 {
     return h == nullptr ? 0 : h->last_kernel;
+}
+
+int kudnn_b200_grouped_force_tile(kudnn_b200_grouped_t h, int tile_rows, int rows_on_m)
+{
+    if (h == nullptr || (tile_rows != 0 && tile_rows != 32 && tile_rows != 64 && tile_rows != 128 && tile_rows != 256)) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "grouped: tiles have 32, 64, 128 or 256 rows");
+    }
+    if (rows_on_m != 0 && (tile_rows != 256 || h->d.ab_dtype != KUDNN_B200_E4M3)) {
+        return fail(KUDNN_B200_UNSUPPORTED, "grouped: the rows stand on the M side in tiles of 256 rows of E4M3 operands only");
+    }
+    h->forced_tile = {tile_rows, rows_on_m != 0 ? 1 : 0, 0};
+    return KUDNN_B200_OK;
+}
+
+int kudnn_b200_grouped_last_tile(kudnn_b200_grouped_t h, int *tile_rows, int *rows_on_m, int *splits)
+{
+    if (h == nullptr || tile_rows == nullptr || rows_on_m == nullptr || splits == nullptr) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "grouped: null handle or arguments");
+    }
+    *tile_rows = h->last_tile.rows;
+    *rows_on_m = h->last_tile.on_m;
+    *splits = h->last_tile.splits;
+    return KUDNN_B200_OK;
 }
 
 int kudnn_b200_grouped_set_wait(kudnn_b200_grouped_t h, long long wait_limit_cycles, int skip_kblock)

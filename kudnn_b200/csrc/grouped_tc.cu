@@ -117,20 +117,24 @@ int choose_tile(const GroupedParams &g, const TcParams &p, bool scaled, bool tal
 }
 
 template <int kMode>
-cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &tb, cudaStream_t stream)
+cudaError_t launch_kind(const GroupedParams &g, TcParams &p, int sm_count, const CUtensorMap &tb, GroupedTile *tile, cudaStream_t stream)
 {
     constexpr bool kScaled = kMode == kWithScales;
     // Tall tiles of scaled products: rows on the M side, unless the groups' last tiles, which that pads to 256 rows, would take more than the
     // faster sums save (850 against 1170 cycles per block of K).
-    const bool tall_on_m = kScaled && (g.offsets == nullptr || g.rows >= 192ll * g.groups);
-    const int tn = choose_tile(g, p, kScaled, tall_on_m, sm_count);
+    if (tile->rows == 0) {
+        const bool tall_on_m = kScaled && (g.offsets == nullptr || g.rows >= 192ll * g.groups);
+        tile->rows = choose_tile(g, p, kScaled, tall_on_m, sm_count);
+        tile->on_m = tall_on_m && tile->rows == 256 ? 1 : 0;
+    }
+    const int tn = tile->rows;
     // offsets may leave out rows and make up to min(groups, rows) short tiles
     const long long tiles = g.offsets == nullptr ? (g.rows + tn - 1) / tn : std::min(g.groups, g.rows) + g.rows / tn;
     p.tiles_n = tn == 256 ? (g.n + 2 * kTileN - 1) / (2 * kTileN) : (g.n + kTileN - 1) / kTileN;
     p.idesc = make_idesc(g.ab_dtype == KUDNN_B200_BF16 ? KUDNN_B200_BF16 : KUDNN_B200_F16, 0, tn == 256 ? 2 * kTileN : kTileN);  // e4m3 and fp16: code 0
     const long long bound = tiles * p.tiles_n;
     if constexpr (kScaled) {
-        if (tn == 256 && tall_on_m) {
+        if (tile->on_m != 0) {
             p.idesc |= 256u >> 3 << 17;
             if (p.vec != 0 && g.c_sm * dtype_size(g.c_dtype) % 32 == 0 && reinterpret_cast<uintptr_t>(g.c) % 32 == 0) {
                 p.vec = 2;
@@ -158,7 +162,7 @@ bool grouped_tc_takes(const GroupedParams &p)
 }
 
 cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus *status, long long wait_limit_cycles, int skip_kblock,
-                              cudaStream_t stream)
+                              GroupedTile *tile, cudaStream_t stream)
 {
     const bool scaled = g.ab_dtype == KUDNN_B200_E4M3;
     const int es = scaled ? 1 : 2, c_size = dtype_size(g.c_dtype);
@@ -180,11 +184,12 @@ cudaError_t launch_grouped_tc(const GroupedParams &g, int sm_count, DeviceStatus
     p.status = status;
     p.wait_limit = wait_limit_cycles > 0 ? wait_limit_cycles : kDefaultWaitLimitCycles;
     p.drain = 4;
-    if (scaled) {
-        return launch_kind<kWithScales>(g, p, sm_count, tb, stream);
-    }
-    return g.c_dtype == KUDNN_B200_F32 && p.num_kb > p.drain ? launch_kind<kDrained>(g, p, sm_count, tb, stream)
-                                                              : launch_kind<kPlain>(g, p, sm_count, tb, stream);
+    p.splits = 1;
+    const cudaError_t launched = scaled ? launch_kind<kWithScales>(g, p, sm_count, tb, tile, stream)
+                                 : g.c_dtype == KUDNN_B200_F32 && p.num_kb > p.drain ? launch_kind<kDrained>(g, p, sm_count, tb, tile, stream)
+                                                                                     : launch_kind<kPlain>(g, p, sm_count, tb, tile, stream);
+    tile->splits = p.splits;
+    return launched;
 }
 
 }  // namespace kb
