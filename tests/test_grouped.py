@@ -221,6 +221,16 @@ def test_the_general_kernel(cuda_device, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", OPERANDS)
+def test_fp32_results_of_the_general_kernel_keep_their_bits(cuda_device, dtype):
+    """128 products add up, then 64 of these sums.  An addition is off by 0.42 * 2^-24 of the running sum in the square mean, and that is half
+    of the last one on average: 0.3 * 2^-24 * sqrt(128 + 64) = 4.1 * 2^-24 in the norm.  Twice that is the limit."""
+    p = Problem(130, 200, 8192, dtype, out="f32", sizes=[60, 70]).check(kb.KERNEL_SIMT)
+    y, _ = p.exact()
+    assert torch.linalg.vector_norm(p.c.double() - y) <= 8.2 * 2.0 ** -24 * torch.linalg.vector_norm(y)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_what_is_not_finite_stays_in_its_row_or_column(cuda_device, dtype):
     p = Problem(300, 264, 400, dtype, sizes=[100, 0, 200])
