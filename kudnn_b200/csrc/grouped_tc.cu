@@ -48,8 +48,9 @@ cudaError_t launch_shape(const GroupedParams &g, TcParams &p, long long item_bou
     if (e != cudaSuccess) {
         return e;
     }
-    // Where the items leave SMs idle, two or four CTAs of a cluster cut K, if that fills the SMs better: 86 items of one row, 32 blocks of K:
-    // 11.8 us uncut, 12.2 at two (172 CTAs on 148 SMs), 10.4 at four.  Clusters of 8 and odd ones find no room next to one another.
+    // Where the items leave SMs idle, two or four CTAs of a cluster cut K, if that fills the SMs better: 86 items of one row, 32 blocks of K,
+    // all of it in L2: 11.8 us uncut, 12.2 at two (172 CTAs on 148 SMs), 10.4 at four (13.0 from HBM).  Clusters of 8 and odd ones find no room
+    // next to one another.
     // The CTAs that then share an SM share its memory for their rings.
     auto filled = [&](long long ctas) { return static_cast<double>(ctas) / sm_count / ((ctas + sm_count - 1) / sm_count); };
     p.splits = 1;
