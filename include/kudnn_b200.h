@@ -213,6 +213,33 @@ KUDNN_B200_API int kudnn_b200_rmsnorm_run(const void *src, void *dst, const void
                                           int64_t axis, int dtype, int flags, int save_stats, float eps,
                                           void *cuda_stream);
 
+/* ---- layer normalisation and its gradient --------------------------------------------------------------------------
+ * Over the last axis of [rows, axis] values F32 / F16 / BF16 at row pitches; device pointers only, each a multiple of its elements' size;
+ * asynchronous on the stream.  Beside kudnn_b200_rmsnorm_*, for models that subtract the mean:
+ *   m = mean(x), v = mean((x - m)^2), r = 1 / sqrt(v + eps), y = (x - m) r * scale + shift
+ * and, with g = dy * scale and xh = (x - m) r,
+ *   dx = r (g - mean(g) - xh mean(g xh)), dscale = sum over rows of dy xh, dshift = sum over rows of dy.
+ * All arithmetic is fp32; each result is rounded once, to nearest even.  The same call gives the same bits every time.
+ * flags: USE_SCALE, USE_SHIFT (without them 1 and 0); USE_GLOBAL_STATS: mean and variance (fp32, one per row) are given, and constants for the
+ * gradient (dx = r g).  Otherwise a run writes them unless they are NULL; the gradient always reads them.
+ * scale, shift and their gradients are of param_dtype: F32 or dtype.  dx, dscale and dshift may each be NULL.  y may be x and dx may be x or
+ * dy, with the same pitch; other overlaps are not allowed.  What lies between the rows is not written. */
+typedef struct kudnn_b200_layernorm_desc {
+    int64_t rows, axis;
+    int64_t x_ld, y_ld, dy_ld, dx_ld; /* row pitches in elements; columns are contiguous */
+    int32_t dtype, param_dtype, flags, reserved;
+    float eps, reserved_f;
+} kudnn_b200_layernorm_desc;
+KUDNN_B200_API int kudnn_b200_layernorm_validate(const kudnn_b200_layernorm_desc *desc);
+KUDNN_B200_API int kudnn_b200_layernorm_run(const kudnn_b200_layernorm_desc *desc, const void *x, const void *scale, const void *shift, void *y,
+                                            float *mean, float *variance, void *cuda_stream);
+/* The gradient needs scratch in device memory for dscale or dshift: as many bytes as the first function says (host arithmetic), on a 4-byte
+ * boundary, its contents irrelevant, used by one run at a time. */
+KUDNN_B200_API int kudnn_b200_layernorm_backward_workspace(const kudnn_b200_layernorm_desc *desc, int64_t *bytes);
+KUDNN_B200_API int kudnn_b200_layernorm_backward_run(const kudnn_b200_layernorm_desc *desc, const void *x, const void *dy, const void *scale,
+                                                     const float *mean, const float *variance, void *dx, void *dscale, void *dshift,
+                                                     void *workspace, int64_t workspace_bytes, void *cuda_stream);
+
 /* ---- feed-forward layers in 8-bit floating point, and of experts ---------------------------------------------------
  * No counterpart in the reference.  Device pointers only, each a multiple of its elements' size; asynchronous on the stream; forward
  * only, as everything here.

@@ -14,6 +14,7 @@ from .capi import (  # noqa: F401
     peer_buffer_close, peer_buffer_create, peer_buffer_destroy, peer_buffer_open, rmsnorm,
     NORM_USE_GLOBAL_STATS, NORM_USE_SCALE, SHARD_COLS, SHARD_ROWS,
     SCALE_BLOCK, Grouped, GroupedDesc, QuantizeDesc, make_grouped_desc, make_quantize_desc, quantize,
+    LayernormDesc, layernorm, layernorm_backward, layernorm_backward_workspace, make_layernorm_desc,
 )
 
 __all__ = [
@@ -25,4 +26,5 @@ __all__ = [
     "peer_buffer_close", "peer_buffer_create", "peer_buffer_destroy", "peer_buffer_open", "rmsnorm",
     "NORM_USE_GLOBAL_STATS", "NORM_USE_SCALE", "SHARD_COLS", "SHARD_ROWS",
     "SCALE_BLOCK", "Grouped", "GroupedDesc", "QuantizeDesc", "make_grouped_desc", "make_quantize_desc", "quantize",
+    "LayernormDesc", "layernorm", "layernorm_backward", "layernorm_backward_workspace", "make_layernorm_desc",
 ]

@@ -90,6 +90,17 @@ class GroupedArgs(ctypes.Structure):
                 ("a_scale", ctypes.c_void_p), ("b_scale", ctypes.c_void_p), ("offsets", ctypes.c_void_p)]
 
 
+class LayernormDesc(ctypes.Structure):
+    """kudnn_b200_layernorm_desc."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("axis", ctypes.c_int64),
+        ("x_ld", ctypes.c_int64), ("y_ld", ctypes.c_int64), ("dy_ld", ctypes.c_int64), ("dx_ld", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32), ("flags", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("reserved_f", ctypes.c_float),
+    ]
+
+
 EXPORTS = [
     "kudnn_b200_linear_validate", "kudnn_b200_linear_create", "kudnn_b200_linear_clone", "kudnn_b200_linear_destroy",
     "kudnn_b200_linear_prepack", "kudnn_b200_linear_run", "kudnn_b200_linear_run_host", "kudnn_b200_linear_check",
@@ -104,6 +115,8 @@ EXPORTS = [
     "kudnn_b200_quantize_validate", "kudnn_b200_quantize_run", "kudnn_b200_grouped_validate", "kudnn_b200_grouped_create",
     "kudnn_b200_grouped_destroy", "kudnn_b200_grouped_run", "kudnn_b200_grouped_check", "kudnn_b200_grouped_force_kernel",
     "kudnn_b200_grouped_last_kernel", "kudnn_b200_grouped_set_wait", "kudnn_b200_grouped_force_tile", "kudnn_b200_grouped_last_tile",
+    "kudnn_b200_layernorm_validate", "kudnn_b200_layernorm_run", "kudnn_b200_layernorm_backward_workspace",
+    "kudnn_b200_layernorm_backward_run",
 ]
 
 _lib = None
@@ -167,6 +180,10 @@ def library():
     lib.kudnn_b200_grouped_set_wait.argtypes = [vp, ctypes.c_longlong, i32]
     lib.kudnn_b200_grouped_force_tile.argtypes = [vp, i32, i32]
     lib.kudnn_b200_grouped_last_tile.argtypes = [vp] + [ctypes.POINTER(ctypes.c_int)] * 3
+    lib.kudnn_b200_layernorm_validate.argtypes = [ctypes.POINTER(LayernormDesc)]
+    lib.kudnn_b200_layernorm_run.argtypes = [ctypes.POINTER(LayernormDesc)] + [vp] * 7
+    lib.kudnn_b200_layernorm_backward_workspace.argtypes = [ctypes.POINTER(LayernormDesc), ctypes.POINTER(i64)]
+    lib.kudnn_b200_layernorm_backward_run.argtypes = [ctypes.POINTER(LayernormDesc)] + [vp] * 9 + [i64, vp]
     lib.kudnn_b200_last_error.restype = ctypes.c_char_p
     lib.kudnn_b200_version.restype = ctypes.c_char_p
     _lib = lib
@@ -275,6 +292,37 @@ def rmsnorm(src, dst, rows, axis, dtype, scale=None, variance=None, flags=0, sav
     """RMS normalisation over the last axis of a dense [rows, axis] tensor; device or host pointers."""
     _check(library().kudnn_b200_rmsnorm_run(_ptr(src), _ptr(dst), _ptr(scale), _ptr(variance), rows, axis, dtype, flags,
                                             1 if save_stats else 0, eps, stream))
+
+
+def make_layernorm_desc(rows, axis, dtype, *, param_dtype=None, has_scale=False, has_shift=False, given_stats=False, eps=1e-5, x_ld=None,
+                        y_ld=None, dy_ld=None, dx_ld=None):
+    """Descriptor of the layer normalisation of [rows, axis] values and of its gradient; dense by default, scale and shift of the rows' type."""
+    d = LayernormDesc()
+    d.rows, d.axis = rows, axis
+    d.x_ld, d.y_ld, d.dy_ld, d.dx_ld = [axis if ld is None else ld for ld in (x_ld, y_ld, dy_ld, dx_ld)]
+    d.dtype, d.param_dtype = dtype, dtype if param_dtype is None else param_dtype
+    d.flags = (NORM_USE_SCALE if has_scale else 0) | (NORM_USE_SHIFT if has_shift else 0) | (NORM_USE_GLOBAL_STATS if given_stats else 0)
+    d.eps = eps
+    return d
+
+
+def layernorm(desc, x, y, scale=None, shift=None, mean=None, variance=None, stream=None):
+    """y = (x - mean) / sqrt(variance + eps) * scale + shift; mean and variance (fp32) are written unless given or None.  Device pointers,
+    asynchronous on `stream`."""
+    _check(library().kudnn_b200_layernorm_run(ctypes.byref(desc), _ptr(x), _ptr(scale), _ptr(shift), _ptr(y), _ptr(mean), _ptr(variance), stream))
+
+
+def layernorm_backward_workspace(desc):
+    """Bytes of scratch that layernorm_backward needs for dscale or dshift."""
+    size = ctypes.c_int64()
+    _check(library().kudnn_b200_layernorm_backward_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
+
+
+def layernorm_backward(desc, x, dy, scale, mean, variance, dx=None, dscale=None, dshift=None, workspace=None, workspace_bytes=0, stream=None):
+    """The gradients that are not None, of x, the scale and the shift; device pointers, asynchronous on `stream`."""
+    _check(library().kudnn_b200_layernorm_backward_run(ctypes.byref(desc), _ptr(x), _ptr(dy), _ptr(scale), _ptr(mean), _ptr(variance), _ptr(dx),
+                                                       _ptr(dscale), _ptr(dshift), _ptr(workspace), workspace_bytes, stream))
 
 
 SCALE_BLOCK = 128
