@@ -312,6 +312,63 @@ KUDNN_B200_API int kudnn_b200_grouped_set_wait(kudnn_b200_grouped_t handle, long
 KUDNN_B200_API int kudnn_b200_grouped_force_tile(kudnn_b200_grouped_t handle, int tile_rows, int rows_on_m);
 KUDNN_B200_API int kudnn_b200_grouped_last_tile(kudnn_b200_grouped_t handle, int *tile_rows, int *rows_on_m, int *splits);
 
+/* ---- a block of experts for few tokens, and its router ---------------------------------------------------------------
+ * No counterpart in the reference.  Device pointers only, each a multiple of its elements' size; asynchronous on the stream; forward only.
+ *
+ * Router: which `top` experts each token goes to, and with what weights.
+ *   logit[t, e] = sum over h of x[t, h] w[e, h], products and sums in 64 bits, so that the choice is that of the exact scores
+ *   score       = softmax of a token's logits over the experts that take part, or 1 / (1 + exp(-logit))
+ *   key         = score + bias[e] (without a bias: score)
+ * The experts with the largest keys are chosen, largest first, the lower index first among equals.  Their scores (without the bias) become
+ * the weights, with `normalise` divided by their sum, then times `scale`; fp32.  An expert whose bias is minus infinity or whose key is NaN
+ * takes no part; where fewer than `top` do, the places left over get the id -1 and the weight 0.
+ * x, w: F32 / F16 / BF16 at row pitches; bias fp32; ids int32 and weights fp32 are dense [tokens, top].  At most 1024 experts, top at most 64. */
+#define KUDNN_B200_SCORE_SOFTMAX 0
+#define KUDNN_B200_SCORE_SIGMOID 1
+typedef struct kudnn_b200_route_desc {
+    int64_t tokens, hidden, x_ld, w_ld;
+    int32_t experts, top, x_dtype, w_dtype, score, normalise;
+    float scale, reserved_f;
+} kudnn_b200_route_desc;
+KUDNN_B200_API int kudnn_b200_route_validate(const kudnn_b200_route_desc *desc);
+KUDNN_B200_API int kudnn_b200_route_run(const kudnn_b200_route_desc *desc, const void *x, const void *w, const float *bias, float *weights,
+                                        int32_t *ids, void *cuda_stream);
+
+/* Block of experts: with h = silu(gate[e] . x[t]) * (up[e] . x[t]),
+ *   y[t] = sum over j of weights[t, j] * down[e] . h,  e = ids[t, j].
+ * For at most 64 tokens and a top of at most 16 (decoding steps; larger batches: kudnn_b200_grouped_*).  Each chosen expert's weights are read
+ * once.  ids outside [0, experts) take no part, whatever their weights; a token without experts gets zeros; one that an id names twice has the
+ * expert once with both weights.
+ * gate_up [experts, 2 ffn, hidden] holds gate's rows, then up's; down [experts, hidden, ffn].  x and y: F16 or BF16; the weights of the same
+ * type or E4M3 with fp32 scales per 128 x 128 block of [2 ffn, hidden] and [hidden, ffn], as kudnn_b200_quantize_run writes them: x and h are
+ * not quantised.  Sums and h are held in 32 bits or as two 16-bit halves of them; y is rounded once.  The same call gives the same bits.
+ * y may be x.  Weights whose rows are K-contiguous, 16-byte aligned and 16 bytes apart or a multiple of it are streamed by the fast kernels;
+ * other strides take general ones, many times slower.
+ * The workspace: as many bytes of device memory as experts_workspace says (host arithmetic), on a 16-byte boundary, contents irrelevant, used by
+ * one run at a time. */
+typedef struct kudnn_b200_experts_desc {
+    int64_t tokens, hidden, ffn;
+    int32_t experts, top, x_dtype, w_dtype;
+    int64_t x_ld, y_ld;
+    int64_t gate_up_se, gate_up_sn, gate_up_sk;                   /* per expert, row, column, in elements */
+    int64_t down_se, down_sn, down_sk;
+    int64_t gate_up_scale_se, gate_up_scale_sn, gate_up_scale_sk; /* per expert, block of rows, block of columns */
+    int64_t down_scale_se, down_scale_sn, down_scale_sk;
+} kudnn_b200_experts_desc;
+typedef struct kudnn_b200_experts_args {
+    const void *x;
+    const float *weights;                    /* [tokens, top] */
+    const int32_t *ids;                      /* [tokens, top] */
+    const void *gate_up, *down;
+    const float *gate_up_scale, *down_scale; /* non-NULL iff w_dtype is E4M3 */
+    void *y;
+    void *workspace;
+    int64_t workspace_bytes;
+} kudnn_b200_experts_args;
+KUDNN_B200_API int kudnn_b200_experts_validate(const kudnn_b200_experts_desc *desc);
+KUDNN_B200_API int kudnn_b200_experts_workspace(const kudnn_b200_experts_desc *desc, int64_t *bytes);
+KUDNN_B200_API int kudnn_b200_experts_run(const kudnn_b200_experts_desc *desc, const kudnn_b200_experts_args *args, void *cuda_stream);
+
 /* Reads the device-side status word of the handle (bounded waits that gave up) after synchronising the stream. */
 KUDNN_B200_API int kudnn_b200_linear_check(kudnn_b200_linear_t handle, void *cuda_stream);
 

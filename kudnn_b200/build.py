@@ -29,7 +29,8 @@ NVCC_FLAGS = [
 
 CUDA_SOURCES = ["linear_api.cu", "simt_gemm.cu", "gemv.cu", "tc_gemm.cu", "tc_inst_f32.cu", "tc_inst_f16.cu", "tc_inst_bf16.cu",
                 "tc_inst_s8.cu", "tc_wide_f16.cu", "tc_wide_bf16.cu", "tc_wide_s8.cu", "tc_planes.cu", "pack.cu", "static_scratch.cu", "peer.cu", "eltwise.cu", "eltwise_api.cu", "quantize.cu",
-                "grouped_simt.cu", "grouped_tc.cu", "grouped_api.cu", "layernorm.cu", "layernorm_api.cu"]
+                "grouped_simt.cu", "grouped_tc.cu", "grouped_api.cu", "layernorm.cu", "layernorm_api.cu", "route.cu", "experts_any.cu",
+                "experts_api.cu"]
 
 
 def _nvcc():
@@ -76,7 +77,7 @@ def build_cuda(verbose=False, force=False, ptxas_info=False):
         objs.append(o)
         # the tensor-core kernels' own headers concern their own translation units only
         unused = "tc_wide" if src.startswith("tc_inst_") else "tc_inst" if src.startswith("tc_") else "tc_"
-        unused = (unused,) + tuple(part for part, users in (("grouped", ("grouped", "quantize")), ("layernorm", ("layernorm",)))
+        unused = (unused,) + tuple(part for part, users in (("grouped", ("grouped", "quantize")), ("layernorm", ("layernorm",)), ("experts", ("experts", "route")))
                                    if not src.startswith(users))
         deps = [h for h in headers if not os.path.basename(h).startswith(unused)]
         if force or not _newer(o, [s] + deps):

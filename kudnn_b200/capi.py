@@ -101,6 +101,38 @@ class LayernormDesc(ctypes.Structure):
     ]
 
 
+class RouteDesc(ctypes.Structure):
+    """kudnn_b200_route_desc."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("hidden", ctypes.c_int64), ("x_ld", ctypes.c_int64), ("w_ld", ctypes.c_int64),
+        ("experts", ctypes.c_int32), ("top", ctypes.c_int32), ("x_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
+        ("score", ctypes.c_int32), ("normalise", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved_f", ctypes.c_float),
+    ]
+
+
+class ExpertsDesc(ctypes.Structure):
+    """kudnn_b200_experts_desc."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("hidden", ctypes.c_int64), ("ffn", ctypes.c_int64),
+        ("experts", ctypes.c_int32), ("top", ctypes.c_int32), ("x_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
+        ("x_ld", ctypes.c_int64), ("y_ld", ctypes.c_int64),
+        ("gate_up_se", ctypes.c_int64), ("gate_up_sn", ctypes.c_int64), ("gate_up_sk", ctypes.c_int64),
+        ("down_se", ctypes.c_int64), ("down_sn", ctypes.c_int64), ("down_sk", ctypes.c_int64),
+        ("gate_up_scale_se", ctypes.c_int64), ("gate_up_scale_sn", ctypes.c_int64), ("gate_up_scale_sk", ctypes.c_int64),
+        ("down_scale_se", ctypes.c_int64), ("down_scale_sn", ctypes.c_int64), ("down_scale_sk", ctypes.c_int64),
+    ]
+
+
+class ExpertsArgs(ctypes.Structure):
+    """kudnn_b200_experts_args."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("gate_up", ctypes.c_void_p),
+                ("down", ctypes.c_void_p), ("gate_up_scale", ctypes.c_void_p), ("down_scale", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 EXPORTS = [
     "kudnn_b200_linear_validate", "kudnn_b200_linear_create", "kudnn_b200_linear_clone", "kudnn_b200_linear_destroy",
     "kudnn_b200_linear_prepack", "kudnn_b200_linear_run", "kudnn_b200_linear_run_host", "kudnn_b200_linear_check",
@@ -117,6 +149,8 @@ EXPORTS = [
     "kudnn_b200_grouped_last_kernel", "kudnn_b200_grouped_set_wait", "kudnn_b200_grouped_force_tile", "kudnn_b200_grouped_last_tile",
     "kudnn_b200_layernorm_validate", "kudnn_b200_layernorm_run", "kudnn_b200_layernorm_backward_workspace",
     "kudnn_b200_layernorm_backward_run",
+    "kudnn_b200_route_validate", "kudnn_b200_route_run", "kudnn_b200_experts_validate", "kudnn_b200_experts_workspace",
+    "kudnn_b200_experts_run",
 ]
 
 _lib = None
@@ -184,6 +218,11 @@ def library():
     lib.kudnn_b200_layernorm_run.argtypes = [ctypes.POINTER(LayernormDesc)] + [vp] * 7
     lib.kudnn_b200_layernorm_backward_workspace.argtypes = [ctypes.POINTER(LayernormDesc), ctypes.POINTER(i64)]
     lib.kudnn_b200_layernorm_backward_run.argtypes = [ctypes.POINTER(LayernormDesc)] + [vp] * 9 + [i64, vp]
+    lib.kudnn_b200_route_validate.argtypes = [ctypes.POINTER(RouteDesc)]
+    lib.kudnn_b200_route_run.argtypes = [ctypes.POINTER(RouteDesc)] + [vp] * 6
+    lib.kudnn_b200_experts_validate.argtypes = [ctypes.POINTER(ExpertsDesc)]
+    lib.kudnn_b200_experts_workspace.argtypes = [ctypes.POINTER(ExpertsDesc), ctypes.POINTER(i64)]
+    lib.kudnn_b200_experts_run.argtypes = [ctypes.POINTER(ExpertsDesc), ctypes.POINTER(ExpertsArgs), vp]
     lib.kudnn_b200_last_error.restype = ctypes.c_char_p
     lib.kudnn_b200_version.restype = ctypes.c_char_p
     _lib = lib
@@ -423,6 +462,53 @@ class Grouped:
         got = [ctypes.c_int() for _ in range(3)]
         _check(self._lib.kudnn_b200_grouped_last_tile(self._h, *[ctypes.byref(v) for v in got]))
         return got[0].value, got[1].value != 0, got[2].value
+
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
+
+def make_route_desc(tokens, experts, hidden, top, dtype, *, router_dtype=F32, score=SCORE_SOFTMAX, normalise=True, scale=1.0, x_ld=None, w_ld=None):
+    """Descriptor of the choice of `top` of `experts` experts for each of x [tokens, hidden] by a router [experts, hidden]; dense by default."""
+    d = RouteDesc()
+    d.tokens, d.experts, d.hidden, d.top = tokens, experts, hidden, top
+    d.x_dtype, d.w_dtype, d.score, d.normalise, d.scale = dtype, router_dtype, score, 1 if normalise else 0, scale
+    d.x_ld, d.w_ld = hidden if x_ld is None else x_ld, hidden if w_ld is None else w_ld
+    return d
+
+
+def route(desc, x, router, weights, ids, bias=None, stream=None):
+    """Writes the experts of each token (int32 [tokens, top], the largest score first) and their weights (fp32); device pointers, asynchronous."""
+    _check(library().kudnn_b200_route_run(ctypes.byref(desc), _ptr(x), _ptr(router), _ptr(bias), _ptr(weights), _ptr(ids), stream))
+
+
+def make_experts_desc(tokens, hidden, ffn, experts, top, dtype, *, weight_dtype=None, x_ld=None, y_ld=None, gate_up_strides=None, down_strides=None,
+                      gate_up_scale_strides=None, down_scale_strides=None):
+    """Descriptor of a block of experts for at most 64 tokens; gate_up [experts, 2 ffn, hidden], down [experts, hidden, ffn] and for E4M3 weights
+    their scales per 128 x 128, addressed by (expert, row, column) strides; dense by default."""
+    d = ExpertsDesc()
+    d.tokens, d.hidden, d.ffn, d.experts, d.top = tokens, hidden, ffn, experts, top
+    d.x_dtype, d.w_dtype = dtype, weight_dtype or dtype
+    d.x_ld, d.y_ld = hidden if x_ld is None else x_ld, hidden if y_ld is None else y_ld
+    up, across, inner = -(-2 * ffn // SCALE_BLOCK), -(-hidden // SCALE_BLOCK), -(-ffn // SCALE_BLOCK)
+    d.gate_up_se, d.gate_up_sn, d.gate_up_sk = gate_up_strides or (2 * ffn * hidden, hidden, 1)
+    d.down_se, d.down_sn, d.down_sk = down_strides or (hidden * ffn, ffn, 1)
+    d.gate_up_scale_se, d.gate_up_scale_sn, d.gate_up_scale_sk = gate_up_scale_strides or (up * across, across, 1)
+    d.down_scale_se, d.down_scale_sn, d.down_scale_sk = down_scale_strides or (across * inner, inner, 1)
+    return d
+
+
+def experts_workspace(desc):
+    """Bytes of device memory that experts needs."""
+    size = ctypes.c_int64()
+    _check(library().kudnn_b200_experts_workspace(ctypes.byref(desc), ctypes.byref(size)))
+    return size.value
+
+
+def experts(desc, x, weights, ids, gate_up, down, y, workspace, workspace_bytes, gate_up_scale=None, down_scale=None, stream=None):
+    """y[t] = sum over j of weights[t, j] * down[e](silu(gate[e](x[t])) * up[e](x[t])), e = ids[t, j]; device pointers, asynchronous on `stream`."""
+    args = ExpertsArgs(_ptr(x), _ptr(weights), _ptr(ids), _ptr(gate_up), _ptr(down), _ptr(gate_up_scale), _ptr(down_scale), _ptr(y),
+                       _ptr(workspace), workspace_bytes)
+    _check(library().kudnn_b200_experts_run(ctypes.byref(desc), ctypes.byref(args), stream))
 
 
 def debug_fail_allocation(nth):
