@@ -39,6 +39,9 @@ struct ExpertsParams {
     int x_dtype, w_dtype;
 };
 long long experts_workspace_bytes(long long tokens, long long top, long long ffn);
+// The kernels that stream the weights take K-contiguous rows on 16-byte boundaries; the general ones any.
+bool experts_stream_takes(const ExpertsParams &p);
+cudaError_t launch_experts_stream(const ExpertsParams &p, int sm_count, cudaStream_t stream);
 cudaError_t launch_experts_any(const ExpertsParams &p, cudaStream_t stream);
 
 // silu(gate) * up in fp32: e raised to a power below zero, so that the divisor lies in [1, 2]

@@ -234,7 +234,7 @@ int kudnn_b200_experts_run(const kudnn_b200_experts_desc *d, const kudnn_b200_ex
     p.x_dtype = d->x_dtype;
     p.w_dtype = d->w_dtype;
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-    const cudaError_t e = kb::launch_experts_any(p, stream);
+    const cudaError_t e = kb::experts_stream_takes(p) ? kb::launch_experts_stream(p, sms, stream) : kb::launch_experts_any(p, stream);
     return e == cudaSuccess ? KUDNN_B200_OK : fail_cuda(e, "experts kernel launch");
 }
 
