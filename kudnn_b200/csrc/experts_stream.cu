@@ -3,9 +3,9 @@
 // What bounds it is reading the chosen experts' weights; everything here serves to keep as many bytes in flight as HBM wants, without pauses:
 //   * Both products are cut by weight rows alone: the rows (gate and up rows in pairs) of all chosen experts are dealt out evenly, one CTA per SM,
 //     so that every SM streams the same number of bytes; nothing is added up across CTAs, no atomics, and the same call gives the same bits.
-//   * The 16 warps of a CTA stream on their own, without barriers.  First kernel: as many groups of warps as the CTA has tiles of rows, up to 16;
+//   * The 8 warps of a CTA stream on their own, without barriers.  First kernel: as many groups of warps as the CTA has tiles of rows, up to 8;
 //     a group's warps split K and add up at the end of a tile (with a tile per warp, what large batches have, nothing is added up).  Second
-//     kernel: each warp a sixteenth of all steps of all experts at the CTA's rows, with sums of y of its own, added up at the end.
+//     kernel: each warp an eighth of all steps of all experts at the CTA's rows, with sums of y of its own, added up at the end.
 //   * Every lane copies its own 16 bytes of a few rows into a ring in shared memory (cp.async, some steps ahead) and reads back only what it
 //     copied itself.  Copies of what lies beyond the last row or column bring zeros.
 //   * The lanes' pieces are, as they are, operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on that of 8;
@@ -22,7 +22,7 @@ namespace kb {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostPairs = kMostExpertTokens * kMostExpertTop;
 
@@ -39,6 +39,8 @@ struct Lists {
     float p[kMostPairs];
     int ids[kMostPairs];
     int active;
+    // first kernel: how many warps share a tile, how many tiles an expert's rows are cut into
+    int group_warps, tiles;
 };
 
 // All threads of the CTA.  An id that a token names twice counts once, with both weights.
@@ -105,9 +107,18 @@ __device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p)
     __syncthreads();
 }
 
-__device__ __forceinline__ void copy_16(uint32_t to, const void *from, int bytes)
+// 16 bytes, or zeros; or nothing at all
+__device__ __forceinline__ void copy_16(uint32_t to, const void *from, bool zeros, bool any)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    asm volatile(
+        "{\n\t"
+        ".reg .pred z, a;\n\t"
+        "setp.ne.b32 z, %2, 0;\n\t"
+        "setp.ne.b32 a, %3, 0;\n\t"
+        "@a cp.async.cg.shared.global [%0], [%1], 16, z;\n\t"
+        "}" ::"r"(to),
+        "l"(from), "r"(zeros ? 1 : 0), "r"(any ? 1 : 0)
+        : "memory");
 }
 
 template <bool kBf>
@@ -169,6 +180,17 @@ __device__ __forceinline__ uint4 load_8(const unsigned short *at, int left, bool
     return q;
 }
 
+// All but the first `left` bytes become zeros.
+__device__ __forceinline__ void keep_bytes(uint4 &q, int left)
+{
+    uint32_t *w[4] = {&q.x, &q.y, &q.z, &q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int have = left - 4 * i;
+        *w[i] = have >= 4 ? *w[i] : have <= 0 ? 0u : *w[i] & (0xffffffffu >> (32 - 8 * have));
+    }
+}
+
 // The value's upper tf32 half and what is left; a value that is not finite has no rest.
 __device__ __forceinline__ float2 split_tf32(float v)
 {
@@ -182,18 +204,19 @@ __device__ __forceinline__ long long h_pitch(const ExpertsParams &p)
     return (p.ffn + 63) / 64 * 64;
 }
 
-// A tile has 16 rows of weights, a step 128 bytes of each.
-constexpr int kRows = 16;
+// A tile has 32 rows of weights, a step 128 bytes of each.
+constexpr int kRows = 32;
+constexpr int kMostTilePairs = kRows / 2;  // of a gate's and an up's row
 constexpr int kStageBytes = kRows * 128;
 
 // The kernels for experts of up to 8 kTokens tokens: the ring, and behind it the warps' sums.
 template <bool kDown, int kTokens>
 struct Layout {
-    static constexpr int kTileRows = kDown ? kRows : kRows / 2;  // rows of y, or pairs of a gate's and an up's row
-    static constexpr int kStages = kTokens == 8 ? 4 : 5;
+    static constexpr int kTileRows = kDown ? kRows : kMostTilePairs;
+    static constexpr int kStages = kTokens == 8 && kDown ? 4 : 5;
     static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
     // up: the sums of 8 tokens of every warp, in two buffers; down: each warp's sums of y
-    static constexpr int kSumBytes = kDown ? kWarps * 8 * kTokens * kRows * 4 : 2 * kWarps * 512;
+    static constexpr int kSumBytes = kDown ? kWarps * 8 * kTokens * kRows * 4 : 2 * kWarps * 1024;
     static constexpr size_t kBytes = kRingBytes + kSumBytes + sizeof(Lists);
 };
 
@@ -202,31 +225,30 @@ template <bool kDown, int kTileRows>
 struct Cursor {
     int rank, row, rows;       // the expert, its first row (of the gate, or of down), how many
     int step, steps, stride;   // of K
-    long long at, end;         // up: pairs of rows of all active experts, one after the other; down: rows of y
+    long long at, end;         // up: tiles of all active experts, one after the other; down: rows of y
     long long begin, until, position;  // down: the warp's steps of all experts at the same rows
     int depth;                 // steps of an expert
     int offset;                // up: of the warp in its group
-    __device__ __forceinline__ void start_up(const ExpertsParams &p, const Lists &l, int warp, int group_warps, int depth_steps)
+    __device__ __forceinline__ void start_up(const Lists &l, int warp, int depth_steps)
     {
-        const long long all = static_cast<long long>(l.active) * p.ffn;
-        const long long from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
-        const int groups = kWarps / group_warps, group = warp / group_warps;
-        at = from + (to - from) * group / groups;
-        end = from + (to - from) * (group + 1) / groups;
-        offset = warp % group_warps;
-        stride = group_warps;
+        const int groups = kWarps / l.group_warps;
+        // consecutive tiles go to different SMs; next_up() adds a whole round
+        at = (warp / l.group_warps - groups) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
+        end = static_cast<long long>(l.active) * l.tiles;
+        offset = warp % l.group_warps;
+        stride = l.group_warps;
         depth = depth_steps;
-        rows = 0;
     }
-    __device__ __forceinline__ bool next_up(const ExpertsParams &p)
+    __device__ __forceinline__ bool next_up(const ExpertsParams &p, const Lists &l)
     {
-        at += rows;
+        at += kWarps / l.group_warps * static_cast<int>(gridDim.x);
         if (at >= end) {
             return false;
         }
-        rank = static_cast<int>(at / p.ffn);
-        row = static_cast<int>(at - static_cast<long long>(rank) * p.ffn);
-        equal_tile(min(end - at, static_cast<long long>(p.ffn - row)));
+        rank = static_cast<int>(at / l.tiles);
+        const int tile = static_cast<int>(at - static_cast<long long>(rank) * l.tiles);
+        row = static_cast<int>(static_cast<long long>(p.ffn) * tile / l.tiles);
+        rows = static_cast<int>(static_cast<long long>(p.ffn) * (tile + 1) / l.tiles) - row;
         step = offset;
         steps = depth > offset ? (depth - offset + stride - 1) / stride : 0;
         return true;
@@ -273,6 +295,36 @@ struct Cursor {
     }
 };
 
+// How the first kernel's tiles are cut, by one warp: with kWarps / w groups of w warps per SM and r rounds of tiles, an expert's rows are cut into
+// as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (about 24 a cycle), or the
+// steps of a warp at what one takes in latency where HBM waits (about 800 cycles), and the sums of a group.
+__device__ __forceinline__ void plan_tiles(Lists &l, const ExpertsParams &p, int depth_steps, int lane)
+{
+    const int w = 1 << (lane & 3), extra = lane >> 2;
+    const long long groups = static_cast<long long>(kWarps / w) * gridDim.x;
+    const int least = (p.ffn + kMostTilePairs - 1) / kMostTilePairs;
+    const long long rounds = (static_cast<long long>(l.active) * least + groups - 1) / groups + extra;
+    const int tiles = static_cast<int>(min(static_cast<long long>(p.ffn), max(rounds * groups / max(l.active, 1), static_cast<long long>(least))));
+    const int pairs = (p.ffn + tiles - 1) / tiles;
+    const float steps = static_cast<float>((depth_steps + w - 1) / w);
+    const float bytes = static_cast<float>(kWarps / w * pairs) * 256.0f * static_cast<float>(depth_steps);
+    float cost = static_cast<float>(rounds) * (fmaxf(bytes / 24.0f, 800.0f * steps) + (w > 1 ? 600.0f : 300.0f));
+    int at = lane;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, cost, o);
+        const int other_at = __shfl_xor_sync(0xffffffffu, at, o);
+        if (other < cost || (other == cost && other_at < at)) {
+            cost = other;
+            at = other_at;
+        }
+    }
+    if (at == lane) {
+        l.group_warps = w;
+        l.tiles = tiles;
+    }
+}
+
 // kTokens: an expert's most, in eights.
 template <Weights kW, bool kBf, bool kDown, int kTokens>
 __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __grid_constant__ ExpertsParams p)
@@ -284,10 +336,11 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     constexpr int kPiece = 16 / kElem;                // of a lane, twice in a step
     constexpr bool kTf32 = kDown && kW == kF16;       // h in fp32, products of tf32
     constexpr bool kBfMma = kW == kBf16 || (kW == kE4m3 && (kBf || kDown));
+    constexpr int kPlanes = kDown ? 2 : 1, kLoads = kPiece / 8;
     extern __shared__ __align__(16) unsigned char shared[];
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     unsigned char *ring = shared + warp * kStages * kStageBytes;
-    float4 *sums = reinterpret_cast<float4 *>(shared + L::kRingBytes);  // up: [2][kWarps][32]
+    float4 *sums = reinterpret_cast<float4 *>(shared + L::kRingBytes);  // up: [2][kWarps][2][32]
     float *y_sums = reinterpret_cast<float *>(shared + L::kRingBytes);  // down: [kWarps][tokens][kRows]
     Lists &lists = *reinterpret_cast<Lists *>(shared + L::kRingBytes + L::kSumBytes);
     const int depth = kDown ? p.ffn : p.hidden;  // K
@@ -300,73 +353,74 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     }
     make_lists(lists, p);
 
-    // up: warps that share a tile, as few as leave no group without one
-    int group_warps = 1;
     if (!kDown) {
-        const long long pairs = static_cast<long long>(lists.active) * p.ffn / gridDim.x + 1;
-        group_warps = kWarps;
-        while (group_warps > 1 && pairs > static_cast<long long>(kWarps / group_warps) * L::kTileRows) {
-            group_warps /= 2;
+        if (warp == 0) {
+            plan_tiles(lists, p, (depth + kStep - 1) / kStep, lane);
         }
+        __syncthreads();
     }
-
-    // ---- the stream: copy i of a step brings 128 bytes of rows 4 i .. 4 i + 3, the chunk of 16 bytes in place c ^ 4 (row % 2), so that the
-    // fragments are read without bank conflicts
     using Place = Cursor<kDown, L::kTileRows>;
     auto start = [&](Place &c) {
         if (kDown) {
             c.start_down(p, lists, warp, (depth + kStep - 1) / kStep);
         } else {
-            c.start_up(p, lists, warp, group_warps, (depth + kStep - 1) / kStep);
+            c.start_up(lists, warp, (depth + kStep - 1) / kStep);
         }
     };
+    // the next piece with steps of its own; false: none is left
+    auto advance = [&](Place &c) {
+        do {
+            if (kDown) {
+                while (!c.next_down()) {
+                    if (!c.next_rows() || c.position >= c.until) {
+                        return false;  // no rows are left, or this warp has no steps at any
+                    }
+                }
+            } else if (!c.next_up(p, lists)) {
+                return false;
+            }
+        } while (c.steps == 0);
+        return true;
+    };
+
+    // ---- the stream: copy i of a step brings 128 bytes of rows 4 i .. 4 i + 3, the chunk of 16 bytes in place c ^ 4 (row % 2), so that the
+    // fragments are read without bank conflicts
     const int copy_row = lane >> 3, chunk = lane & 7;
     const uint32_t copy_to = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) +
                              static_cast<uint32_t>(copy_row * 128 + (chunk ^ (copy_row & 1) * 4) * 16);
-    const char *row_at[4];
-    int row_here = 0;  // bit i: the row of copy i exists
+    const char *row_at[8];  // of the lane's copies, at its next chunk
+    int row_here = 0;       // bit i: the row of copy i exists; where it does not, what the ring holds meets rows of sums that nobody reads
     int ahead_k = 0, ahead_left = 0, ahead_stage = 0;
     Place ahead;
     start(ahead);
-    // the next piece with steps of its own
-    auto advance = [&]() {
-        do {
-            if (kDown) {
-                while (!ahead.next_down()) {
-                    if (!ahead.next_rows() || ahead.position >= ahead.until) {
-                        return;  // no rows are left, or this warp has no steps at any
-                    }
-                }
-            } else if (!ahead.next_up(p)) {
-                return;
-            }
+    auto aim = [&]() {
+        ahead_left = 0;
+        if (advance(ahead)) {
             ahead_left = ahead.steps;
-        } while (ahead_left == 0);
-        ahead_k = ahead.step * kStep + chunk * kPiece;
-        row_here = 0;
-        const char *expert = weights + lists.expert[ahead.rank] * se * kElem;
+            ahead_k = ahead.step * kStep + chunk * kPiece;
+            const char *first = weights + (lists.expert[ahead.rank] * se + ahead.row * sn + ahead_k) * kElem;
+            row_here = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int in_tile = i * 4 + copy_row, r = kDown ? in_tile : in_tile & 7;  // up: eight of the gate, then their eight of the up
-            const bool here = r < ahead.rows;
-            const long long row = ahead.row + r + (!kDown && i >= 2 ? p.ffn : 0);
-            row_at[i] = here ? expert + row * sn * kElem : weights;
-            row_here |= here ? 1 << i : 0;
+            for (int i = 0; i < 8; ++i) {  // up: eight of the gate, the same eight of the up, twice
+                const int r = (kDown ? i * 4 : (i >> 2) * 8 + (i & 1) * 4) + copy_row;
+                row_at[i] = first + (r + (!kDown && (i & 2) != 0 ? p.ffn : 0)) * sn * kElem;
+                row_here |= r < ahead.rows ? 1 << i : 0;
+            }
         }
     };
-    advance();
+    aim();
     auto issue = [&]() {
         if (ahead_left > 0) {
-            const int bytes = max(0, min(16, (depth - ahead_k) * kElem));
+            const bool beyond = ahead_k >= depth;
             const uint32_t to = copy_to + static_cast<uint32_t>(ahead_stage * kStageBytes);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int n = (row_here >> i & 1) != 0 ? bytes : 0;
-                copy_16(to + i * 512, row_at[i] + (n > 0 ? static_cast<long long>(ahead_k) * kElem : 0), n);
+            for (int i = 0; i < 8; ++i) {
+                copy_16(to + i * 512, beyond ? weights : row_at[i], beyond, (row_here >> i & 1) != 0);
+                row_at[i] += ahead.stride * 128;
             }
             ahead_k += ahead.stride * kStep;
             if (--ahead_left == 0) {
-                advance();
+                aim();
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -385,139 +439,204 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
         __syncthreads();
     }
 
-    // ---- the products
+    // ---- the tokens' fragments of a step, and its scales: the first eight tokens' are fetched one step ahead
     const long long pitch = h_pitch(p);
-    const int h_rows = p.tokens * p.top;
-    const unsigned short *x = static_cast<const unsigned short *>(p.x), *h = static_cast<const unsigned short *>(p.h);
+    const long long plane_step = static_cast<long long>(p.tokens) * p.top * pitch;
     const bool vector = kDown || ((reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && p.x_ld % 8 == 0);
     const float *scale = kDown ? p.down_scale : p.gate_up_scale;
     const long long ss_e = kDown ? p.ds_se : p.gus_se, ss_n = kDown ? p.ds_sn : p.gus_sn, ss_k = kDown ? p.ds_sk : p.gus_sk;
-    // where this lane's fragments of rows g and g + 8 lie: chunks t and t + 4
+    struct Tokens {
+        uint4 q[2][kPlanes][kLoads];  // [which 64 bytes of weights]; kTf32: [..][which four][0]
+    };
+    // at: the row of x or h of this lane's token (of lanes without one: of any, their sums are dropped); from element k on; whole: all of the
+    // step's elements exist, on 16-byte boundaries
+    auto load_tokens = [&](Tokens &b, const void *at, int k, bool whole) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int from_k = k + u * 4 * kPiece, some = depth - from_k;
+            if (kTf32) {
+                const float *from = static_cast<const float *>(at) + from_k;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (whole || some >= 4 * i + 4) {
+                        v = reinterpret_cast<const float4 *>(from)[i];
+                    } else if (some > 4 * i) {
+                        v.x = from[4 * i];
+                        v.y = some > 4 * i + 1 ? from[4 * i + 1] : 0.0f;
+                        v.z = some > 4 * i + 2 ? from[4 * i + 2] : 0.0f;
+                    }
+                    b.q[u][i][0] = *reinterpret_cast<const uint4 *>(&v);
+                }
+            } else {
+#pragma unroll
+                for (int plane = 0; plane < kPlanes; ++plane) {
+                    const unsigned short *from = static_cast<const unsigned short *>(at) + plane * plane_step + from_k;
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        b.q[u][plane][i] = whole ? reinterpret_cast<const uint4 *>(from)[i] : load_8(from + i * 8, some - i * 8, vector);
+                    }
+                }
+            }
+        }
+    };
+    auto token_row = [&](int pair) -> const void * {
+        if (kTf32) {
+            return static_cast<const float *>(p.h) + pair * pitch;
+        }
+        return kDown ? static_cast<const unsigned short *>(p.h) + pair * pitch
+                     : static_cast<const unsigned short *>(p.x) + lists.token[pair] * p.x_ld;
+    };
+    Tokens next;
+    float next_scale[4];
+    Place soon;
+    start(soon);
+    int soon_left = 0, soon_step = 0;
+    const void *soon_row = nullptr;
+    const float *soon_scale[4];
+    auto fetch = [&]() {
+        if (soon_left == 0) {
+            if (!advance(soon)) {
+                return;
+            }
+            soon_left = soon.steps;
+            soon_step = soon.step;
+            const int first = lists.first[soon.rank];
+            soon_row = token_row(first + (g < lists.count[soon.rank] ? g : 0));
+            if (kW == kE4m3) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // rows g + 8 i, or g and g of the up, then 8 on
+                    const int r = min(kDown ? i * 8 + g : (i >> 1) * 8 + g, soon.rows - 1);
+                    soon_scale[i] = scale + lists.expert[soon.rank] * ss_e + (soon.row + r + (!kDown && (i & 1) != 0 ? p.ffn : 0)) / 128 * ss_n;
+                }
+            }
+        }
+        load_tokens(next, soon_row, soon_step * kStep + t * kPiece, vector && (soon_step + 1) * kStep <= depth);
+        if (kW == kE4m3) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                next_scale[i] = soon_scale[i][soon_step * ss_k];
+            }
+        }
+        soon_step += soon.stride;
+        --soon_left;
+    };
+    fetch();
+
+    // ---- the products
+    // where this lane's fragments of row g lie: chunks t and t + 4
     const unsigned char *fragment = ring + g * 128 + (t ^ (g & 1) * 4) * 16;
     const int other = (g & 1) != 0 ? -64 : 64;
     int stage = 0, turn = 0;
-    float c[kTokens][4];
+    float c[kTokens][2][4];
 
     auto multiply = [&](const Place &now) {
-        const int expert = lists.expert[now.rank], first = lists.first[now.rank], count = lists.count[now.rank];
-        const int eights = (count + 7) / 8;
+        const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
 #pragma unroll
         for (int n = 0; n < kTokens; ++n) {
-            c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
-        }
-        const float *scale_at[2];
-        if (kW == kE4m3) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = min(kDown ? i * 8 + g : g, now.rows - 1);
-                scale_at[i] = scale + expert * ss_e + (now.row + r + (!kDown && i != 0 ? p.ffn : 0)) / 128 * ss_n;
+            for (int m = 0; m < 2; ++m) {
+                c[n][m][0] = c[n][m][1] = c[n][m][2] = c[n][m][3] = 0.0f;
             }
         }
         int step = now.step;
 #pragma unroll 1
         for (int s = 0; s < now.steps; ++s, step += now.stride) {
-            const int k = step * kStep + t * kPiece, left = depth - k;
-            float of_block[2];
+            Tokens b = next;
+            float of_block[4];
             if (kW == kE4m3) {
-                of_block[0] = scale_at[0][step * ss_k];
-                of_block[1] = scale_at[1][step * ss_k];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    of_block[i] = next_scale[i];
+                }
             }
-            uint4 a[2][2];  // [which 64 bytes][row g or g + 8]
-            bool arrived = false;
+            fetch();
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncwarp();
+            uint4 a[2][4];  // [which 64 bytes][row g + 8 i of the tile's 32]
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const unsigned char *at = fragment + stage * kStageBytes + r * 1024;
+                a[0][r] = *reinterpret_cast<const uint4 *>(at);
+                a[1][r] = *reinterpret_cast<const uint4 *>(at + other);
+            }
+            const bool whole = (step + 1) * kStep <= depth;
+            if (!whole && depth % kPiece != 0) {
+                // what lies behind the last column may be anything, and no number times zero
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        keep_bytes(a[u][r], (depth - (step * kStep + t * kPiece + u * 4 * kPiece)) * kElem);
+                    }
+                }
+            }
 #pragma unroll
             for (int n = 0; n < kTokens; ++n) {
                 if (n < eights) {
-                    const int column = n * 8 + g;
-                    const bool here = column < count;
-                    const int have = here ? left : 0;
-                    constexpr int kPlanes = kDown ? 2 : 1, kLoads = kPiece / 8;
-                    uint4 b[2][kPlanes][kLoads];  // the tokens' fragments; kTf32: 8 values of fp32
+                    if (n > 0) {
+                        load_tokens(b, token_row(first + (n * 8 + g < count ? n * 8 + g : 0)), step * kStep + t * kPiece, vector && whole);
+                    }
+                    // two chains of sums in turn: the matrix instructions of one wait for one another
+                    float part[2][4];
+                    if (kW == kE4m3) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int from_k = k + u * 4 * kPiece, some = have - u * 4 * kPiece;
-                        if (kTf32) {
-                            const float *from = static_cast<const float *>(p.h) + (first + (here ? column : 0)) * pitch + from_k;
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                if (some >= 4 * i + 4) {
-                                    v = reinterpret_cast<const float4 *>(from)[i];
-                                } else if (some > 4 * i) {
-                                    v.x = from[4 * i];
-                                    v.y = some > 4 * i + 1 ? from[4 * i + 1] : 0.0f;
-                                    v.z = some > 4 * i + 2 ? from[4 * i + 2] : 0.0f;
-                                }
-                                b[u][i][0] = *reinterpret_cast<const uint4 *>(&v);
-                            }
-                        } else {
-#pragma unroll
-                            for (int plane = 0; plane < kPlanes; ++plane) {
-                                const unsigned short *from =
-                                    kDown ? h + (static_cast<long long>(plane) * h_rows + first + (here ? column : 0)) * pitch + from_k
-                                          : x + lists.token[first + (here ? column : 0)] * p.x_ld + from_k;
-#pragma unroll
-                                for (int i = 0; i < kLoads; ++i) {
-                                    b[u][plane][i] = load_8(from + i * 8, some - i * 8, vector);
-                                }
-                            }
+                        for (int m = 0; m < 2; ++m) {
+                            part[m][0] = part[m][1] = part[m][2] = part[m][3] = 0.0f;
                         }
                     }
-                    if (!arrived) {
-                        // the weights, behind the first tokens' loads
-                        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-                        __syncwarp();
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const unsigned char *at = fragment + stage * kStageBytes + r * 1024;
-                            a[0][r] = *reinterpret_cast<const uint4 *>(at);
-                            a[1][r] = *reinterpret_cast<const uint4 *>(at + other);
-                        }
-                        arrived = true;
-                    }
-                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    float(&to)[4] = kW == kE4m3 ? part : c[n];
+                    float(&to)[2][4] = kW == kE4m3 ? part : c[n];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         if (kTf32) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const uint4 &q = b[u][j / 2][0];
+                                const uint4 &q = b.q[u][j / 2][0];
                                 const float2 b0 = split_tf32(__uint_as_float(word(q, j % 2 * 2)));
                                 const float2 b1 = split_tf32(__uint_as_float(word(q, j % 2 * 2 + 1)));
-                                const uint32_t w0 = word(a[u][0], j), w1 = word(a[u][1], j);
-                                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&w0));
-                                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&w1));
-                                mma_tf32(to, f0.x, f1.x, f0.y, f1.y, b0.y, b1.y);
-                                mma_tf32(to, f0.x, f1.x, f0.y, f1.y, b0.x, b1.x);
+                                float2 f[4];
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    const uint32_t w = word(a[u][r], j);
+                                    f[r] = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                                }
+                                mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.y, b1.y);
+                                mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.y, b1.y);
+                                mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.x, b1.x);
+                                mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.x, b1.x);
                             }
                         } else {
 #pragma unroll
                             for (int j = 0; j < 2 * kLoads; ++j) {
-                                uint32_t a0, a1, a2, a3;
-                                if (kW == kE4m3) {
-                                    const uint32_t w0 = word(a[u][0], j), w1 = word(a[u][1], j);
-                                    a0 = widen_e4m3<kBfMma>(w0, false);
-                                    a1 = widen_e4m3<kBfMma>(w1, false);
-                                    a2 = widen_e4m3<kBfMma>(w0, true);
-                                    a3 = widen_e4m3<kBfMma>(w1, true);
-                                } else {
-                                    a0 = word(a[u][0], 2 * j);
-                                    a1 = word(a[u][1], 2 * j);
-                                    a2 = word(a[u][0], 2 * j + 1);
-                                    a3 = word(a[u][1], 2 * j + 1);
+                                uint32_t w[2][4];
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    if (kW == kE4m3) {
+                                        w[r / 2][r % 2] = widen_e4m3<kBfMma>(word(a[u][r], j), false);
+                                        w[r / 2][2 + r % 2] = widen_e4m3<kBfMma>(word(a[u][r], j), true);
+                                    } else {
+                                        w[r / 2][r % 2] = word(a[u][r], 2 * j);
+                                        w[r / 2][2 + r % 2] = word(a[u][r], 2 * j + 1);
+                                    }
                                 }
 #pragma unroll
                                 for (int plane = kPlanes - 1; plane >= 0; --plane) {
-                                    const uint4 &q = b[u][plane][j / 2];
-                                    mma_16<kBfMma>(to, a0, a1, a2, a3, word(q, j % 2 * 2), word(q, j % 2 * 2 + 1));
+                                    const uint4 &q = b.q[u][plane][j / 2];
+#pragma unroll
+                                    for (int m = 0; m < 2; ++m) {
+                                        mma_16<kBfMma>(to[m], w[m][0], w[m][1], w[m][2], w[m][3], word(q, j % 2 * 2), word(q, j % 2 * 2 + 1));
+                                    }
                                 }
                             }
                         }
                     }
                     if (kW == kE4m3) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            c[n][i] = fmaf(part[i], of_block[i / 2], c[n][i]);
+                        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                c[n][m][i] = fmaf(part[m][i], of_block[2 * m + i / 2], c[n][m][i]);
+                            }
                         }
                     }
                 }
@@ -538,10 +657,11 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 const float hi = __bfloat162float(__float2bfloat16_rn(v));
                 unsigned short *planes = static_cast<unsigned short *>(p.h);
                 planes[to] = f32_to_bf16_rne_bits(v);
-                planes[h_rows * pitch + to] = f32_to_bf16_rne_bits(isfinite(hi) ? v - hi : 0.0f);
+                planes[plane_step + to] = f32_to_bf16_rne_bits(isfinite(hi) ? v - hi : 0.0f);
             }
         };
-        while (now.next_up(p)) {
+        const int group_warps = lists.group_warps;
+        while (now.next_up(p, lists)) {
             multiply(now);
             const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
 #pragma unroll
@@ -549,30 +669,35 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 if (n < eights) {
                     if (group_warps == 1) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int column = n * 8 + 2 * t + j;
-                            if (g < now.rows && column < count) {
-                                store_h((first + column) * pitch + now.row + g, c[n][j], c[n][2 + j]);
+                        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const int r = m * 8 + g, column = n * 8 + 2 * t + j;
+                                if (r < now.rows && column < count) {
+                                    store_h((first + column) * pitch + now.row + r, c[n][m][j], c[n][m][2 + j]);
+                                }
                             }
                         }
                     } else {
                         // the group's sums, eight tokens at a time; two buffers take turns, so that one barrier does
-                        float4 *buffer = sums + turn * kWarps * 32;
+                        float4 *buffer = sums + turn * kWarps * 64;
                         turn ^= 1;
-                        buffer[warp * 32 + lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            buffer[warp * 64 + m * 32 + lane] = make_float4(c[n][m][0], c[n][m][1], c[n][m][2], c[n][m][3]);
+                        }
                         const int group = warp / group_warps, threads = group_warps * 32;
                         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
-                        const float *from = reinterpret_cast<const float *>(buffer + group * threads);
-                        const int i = tid % threads;
-                        if (i < 64) {
-                            const int of = i >> 1, j = i & 1;  // element j of lane `of`, and the one of the up's row
+                        const float *from = reinterpret_cast<const float *>(buffer + group * group_warps * 64);
+                        for (int i = tid % threads; i < 128; i += threads) {
+                            const int m = i >> 6, of = i >> 1 & 31, j = i & 1;  // element j of lane `of`, and the one of the up's row
                             float gate = 0.0f, up = 0.0f;
                             for (int w = 0; w < group_warps; ++w) {
-                                const float *at = from + (w * 32 + of) * 4 + j;
+                                const float *at = from + (w * 64 + m * 32 + of) * 4 + j;
                                 gate += at[0];
                                 up += at[2];
                             }
-                            const int r = of >> 2, column = n * 8 + (of & 3) * 2 + j;
+                            const int r = m * 8 + (of >> 2), column = n * 8 + (of & 3) * 2 + j;
                             if (r < now.rows && column < count) {
                                 store_h((first + column) * pitch + now.row + r, gate, up);
                             }
@@ -596,8 +721,11 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                             if (column < count) {
                                 float *to = mine + lists.token[first + column] * kRows + g;
                                 const float weight = lists.p[first + column];
-                                to[0] = fmaf(weight, c[n][j], to[0]);
-                                to[8] = fmaf(weight, c[n][2 + j], to[8]);
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) {
+                                    to[m * 16] = fmaf(weight, c[n][m][j], to[m * 16]);
+                                    to[m * 16 + 8] = fmaf(weight, c[n][m][2 + j], to[m * 16 + 8]);
+                                }
                             }
                         }
                     }
