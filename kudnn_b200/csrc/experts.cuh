@@ -42,6 +42,8 @@ long long experts_workspace_bytes(long long tokens, long long top, long long ffn
 // The kernels that stream the weights take K-contiguous rows on 16-byte boundaries; the general ones any.
 bool experts_stream_takes(const ExpertsParams &p);
 cudaError_t launch_experts_stream(const ExpertsParams &p, int sm_count, cudaStream_t stream);
+void experts_set_wait(long long limit_cycles, int skip_step);
+cudaError_t experts_take_status(DeviceStatus *status);  // of the current device, and clears it
 cudaError_t launch_experts_any(const ExpertsParams &p, cudaStream_t stream);
 
 // silu(gate) * up in fp32: e raised to a power below zero, so that the divisor lies in [1, 2]

@@ -6,17 +6,20 @@
 //   * The 8 warps of a CTA stream on their own, without barriers.  First kernel: as many groups of warps as the CTA has tiles of rows, up to 8;
 //     a group's warps split K and add up at the end of a tile (with a tile per warp, what large batches have, nothing is added up).  Second
 //     kernel: each warp an eighth of all steps of all experts at the CTA's rows, with sums of y of its own, added up at the end.
-//   * Every lane copies its own 16 bytes of a few rows into a ring in shared memory (cp.async, some steps ahead) and reads back only what it
-//     copied itself.  Copies of what lies beyond the last row or column bring zeros.
-//   * The lanes' pieces are, as they are, operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on that of 8;
-//     four neighbouring lanes hold 64 neighbouring bytes of a row.  The tokens' fragments are read from L1 and L2 in the same permutation.
+//   * A step of a warp is 128 bytes of up to 32 rows: up to four TMA boxes of eight rows, into a ring of the warp's own, some steps ahead.  Rows and
+//     columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their products are dropped).  (Copies by every lane,
+//     cp.async or straight into registers, took three to five times the instructions of the products, and their latency bound the whole.)
+//   * 16 bytes per lane, as they lie in the ring, are operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on
+//     that of 8.  The tokens' fragments are read from L1 and L2 in the same permutation, one step ahead.
 //   * The second kernel starts its copies of `down` while the first one ends (its CTAs take the place of the first one's as those leave) and
 //     waits only before it reads h.
 // h is kept as the tensor cores take it without loss: two bf16 halves (of bf16 and e4m3 weights), or fp32 that the second kernel splits into two
 // tf32 halves (of fp16 weights: halves of fp16 would overflow beyond 65504 and lose small values).
 #include "experts.cuh"
+#include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace kb {
 
@@ -27,6 +30,17 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMostPairs = kMostExpertTokens * kMostExpertTop;
 
 enum Weights { kBf16, kF16, kE4m3 };
+
+// Waits that gave up, on this device since the last look.
+__device__ DeviceStatus experts_status;
+
+struct Waits {
+    long long limit;  // in cycles
+    int skip_step;    // test hook: from which step of K on nothing is copied, -1 off
+};
+std::atomic<long long> wait_limit{0};
+std::atomic<int> wait_skip{-1};
+
 
 // Which tokens the experts have: pairs in order of experts and tokens.
 struct Lists {
@@ -40,7 +54,10 @@ struct Lists {
     int ids[kMostPairs];
     int active;
     // first kernel: how many warps share a tile, how many tiles an expert's rows are cut into
-    int group_warps, tiles;
+    // of at least tile_pairs pairs of rows, the first `longer` of one more
+    int group_warps, tiles, tile_pairs, longer;
+    int abort;  // some wait of the CTA gave up
+    unsigned long long full[kWarps][8];
 };
 
 // All threads of the CTA.  An id that a token names twice counts once, with both weights.
@@ -107,20 +124,6 @@ __device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p)
     __syncthreads();
 }
 
-// 16 bytes, or zeros; or nothing at all
-__device__ __forceinline__ void copy_16(uint32_t to, const void *from, bool zeros, bool any)
-{
-    asm volatile(
-        "{\n\t"
-        ".reg .pred z, a;\n\t"
-        "setp.ne.b32 z, %2, 0;\n\t"
-        "setp.ne.b32 a, %3, 0;\n\t"
-        "@a cp.async.cg.shared.global [%0], [%1], 16, z;\n\t"
-        "}" ::"r"(to),
-        "l"(from), "r"(zeros ? 1 : 0), "r"(any ? 1 : 0)
-        : "memory");
-}
-
 template <bool kBf>
 __device__ __forceinline__ void mma_16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -180,17 +183,6 @@ __device__ __forceinline__ uint4 load_8(const unsigned short *at, int left, bool
     return q;
 }
 
-// All but the first `left` bytes become zeros.
-__device__ __forceinline__ void keep_bytes(uint4 &q, int left)
-{
-    uint32_t *w[4] = {&q.x, &q.y, &q.z, &q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int have = left - 4 * i;
-        *w[i] = have >= 4 ? *w[i] : have <= 0 ? 0u : *w[i] & (0xffffffffu >> (32 - 8 * have));
-    }
-}
-
 // The value's upper tf32 half and what is left; a value that is not finite has no rest.
 __device__ __forceinline__ float2 split_tf32(float v)
 {
@@ -207,127 +199,127 @@ __device__ __forceinline__ long long h_pitch(const ExpertsParams &p)
 // A tile has 32 rows of weights, a step 128 bytes of each.
 constexpr int kRows = 32;
 constexpr int kMostTilePairs = kRows / 2;  // of a gate's and an up's row
+constexpr int kBoxRows = 8;
+constexpr int kBoxBytes = kBoxRows * 128;
 constexpr int kStageBytes = kRows * 128;
 
 // The kernels for experts of up to 8 kTokens tokens: the ring, and behind it the warps' sums.
 template <bool kDown, int kTokens>
 struct Layout {
-    static constexpr int kTileRows = kDown ? kRows : kMostTilePairs;
     static constexpr int kStages = kTokens == 8 && kDown ? 4 : 5;
     static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
     // up: the sums of 8 tokens of every warp, in two buffers; down: each warp's sums of y
     static constexpr int kSumBytes = kDown ? kWarps * 8 * kTokens * kRows * 4 : 2 * kWarps * 1024;
-    static constexpr size_t kBytes = kRingBytes + kSumBytes + sizeof(Lists);
+    static constexpr size_t kBytes = kRingBytes + kSumBytes + sizeof(Lists) + 1024;  // the ring begins on a multiple of 1024
 };
 
-// A warp's way through the weights, piece by piece: steps of K of up to kTileRows rows of one expert.
-template <bool kDown, int kTileRows>
+// A warp's way through the weights, piece by piece: steps of K of a tile of one expert's rows.  32 bits hold every count (see the launcher).
+template <bool kDown>
 struct Cursor {
     int rank, row, rows;       // the expert, its first row (of the gate, or of down), how many
     int step, steps, stride;   // of K
-    long long at, end;         // up: tiles of all active experts, one after the other; down: rows of y
-    long long begin, until, position;  // down: the warp's steps of all experts at the same rows
     int depth;                 // steps of an expert
-    int offset;                // up: of the warp in its group
+    int at, end;               // up: tiles of all active experts, one after the other; down: rows of y
+    int offset;                // up: of the warp in its group; down: its first step
+    __device__ __forceinline__ void count_steps()
+    {
+        step = offset;
+        steps = depth > offset ? static_cast<int>(static_cast<unsigned>(depth - offset + stride - 1) / static_cast<unsigned>(stride)) : 0;
+    }
     __device__ __forceinline__ void start_up(const Lists &l, int warp, int depth_steps)
     {
-        const int groups = kWarps / l.group_warps;
         // consecutive tiles go to different SMs; next_up() adds a whole round
-        at = (warp / l.group_warps - groups) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
-        end = static_cast<long long>(l.active) * l.tiles;
-        offset = warp % l.group_warps;
+        at = (warp / l.group_warps - kWarps / l.group_warps) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
+        end = l.active * l.tiles;
         stride = l.group_warps;
+        offset = warp & (stride - 1);
         depth = depth_steps;
+        count_steps();
     }
-    __device__ __forceinline__ bool next_up(const ExpertsParams &p, const Lists &l)
+    __device__ __forceinline__ bool next_up(const Lists &l)
     {
-        at += kWarps / l.group_warps * static_cast<int>(gridDim.x);
+        at += kWarps / stride * static_cast<int>(gridDim.x);
         if (at >= end) {
             return false;
         }
-        rank = static_cast<int>(at / l.tiles);
-        const int tile = static_cast<int>(at - static_cast<long long>(rank) * l.tiles);
-        row = static_cast<int>(static_cast<long long>(p.ffn) * tile / l.tiles);
-        rows = static_cast<int>(static_cast<long long>(p.ffn) * (tile + 1) / l.tiles) - row;
-        step = offset;
-        steps = depth > offset ? (depth - offset + stride - 1) / stride : 0;
+        rank = static_cast<int>(static_cast<unsigned>(at) / static_cast<unsigned>(l.tiles));
+        const int tile = at - rank * l.tiles;
+        row = tile * l.tile_pairs + min(tile, l.longer);
+        rows = l.tile_pairs + (tile < l.longer ? 1 : 0);
         return true;
     }
-    __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int warp, int depth_steps)
+    // Down: the steps of all experts at the same rows are dealt out to the warps one by one, so that together they read what lies side by side.
+    __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int depth_steps)
     {
-        at = static_cast<long long>(p.hidden) * blockIdx.x / gridDim.x;
-        end = static_cast<long long>(p.hidden) * (blockIdx.x + 1) / gridDim.x;
+        at = static_cast<int>(static_cast<unsigned>(p.hidden) * blockIdx.x / gridDim.x);
+        end = static_cast<int>(static_cast<unsigned>(p.hidden) * (blockIdx.x + 1) / gridDim.x);
         depth = depth_steps;
-        const long long all = static_cast<long long>(l.active) * depth;  // at most 1024 x 2^26: 64 bits
-        begin = all * warp / kWarps;
-        until = all * (warp + 1) / kWarps;
-        stride = 1;
+        stride = kWarps;
         rows = 0;
-        position = until;
+        rank = l.active;
     }
-    // Down: true while the warp has pieces at the present rows.
-    __device__ __forceinline__ bool next_down()
+    // true while there are experts at the present rows
+    __device__ __forceinline__ bool next_down(const Lists &l)
     {
-        if (position >= until) {
+        if (rank + 1 >= l.active) {
             return false;
         }
-        rank = static_cast<int>(position / depth);
-        step = static_cast<int>(position - static_cast<long long>(rank) * depth);
-        steps = static_cast<int>(min(until - position, static_cast<long long>(depth - step)));
-        position += steps;
+        ++rank;
+        offset = (offset - depth) & (kWarps - 1);
+        count_steps();
         return true;
     }
-    __device__ __forceinline__ bool next_rows()
+    __device__ __forceinline__ bool next_rows(int warp)
     {
         at += rows;
         if (at >= end) {
             return false;
         }
-        row = static_cast<int>(at);
-        equal_tile(end - at);
-        position = begin;
+        row = at;
+        const int tiles = (end - at + kRows - 1) / kRows;  // equal ones
+        rows = (end - at + tiles - 1) / tiles;
+        rank = -1;
+        offset = warp + depth;
         return true;
-    }
-    __device__ __forceinline__ void equal_tile(long long left)
-    {
-        const int tiles = static_cast<int>((left + kTileRows - 1) / kTileRows);
-        rows = static_cast<int>((left + tiles - 1) / tiles);
     }
 };
 
 // How the first kernel's tiles are cut, by one warp: with kWarps / w groups of w warps per SM and r rounds of tiles, an expert's rows are cut into
-// as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (about 24 a cycle), or the
-// steps of a warp at what one takes in latency where HBM waits (about 800 cycles), and the sums of a group.
+// as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (24 a cycle; a tenth more
+// where no warps read side by side), or the steps of a warp at what one takes in latency where HBM waits (800 cycles), and the sums of a group.
 __device__ __forceinline__ void plan_tiles(Lists &l, const ExpertsParams &p, int depth_steps, int lane)
 {
-    const int w = 1 << (lane & 3), extra = lane >> 2;
-    const long long groups = static_cast<long long>(kWarps / w) * gridDim.x;
-    const int least = (p.ffn + kMostTilePairs - 1) / kMostTilePairs;
-    const long long rounds = (static_cast<long long>(l.active) * least + groups - 1) / groups + extra;
-    const int tiles = static_cast<int>(min(static_cast<long long>(p.ffn), max(rounds * groups / max(l.active, 1), static_cast<long long>(least))));
+    const int w = 1 << (lane & 3), extra = lane >> 2, active = max(l.active, 1);
+    const unsigned groups = kWarps / w * gridDim.x;
+    const unsigned least = (p.ffn + kMostTilePairs - 1) / kMostTilePairs;
+    const unsigned rounds = (active * least + groups - 1) / groups + extra;
+    const int tiles = static_cast<int>(min(static_cast<unsigned>(p.ffn), max(rounds * groups / active, least)));
     const int pairs = (p.ffn + tiles - 1) / tiles;
     const float steps = static_cast<float>((depth_steps + w - 1) / w);
     const float bytes = static_cast<float>(kWarps / w * pairs) * 256.0f * static_cast<float>(depth_steps);
-    float cost = static_cast<float>(rounds) * (fmaxf(bytes / 24.0f, 800.0f * steps) + (w > 1 ? 600.0f : 300.0f));
-    int at = lane;
+    float cost = static_cast<float>(rounds) * (fmaxf(bytes / (w > 2 ? 24.0f : w > 1 ? 23.0f : 21.5f), 800.0f * steps) + (w > 1 ? 600.0f : 300.0f));
+    int best = lane;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float other = __shfl_xor_sync(0xffffffffu, cost, o);
-        const int other_at = __shfl_xor_sync(0xffffffffu, at, o);
-        if (other < cost || (other == cost && other_at < at)) {
+        const int other_best = __shfl_xor_sync(0xffffffffu, best, o);
+        if (other < cost || (other == cost && other_best < best)) {
             cost = other;
-            at = other_at;
+            best = other_best;
         }
     }
-    if (at == lane) {
+    if (best == lane) {
         l.group_warps = w;
         l.tiles = tiles;
+        l.tile_pairs = p.ffn / tiles;
+        l.longer = p.ffn % tiles;
     }
 }
 
 // kTokens: an expert's most, in eights.
 template <Weights kW, bool kBf, bool kDown, int kTokens>
-__global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __grid_constant__ ExpertsParams p)
+__global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __grid_constant__ ExpertsParams p, const __grid_constant__ CUtensorMap map,
+                                                                     const __grid_constant__ Waits waits)
 {
     using L = Layout<kDown, kTokens>;
     constexpr int kStages = L::kStages;
@@ -337,15 +329,24 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     constexpr bool kTf32 = kDown && kW == kF16;       // h in fp32, products of tf32
     constexpr bool kBfMma = kW == kBf16 || (kW == kE4m3 && (kBf || kDown));
     constexpr int kPlanes = kDown ? 2 : 1, kLoads = kPiece / 8;
-    extern __shared__ __align__(16) unsigned char shared[];
+    extern __shared__ unsigned char raw[];
+    unsigned char *shared = raw + (1024u - (smem_u32(raw) & 1023u)) % 1024u;
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     unsigned char *ring = shared + warp * kStages * kStageBytes;
     float4 *sums = reinterpret_cast<float4 *>(shared + L::kRingBytes);  // up: [2][kWarps][2][32]
     float *y_sums = reinterpret_cast<float *>(shared + L::kRingBytes);  // down: [kWarps][tokens][kRows]
     Lists &lists = *reinterpret_cast<Lists *>(shared + L::kRingBytes + L::kSumBytes);
     const int depth = kDown ? p.ffn : p.hidden;  // K
-    const char *weights = static_cast<const char *>(kDown ? p.down : p.gate_up);
-    const long long se = kDown ? p.d_se : p.gu_se, sn = kDown ? p.d_sn : p.gu_sn;
+    uint64_t *full = reinterpret_cast<uint64_t *>(lists.full[warp]);  // a barrier per stage of the warp's ring
+    volatile int *abort_flag = &lists.abort;
+    if (tid == 0) {
+        lists.abort = 0;
+    }
+    if (lane < kStages) {
+        mbar_init(full + lane, 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 
     if (!kDown) {
         pdl_wait();
@@ -359,10 +360,10 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
         }
         __syncthreads();
     }
-    using Place = Cursor<kDown, L::kTileRows>;
+    using Place = Cursor<kDown>;
     auto start = [&](Place &c) {
         if (kDown) {
-            c.start_down(p, lists, warp, (depth + kStep - 1) / kStep);
+            c.start_down(p, lists, (depth + kStep - 1) / kStep);
         } else {
             c.start_up(lists, warp, (depth + kStep - 1) / kStep);
         }
@@ -371,63 +372,54 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     auto advance = [&](Place &c) {
         do {
             if (kDown) {
-                while (!c.next_down()) {
-                    if (!c.next_rows() || c.position >= c.until) {
-                        return false;  // no rows are left, or this warp has no steps at any
+                while (!c.next_down(lists)) {
+                    if (lists.active == 0 || !c.next_rows(warp)) {
+                        return false;
                     }
                 }
-            } else if (!c.next_up(p, lists)) {
+            } else if (!c.next_up(lists)) {
                 return false;
             }
         } while (c.steps == 0);
         return true;
     };
 
-    // ---- the stream: copy i of a step brings 128 bytes of rows 4 i .. 4 i + 3, the chunk of 16 bytes in place c ^ 4 (row % 2), so that the
-    // fragments are read without bank conflicts
-    const int copy_row = lane >> 3, chunk = lane & 7;
-    const uint32_t copy_to = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) +
-                             static_cast<uint32_t>(copy_row * 128 + (chunk ^ (copy_row & 1) * 4) * 16);
-    const char *row_at[8];  // of the lane's copies, at its next chunk
-    int row_here = 0;       // bit i: the row of copy i exists; where it does not, what the ring holds meets rows of sums that nobody reads
-    int ahead_k = 0, ahead_left = 0, ahead_stage = 0;
+    // ---- the stream: lane i < 4 brings eight rows (up: of the gate, of the up, and the next eight of both)
+    int box_row = 0, boxes = 0;
+    int ahead_k = 0, ahead_left = 0, ahead_stage = 0, ahead_expert = 0;
     Place ahead;
     start(ahead);
     auto aim = [&]() {
         ahead_left = 0;
         if (advance(ahead)) {
             ahead_left = ahead.steps;
-            ahead_k = ahead.step * kStep + chunk * kPiece;
-            const char *first = weights + (lists.expert[ahead.rank] * se + ahead.row * sn + ahead_k) * kElem;
-            row_here = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // up: eight of the gate, the same eight of the up, twice
-                const int r = (kDown ? i * 4 : (i >> 2) * 8 + (i & 1) * 4) + copy_row;
-                row_at[i] = first + (r + (!kDown && (i & 2) != 0 ? p.ffn : 0)) * sn * kElem;
-                row_here |= r < ahead.rows ? 1 << i : 0;
-            }
+            ahead_k = ahead.step * kStep;
+            ahead_expert = lists.expert[ahead.rank];
+            boxes = kDown ? (ahead.rows + 7) / 8 : ahead.rows > 8 ? 4 : 2;
+            box_row = ahead.row + (kDown ? lane * 8 : (lane >> 1) * 8 + (lane & 1) * p.ffn);
         }
     };
     aim();
+    bool gave_up = false;
     auto issue = [&]() {
         if (ahead_left > 0) {
-            const bool beyond = ahead_k >= depth;
-            const uint32_t to = copy_to + static_cast<uint32_t>(ahead_stage * kStageBytes);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                copy_16(to + i * 512, beyond ? weights : row_at[i], beyond, (row_here >> i & 1) != 0);
-                row_at[i] += ahead.stride * 128;
+            if (lane < boxes && !gave_up) {
+                if (lane == 0) {
+                    mbar_expect_tx(full + ahead_stage, boxes * kBoxBytes);
+                }
+                if (waits.skip_step < 0 || ahead_k / kStep < waits.skip_step) {
+                    tma_load_3d(ring + ahead_stage * kStageBytes + lane * kBoxBytes, &map, full + ahead_stage, ahead_k, box_row, ahead_expert);
+                }
             }
             ahead_k += ahead.stride * kStep;
             if (--ahead_left == 0) {
                 aim();
             }
+            ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
     };
 #pragma unroll 1
-    for (int i = 0; i < kStages - 1; ++i) {
+    for (int i = 0; i < kStages; ++i) {
         issue();
     }
     if (kDown) {
@@ -524,10 +516,11 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     fetch();
 
     // ---- the products
-    // where this lane's fragments of row g lie: chunks t and t + 4
-    const unsigned char *fragment = ring + g * 128 + (t ^ (g & 1) * 4) * 16;
-    const int other = (g & 1) != 0 ? -64 : 64;
+    // where this lane's fragments of row g lie: chunks t and t + 4, which the copies put in place t ^ g and so on
+    const unsigned char *fragment = ring + g * 128 + (t ^ g) * 16;
+    const int other = (g & 4) != 0 ? -64 : 64;
     int stage = 0, turn = 0;
+    uint32_t parity = 0;
     float c[kTokens][2][4];
 
     auto multiply = [&](const Place &now) {
@@ -551,8 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 }
             }
             fetch();
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            __syncwarp();
+            gave_up = gave_up || !mbar_wait(full + stage, parity, abort_flag, &experts_status, kDown ? 2 : 1, waits.limit);
             uint4 a[2][4];  // [which 64 bytes][row g + 8 i of the tile's 32]
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -561,16 +553,8 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 a[1][r] = *reinterpret_cast<const uint4 *>(at + other);
             }
             const bool whole = (step + 1) * kStep <= depth;
-            if (!whole && depth % kPiece != 0) {
-                // what lies behind the last column may be anything, and no number times zero
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        keep_bytes(a[u][r], (depth - (step * kStep + t * kPiece + u * 4 * kPiece)) * kElem);
-                    }
-                }
-            }
+            __syncwarp();
+            issue();  // into the stage that has just been read
 #pragma unroll
             for (int n = 0; n < kTokens; ++n) {
                 if (n < eights) {
@@ -641,8 +625,10 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                     }
                 }
             }
-            issue();
-            stage = stage + 1 == kStages ? 0 : stage + 1;
+            if (++stage == kStages) {
+                stage = 0;
+                parity ^= 1u;
+            }
         }
     };
 
@@ -661,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
             }
         };
         const int group_warps = lists.group_warps;
-        while (now.next_up(p, lists)) {
+        while (now.next_up(lists)) {
             multiply(now);
             const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
 #pragma unroll
@@ -708,8 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
         }
     } else {
         float *mine = y_sums + warp * p.tokens * kRows;
-        while (now.next_rows()) {
-            while (now.next_down()) {
+        while (now.next_rows(warp)) {
+            while (now.next_down(lists)) {
                 multiply(now);
                 const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
 #pragma unroll
@@ -747,7 +733,13 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
             __syncthreads();
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (gave_up) {
+        // the copies that are still on their way, each for a moment
+        for (int i = 0; i < kStages; ++i) {
+            for (int spin = 0; spin < 100000 && !mbar_try_wait(full + i, parity ^ (i < stage ? 1u : 0u)); ++spin) {
+            }
+        }
+    }
 }
 
 template <Weights kW, bool kBf, bool kDown, int kTokens>
@@ -755,9 +747,17 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
 {
     constexpr size_t kShared = Layout<kDown, kTokens>::kBytes;
     static_assert(kShared <= 227 * 1024, "shared memory");
-    const cudaError_t e =
-        cudaFuncSetAttribute(experts_stream_kernel<kW, kBf, kDown, kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kShared));
-    return e != cudaSuccess ? e : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count), dim3(kThreads), kShared, stream, 1u, p);
+    alignas(64) CUtensorMap map;
+    cudaError_t e = tc_encode_groups(&map, kDown ? p.down : p.gate_up, p.w_dtype, p.experts, kDown ? p.hidden : 2ll * p.ffn, kDown ? p.ffn : p.hidden,
+                                     std::max(kDown ? p.d_se : p.gu_se, 16ll), kDown ? p.d_sn : p.gu_sn, kBoxRows);
+    if (e == cudaSuccess) {
+        e = cudaFuncSetAttribute(experts_stream_kernel<kW, kBf, kDown, kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kShared));
+    }
+    const long long limit = wait_limit.load();
+    const Waits waits = {limit > 0 ? limit : kDefaultWaitLimitCycles, wait_skip.load()};
+    return e != cudaSuccess
+               ? e
+               : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count), dim3(kThreads), kShared, stream, 1u, p, map, waits);
 }
 
 template <Weights kW, bool kBf, int kTokens>
@@ -778,14 +778,35 @@ cudaError_t launch_tokens(const ExpertsParams &p, int sm_count, cudaStream_t str
 
 }  // namespace
 
-// K-contiguous rows on 16-byte boundaries; the tokens may begin anywhere
+// K-contiguous rows on 16-byte boundaries; the tokens may begin anywhere.  Sizes whose counts of rows, tiles and steps 32 bits hold: 148 x 2^22
+// rows, 1024 experts x 2^22 / 16 tiles (and a round or eight more).
 bool experts_stream_takes(const ExpertsParams &p)
 {
+    if (p.hidden > 1 << 22 || p.ffn > 1 << 22) {
+        return false;
+    }
     const long long elem = p.w_dtype == KUDNN_B200_E4M3 ? 1 : 2;
     auto rows = [&](const void *w, long long se, long long sn, long long sk, long long depth) {
-        return (sk == 1 || depth == 1) && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && se * elem % 16 == 0 && sn * elem % 16 == 0;
+        return (sk == 1 || depth == 1) && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && se * elem % 16 == 0 && sn * elem % 16 == 0 && sn > 0 &&
+               (se > 0 || p.experts == 1) && se < 1ll << 38 && sn < 1ll << 38;
     };
     return rows(p.gate_up, p.gu_se, p.gu_sn, p.gu_sk, p.hidden) && rows(p.down, p.d_se, p.d_sn, p.d_sk, p.ffn);
+}
+
+void experts_set_wait(long long limit_cycles, int skip_step)
+{
+    wait_limit.store(limit_cycles);
+    wait_skip.store(skip_step);
+}
+
+cudaError_t experts_take_status(DeviceStatus *status)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(status, experts_status, sizeof(DeviceStatus));
+    if (e == cudaSuccess && status->code != kErrNone) {
+        const DeviceStatus none = {};
+        e = cudaMemcpyToSymbol(experts_status, &none, sizeof(DeviceStatus));
+    }
+    return e;
 }
 
 cudaError_t launch_experts_stream(const ExpertsParams &p, int sm_count, cudaStream_t stream)
