@@ -51,7 +51,8 @@ struct Lists {
     short count[kMostExperts];
     unsigned char token[kMostPairs];
     float p[kMostPairs];
-    int ids[kMostPairs];
+    int ids[kMostPairs];  // as given, and the weights
+    float given[kMostPairs];
     int active;
     // first kernel: how many warps share a tile, how many tiles an expert's rows are cut into
     // of at least tile_pairs pairs of rows, the first `longer` of one more
@@ -59,70 +60,6 @@ struct Lists {
     int abort;  // some wait of the CTA gave up
     unsigned long long full[kWarps][8];
 };
-
-// All threads of the CTA.  An id that a token names twice counts once, with both weights.
-__device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p)
-{
-    const int pairs = p.tokens * p.top, tid = static_cast<int>(threadIdx.x);
-    for (int e = tid; e < p.experts; e += kThreads) {
-        l.tokens[e] = 0ull;
-    }
-    for (int i = tid; i < pairs; i += kThreads) {
-        l.ids[i] = p.ids[i];
-    }
-    __syncthreads();
-    for (int i = tid; i < pairs; i += kThreads) {
-        const int e = l.ids[i];
-        if (e >= 0 && e < p.experts) {
-            atomicOr(&l.tokens[e], 1ull << (i / p.top));  // whatever the order
-        }
-    }
-    __syncthreads();
-    if (tid < 32) {
-        int active = 0, first = 0;
-        for (int e0 = 0; e0 < p.experts; e0 += 32) {
-            const int e = e0 + tid, count = e < p.experts ? __popcll(l.tokens[e]) : 0;
-            const unsigned some = __ballot_sync(0xffffffffu, count > 0);
-            int sum = count;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, sum, o);
-                sum += tid >= o ? other : 0;
-            }
-            if (count > 0) {
-                const int at = active + __popc(some & ((1u << tid) - 1u)), start = first + sum - count;
-                l.start[e] = static_cast<short>(start);
-                l.expert[at] = static_cast<short>(e);
-                l.first[at] = static_cast<short>(start);
-                l.count[at] = static_cast<short>(count);
-            }
-            active += __popc(some);
-            first += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (tid == 0) {
-            l.active = active;
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < pairs; i += kThreads) {
-        const int e = l.ids[i], t = i / p.top;
-        if (e >= 0 && e < p.experts) {
-            bool again = false;
-            float sum = 0.0f;
-            for (int j = t * p.top; j < (t + 1) * p.top; ++j) {
-                const bool same = l.ids[j] == e;
-                again |= same && j < i;
-                sum += same ? p.p[j] : 0.0f;
-            }
-            if (!again) {
-                const int at = l.start[e] + __popcll(l.tokens[e] & ((1ull << t) - 1ull));
-                l.token[at] = static_cast<unsigned char>(t);
-                l.p[at] = sum;
-            }
-        }
-    }
-    __syncthreads();
-}
 
 template <bool kBf>
 __device__ __forceinline__ void mma_16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -165,22 +102,27 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t w, bool upper)
     return *reinterpret_cast<const uint32_t *>(&b);
 }
 
-// 8 values of 16 bits from `at`, of which `left` exist, mostly all or (lanes without a token) none; vector: `at` is on a 16-byte boundary
-__device__ __forceinline__ uint4 load_8(const unsigned short *at, int left, bool vector)
+// The first `left` of 8 values of 16 bits (a loop: it is seldom run, and must not become instructions of the path beside it)
+__device__ __forceinline__ uint4 load_some(const unsigned short *at, int left)
 {
-    uint4 q = make_uint4(0u, 0u, 0u, 0u);
-    if (vector && left >= 8) {
-        q = *reinterpret_cast<const uint4 *>(at);
-    } else if (left > 0) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = 2 * i < left ? at[2 * i] : 0u, hi = 2 * i + 1 < left ? at[2 * i + 1] : 0u;
-            w[i] = lo | hi << 16;
-        }
-        q = make_uint4(w[0], w[1], w[2], w[3]);
+    unsigned long long lo = 0ull, hi = 0ull;
+#pragma unroll 1
+    for (int i = min(left, 8) - 1; i >= 0; --i) {
+        hi = hi << 16 | lo >> 48;
+        lo = lo << 16 | at[i];
     }
-    return q;
+    return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
+}
+// The first `left` of 4 values of fp32
+__device__ __forceinline__ uint4 load_some(const float *at, int left)
+{
+    unsigned long long lo = 0ull, hi = 0ull;
+#pragma unroll 1
+    for (int i = min(left, 4) - 1; i >= 0; --i) {
+        hi = hi << 32 | lo >> 32;
+        lo = lo << 32 | __float_as_uint(at[i]);
+    }
+    return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
 }
 
 // The value's upper tf32 half and what is left; a value that is not finite has no rest.
@@ -220,12 +162,8 @@ struct Cursor {
     int step, steps, stride;   // of K
     int depth;                 // steps of an expert
     int at, end;               // up: tiles of all active experts, one after the other; down: rows of y
-    int offset;                // up: of the warp in its group; down: its first step
-    __device__ __forceinline__ void count_steps()
-    {
-        step = offset;
-        steps = depth > offset ? static_cast<int>(static_cast<unsigned>(depth - offset + stride - 1) / static_cast<unsigned>(stride)) : 0;
-    }
+    int offset;                // of the warp in its group
+    int begin, until, begin_rank, position;  // down: the group's steps of all experts, one after the other
     __device__ __forceinline__ void start_up(const Lists &l, int warp, int depth_steps)
     {
         // consecutive tiles go to different SMs; next_up() adds a whole round
@@ -234,7 +172,8 @@ struct Cursor {
         stride = l.group_warps;
         offset = warp & (stride - 1);
         depth = depth_steps;
-        count_steps();
+        step = offset;
+        steps = depth > offset ? (depth - offset + stride - 1) / stride : 0;
     }
     __device__ __forceinline__ bool next_up(const Lists &l)
     {
@@ -248,28 +187,36 @@ struct Cursor {
         rows = l.tile_pairs + (tile < l.longer ? 1 : 0);
         return true;
     }
-    // Down: the steps of all experts at the same rows are dealt out to the warps one by one, so that together they read what lies side by side.
-    __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int depth_steps)
+    // Down: the steps of all experts at the same rows go to groups of warps, as many to each, and a group's warps take turns, so that they read
+    // what lies side by side; groups of as many warps as leave each eight steps of an expert.
+    __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int warp, int depth_steps)
     {
         at = static_cast<int>(static_cast<unsigned>(p.hidden) * blockIdx.x / gridDim.x);
         end = static_cast<int>(static_cast<unsigned>(p.hidden) * (blockIdx.x + 1) / gridDim.x);
         depth = depth_steps;
-        stride = kWarps;
+        stride = depth >= 64 ? 8 : depth >= 32 ? 4 : depth >= 16 ? 2 : 1;
+        const int groups = kWarps / stride, group = warp / stride, all = l.active * depth;
+        begin = all * group / groups;
+        until = all * (group + 1) / groups;
+        begin_rank = begin / depth;
+        offset = warp & (stride - 1);
         rows = 0;
-        rank = l.active;
+        position = until;
     }
-    // true while there are experts at the present rows
-    __device__ __forceinline__ bool next_down(const Lists &l)
+    // true while the group has steps at the present rows
+    __device__ __forceinline__ bool next_down()
     {
-        if (rank + 1 >= l.active) {
+        if (position >= until) {
             return false;
         }
         ++rank;
-        offset = (offset - depth) & (kWarps - 1);
-        count_steps();
+        const int from = position - rank * depth, to = min(depth, until - rank * depth);
+        step = from + offset;
+        steps = to > step ? (to - step + stride - 1) / stride : 0;
+        position += to - from;
         return true;
     }
-    __device__ __forceinline__ bool next_rows(int warp)
+    __device__ __forceinline__ bool next_rows()
     {
         at += rows;
         if (at >= end) {
@@ -278,8 +225,8 @@ struct Cursor {
         row = at;
         const int tiles = (end - at + kRows - 1) / kRows;  // equal ones
         rows = (end - at + tiles - 1) / tiles;
-        rank = -1;
-        offset = warp + depth;
+        rank = begin_rank - 1;
+        position = begin;
         return true;
     }
 };
@@ -287,14 +234,14 @@ struct Cursor {
 // How the first kernel's tiles are cut, by one warp: with kWarps / w groups of w warps per SM and r rounds of tiles, an expert's rows are cut into
 // as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (24 a cycle; a tenth more
 // where no warps read side by side), or the steps of a warp at what one takes in latency where HBM waits (800 cycles), and the sums of a group.
-__device__ __forceinline__ void plan_tiles(Lists &l, const ExpertsParams &p, int depth_steps, int lane)
+__device__ __forceinline__ void plan_tiles(Lists &l, int active, int ffn, int depth_steps, int lane)
 {
-    const int w = 1 << (lane & 3), extra = lane >> 2, active = max(l.active, 1);
+    const int w = 1 << (lane & 3), extra = lane >> 2, some = max(active, 1);
     const unsigned groups = kWarps / w * gridDim.x;
-    const unsigned least = (p.ffn + kMostTilePairs - 1) / kMostTilePairs;
-    const unsigned rounds = (active * least + groups - 1) / groups + extra;
-    const int tiles = static_cast<int>(min(static_cast<unsigned>(p.ffn), max(rounds * groups / active, least)));
-    const int pairs = (p.ffn + tiles - 1) / tiles;
+    const unsigned least = (ffn + kMostTilePairs - 1) / kMostTilePairs;
+    const unsigned rounds = (some * least + groups - 1) / groups + extra;
+    const int tiles = static_cast<int>(min(static_cast<unsigned>(ffn), max(rounds * groups / some, least)));
+    const int pairs = (ffn + tiles - 1) / tiles;
     const float steps = static_cast<float>((depth_steps + w - 1) / w);
     const float bytes = static_cast<float>(kWarps / w * pairs) * 256.0f * static_cast<float>(depth_steps);
     float cost = static_cast<float>(rounds) * (fmaxf(bytes / (w > 2 ? 24.0f : w > 1 ? 23.0f : 21.5f), 800.0f * steps) + (w > 1 ? 600.0f : 300.0f));
@@ -311,9 +258,72 @@ __device__ __forceinline__ void plan_tiles(Lists &l, const ExpertsParams &p, int
     if (best == lane) {
         l.group_warps = w;
         l.tiles = tiles;
-        l.tile_pairs = p.ffn / tiles;
-        l.longer = p.ffn % tiles;
+        l.tile_pairs = ffn / tiles;
+        l.longer = ffn % tiles;
     }
+}
+
+// All threads of the CTA; l.tokens is zero.  An id that a token names twice counts once, with both weights.
+template <bool kPlan>
+__device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p, int depth_steps)
+{
+    const int pairs = p.tokens * p.top, tid = static_cast<int>(threadIdx.x);
+    for (int i = tid; i < pairs; i += kThreads) {
+        const int e = p.ids[i];
+        l.ids[i] = e;
+        l.given[i] = p.p[i];
+        if (e >= 0 && e < p.experts) {
+            atomicOr(&l.tokens[e], 1ull << (i / p.top));  // whatever the order
+        }
+    }
+    __syncthreads();
+    if (tid < 32) {
+        int active = 0, first = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + tid, count = e < p.experts ? __popcll(l.tokens[e]) : 0;
+            const unsigned some = __ballot_sync(0xffffffffu, count > 0);
+            int sum = count;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, o);
+                sum += tid >= o ? other : 0;
+            }
+            if (count > 0) {
+                const int at = active + __popc(some & ((1u << tid) - 1u)), start = first + sum - count;
+                l.start[e] = static_cast<short>(start);
+                l.expert[at] = static_cast<short>(e);
+                l.first[at] = static_cast<short>(start);
+                l.count[at] = static_cast<short>(count);
+            }
+            active += __popc(some);
+            first += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (tid == 0) {
+            l.active = active;
+        }
+        if (kPlan) {
+            plan_tiles(l, active, p.ffn, depth_steps, tid);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < pairs; i += kThreads) {
+        const int e = l.ids[i], t = i / p.top;
+        if (e >= 0 && e < p.experts) {
+            bool again = false;
+            float sum = 0.0f;
+            for (int j = t * p.top; j < (t + 1) * p.top; ++j) {
+                const bool same = l.ids[j] == e;
+                again |= same && j < i;
+                sum += same ? l.given[j] : 0.0f;
+            }
+            if (!again) {
+                const int at = l.start[e] + __popcll(l.tokens[e] & ((1ull << t) - 1ull));
+                l.token[at] = static_cast<unsigned char>(t);
+                l.p[at] = sum;
+            }
+        }
+    }
+    __syncthreads();
 }
 
 // kTokens: an expert's most, in eights.
@@ -348,32 +358,33 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 
+    if (warp == 0 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    }
+    for (int e = tid; e < p.experts; e += kThreads) {
+        lists.tokens[e] = 0ull;
+    }
+    __syncthreads();
+    const int depth_steps = (depth + kStep - 1) / kStep;
     if (!kDown) {
         pdl_wait();
         pdl_launch_dependents();  // behind the wait: what the second kernel reads ahead of its own is older than this one
     }
-    make_lists(lists, p);
-
-    if (!kDown) {
-        if (warp == 0) {
-            plan_tiles(lists, p, (depth + kStep - 1) / kStep, lane);
-        }
-        __syncthreads();
-    }
+    make_lists<!kDown>(lists, p, depth_steps);
     using Place = Cursor<kDown>;
     auto start = [&](Place &c) {
         if (kDown) {
-            c.start_down(p, lists, (depth + kStep - 1) / kStep);
+            c.start_down(p, lists, warp, depth_steps);
         } else {
-            c.start_up(lists, warp, (depth + kStep - 1) / kStep);
+            c.start_up(lists, warp, depth_steps);
         }
     };
     // the next piece with steps of its own; false: none is left
     auto advance = [&](Place &c) {
         do {
             if (kDown) {
-                while (!c.next_down(lists)) {
-                    if (lists.active == 0 || !c.next_rows(warp)) {
+                while (!c.next_down()) {
+                    if (!c.next_rows() || c.begin == c.until) {
                         return false;
                     }
                 }
@@ -446,27 +457,24 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int from_k = k + u * 4 * kPiece, some = depth - from_k;
-            if (kTf32) {
-                const float *from = static_cast<const float *>(at) + from_k;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (whole || some >= 4 * i + 4) {
-                        v = reinterpret_cast<const float4 *>(from)[i];
-                    } else if (some > 4 * i) {
-                        v.x = from[4 * i];
-                        v.y = some > 4 * i + 1 ? from[4 * i + 1] : 0.0f;
-                        v.z = some > 4 * i + 2 ? from[4 * i + 2] : 0.0f;
+            for (int plane = 0; plane < kPlanes; ++plane) {
+                if (kTf32) {
+                    const float *from = static_cast<const float *>(at) + from_k + plane * 4;
+                    if (whole) {
+                        b.q[u][plane][0] = *reinterpret_cast<const uint4 *>(from);
+                    } else {
+                        b.q[u][plane][0] = load_some(from, some - plane * 4);
                     }
-                    b.q[u][i][0] = *reinterpret_cast<const uint4 *>(&v);
-                }
-            } else {
-#pragma unroll
-                for (int plane = 0; plane < kPlanes; ++plane) {
+                } else {
                     const unsigned short *from = static_cast<const unsigned short *>(at) + plane * plane_step + from_k;
 #pragma unroll
                     for (int i = 0; i < kLoads; ++i) {
-                        b.q[u][plane][i] = whole ? reinterpret_cast<const uint4 *>(from)[i] : load_8(from + i * 8, some - i * 8, vector);
+                        if (whole) {
+                            b.q[u][plane][i] = reinterpret_cast<const uint4 *>(from)[i];
+                        } else {
+                            b.q[u][plane][i] = load_some(from + i * 8, some - i * 8);
+                        }
                     }
                 }
             }
@@ -494,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
             soon_left = soon.steps;
             soon_step = soon.step;
             const int first = lists.first[soon.rank];
-            soon_row = token_row(first + (g < lists.count[soon.rank] ? g : 0));
+            soon_row = token_row(first + min(g, lists.count[soon.rank] - 1));
             if (kW == kE4m3) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {  // rows g + 8 i, or g and g of the up, then 8 on
@@ -521,12 +529,14 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     const int other = (g & 4) != 0 ? -64 : 64;
     int stage = 0, turn = 0;
     uint32_t parity = 0;
-    float c[kTokens][2][4];
 
-    auto multiply = [&](const Place &now) {
-        const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
+    // a piece for experts of up to 8 kN tokens: sums in c
+    auto multiply = [&](const Place &now, auto &c) {
+        constexpr int kN = sizeof(c) / 32;
+        constexpr bool kAhead = kW == kE4m3 && kN > 1;  // widened once for all tokens
+        const int first = lists.first[now.rank], count = lists.count[now.rank];
 #pragma unroll
-        for (int n = 0; n < kTokens; ++n) {
+        for (int n = 0; n < kN; ++n) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 c[n][m][0] = c[n][m][1] = c[n][m][2] = c[n][m][3] = 0.0f;
@@ -535,15 +545,6 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
         int step = now.step;
 #pragma unroll 1
         for (int s = 0; s < now.steps; ++s, step += now.stride) {
-            Tokens b = next;
-            float of_block[4];
-            if (kW == kE4m3) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    of_block[i] = next_scale[i];
-                }
-            }
-            fetch();
             gave_up = gave_up || !mbar_wait(full + stage, parity, abort_flag, &experts_status, kDown ? 2 : 1, waits.limit);
             uint4 a[2][4];  // [which 64 bytes][row g + 8 i of the tile's 32]
 #pragma unroll
@@ -552,83 +553,125 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 a[0][r] = *reinterpret_cast<const uint4 *>(at);
                 a[1][r] = *reinterpret_cast<const uint4 *>(at + other);
             }
-            const bool whole = (step + 1) * kStep <= depth;
             __syncwarp();
             issue();  // into the stage that has just been read
-#pragma unroll
-            for (int n = 0; n < kTokens; ++n) {
-                if (n < eights) {
-                    if (n > 0) {
-                        load_tokens(b, token_row(first + (n * 8 + g < count ? n * 8 + g : 0)), step * kStep + t * kPiece, vector && whole);
-                    }
-                    // two chains of sums in turn: the matrix instructions of one wait for one another
-                    float part[2][4];
-                    if (kW == kE4m3) {
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            part[m][0] = part[m][1] = part[m][2] = part[m][3] = 0.0f;
-                        }
-                    }
-                    float(&to)[2][4] = kW == kE4m3 ? part : c[n];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        if (kTf32) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint4 &q = b.q[u][j / 2][0];
-                                const float2 b0 = split_tf32(__uint_as_float(word(q, j % 2 * 2)));
-                                const float2 b1 = split_tf32(__uint_as_float(word(q, j % 2 * 2 + 1)));
-                                float2 f[4];
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const uint32_t w = word(a[u][r], j);
-                                    f[r] = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-                                }
-                                mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.y, b1.y);
-                                mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.y, b1.y);
-                                mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.x, b1.x);
-                                mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.x, b1.x);
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 2 * kLoads; ++j) {
-                                uint32_t w[2][4];
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    if (kW == kE4m3) {
-                                        w[r / 2][r % 2] = widen_e4m3<kBfMma>(word(a[u][r], j), false);
-                                        w[r / 2][2 + r % 2] = widen_e4m3<kBfMma>(word(a[u][r], j), true);
-                                    } else {
-                                        w[r / 2][r % 2] = word(a[u][r], 2 * j);
-                                        w[r / 2][2 + r % 2] = word(a[u][r], 2 * j + 1);
-                                    }
-                                }
-#pragma unroll
-                                for (int plane = kPlanes - 1; plane >= 0; --plane) {
-                                    const uint4 &q = b.q[u][plane][j / 2];
-#pragma unroll
-                                    for (int m = 0; m < 2; ++m) {
-                                        mma_16<kBfMma>(to[m], w[m][0], w[m][1], w[m][2], w[m][3], word(q, j % 2 * 2), word(q, j % 2 * 2 + 1));
-                                    }
-                                }
-                            }
-                        }
-                    }
-                    if (kW == kE4m3) {
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                c[n][m][i] = fmaf(part[m][i], of_block[2 * m + i / 2], c[n][m][i]);
-                            }
-                        }
-                    }
-                }
-            }
             if (++stage == kStages) {
                 stage = 0;
                 parity ^= 1u;
             }
+            uint32_t wide[kAhead ? 2 : 1][kAhead ? 4 : 1][kAhead ? 8 : 1];
+            if (kAhead) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            wide[kAhead ? u : 0][kAhead ? r : 0][kAhead ? j : 0] = widen_e4m3<kBfMma>(word(a[u][r], j / 2), j % 2 != 0);
+                        }
+                    }
+                }
+            }
+            float of_block[4];
+            if (kW == kE4m3) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    of_block[i] = next_scale[i];
+                }
+            }
+            // sums of the tokens `b`, in two chains in turn: the matrix instructions of one wait for one another
+            auto add = [&](float(&sum)[2][4], const Tokens &b) {
+                float part[2][4];
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    part[m][0] = part[m][1] = part[m][2] = part[m][3] = 0.0f;
+                }
+                float(&to)[2][4] = kW == kE4m3 ? part : sum;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (kTf32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 &q = b.q[u][kPlanes * (j / 2) / 2][0];
+                            const float2 b0 = split_tf32(__uint_as_float(word(q, j % 2 * 2)));
+                            const float2 b1 = split_tf32(__uint_as_float(word(q, j % 2 * 2 + 1)));
+                            float2 f[4];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const uint32_t w = word(a[u][r], j);
+                                f[r] = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+                            }
+                            mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.y, b1.y);
+                            mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.y, b1.y);
+                            mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.x, b1.x);
+                            mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.x, b1.x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2 * kLoads; ++j) {
+                            uint32_t w[2][4];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                if (kAhead) {
+                                    w[r / 2][r % 2] = wide[kAhead ? u : 0][kAhead ? r : 0][kAhead ? 2 * j : 0];
+                                    w[r / 2][2 + r % 2] = wide[kAhead ? u : 0][kAhead ? r : 0][kAhead ? 2 * j + 1 : 0];
+                                } else if (kW == kE4m3) {
+                                    w[r / 2][r % 2] = widen_e4m3<kBfMma>(word(a[u][r], j), false);
+                                    w[r / 2][2 + r % 2] = widen_e4m3<kBfMma>(word(a[u][r], j), true);
+                                } else {
+                                    w[r / 2][r % 2] = word(a[u][r], 2 * j);
+                                    w[r / 2][2 + r % 2] = word(a[u][r], 2 * j + 1);
+                                }
+                            }
+#pragma unroll
+                            for (int plane = kPlanes - 1; plane >= 0; --plane) {
+                                const uint4 &q = b.q[u][plane][j / 2];
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) {
+                                    mma_16<kBfMma>(to[m], w[m][0], w[m][1], w[m][2], w[m][3], word(q, j % 2 * 2), word(q, j % 2 * 2 + 1));
+                                }
+                            }
+                        }
+                    }
+                }
+                if (kW == kE4m3) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            sum[m][i] = fmaf(part[m][i], of_block[2 * m + i / 2], sum[m][i]);
+                        }
+                    }
+                }
+            };
+            add(c[0], next);
+            fetch();
+            if (kN > 1) {
+                const bool whole = vector && (step + 1) * kStep <= depth;
+#pragma unroll
+                for (int n = 1; n < kN; ++n) {
+                    Tokens b;
+                    load_tokens(b, token_row(first + min(n * 8 + g, count - 1)), step * kStep + t * kPiece, whole);
+                    add(c[n], b);
+                }
+            }
+        }
+    };
+    // piece by the number of its expert's tokens: every width has code of its own, so that none runs through what is left out
+    auto by_width = [&](const Place &now, auto &&piece) {
+        const int count = lists.count[now.rank];
+        if (kTokens == 1 || count <= 8) {
+            float c[1][2][4];
+            piece(c, count);
+        } else if (kTokens == 2 || count <= 16) {
+            float c[kTokens < 2 ? kTokens : 2][2][4];
+            piece(c, count);
+        } else if (kTokens == 4 || count <= 32) {
+            float c[kTokens < 4 ? kTokens : 4][2][4];
+            piece(c, count);
+        } else {
+            float c[kTokens][2][4];
+            piece(c, count);
         }
     };
 
@@ -648,11 +691,12 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
         };
         const int group_warps = lists.group_warps;
         while (now.next_up(lists)) {
-            multiply(now);
-            const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
+            const int first = lists.first[now.rank];
+            by_width(now, [&](auto &c, int count) {
+                constexpr int kN = sizeof(c) / 32;
+                multiply(now, c);
 #pragma unroll
-            for (int n = 0; n < kTokens; ++n) {
-                if (n < eights) {
+                for (int n = 0; n < kN; ++n) {
                     if (group_warps == 1) {
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
@@ -675,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                         const int group = warp / group_warps, threads = group_warps * 32;
                         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
                         const float *from = reinterpret_cast<const float *>(buffer + group * group_warps * 64);
-                        for (int i = tid % threads; i < 128; i += threads) {
+                        for (int i = tid & (threads - 1); i < 128; i += threads) {
                             const int m = i >> 6, of = i >> 1 & 31, j = i & 1;  // element j of lane `of`, and the one of the up's row
                             float gate = 0.0f, up = 0.0f;
                             for (int w = 0; w < group_warps; ++w) {
@@ -690,17 +734,18 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                         }
                     }
                 }
-            }
+            });
         }
     } else {
         float *mine = y_sums + warp * p.tokens * kRows;
-        while (now.next_rows(warp)) {
-            while (now.next_down(lists)) {
-                multiply(now);
-                const int first = lists.first[now.rank], count = lists.count[now.rank], eights = (count + 7) / 8;
+        while (now.next_rows()) {
+            while (now.next_down()) {
+                const int first = lists.first[now.rank];
+                by_width(now, [&](auto &c, int count) {
+                    constexpr int kN = sizeof(c) / 32;
+                    multiply(now, c);
 #pragma unroll
-                for (int n = 0; n < kTokens; ++n) {
-                    if (n < eights) {
+                    for (int n = 0; n < kN; ++n) {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const int column = n * 8 + 2 * t + j;
@@ -715,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                             }
                         }
                     }
-                }
+                });
                 __syncwarp();  // the next expert's columns may be other lanes' tokens
             }
             __syncthreads();
