@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) experts_any_down_kernel(const __grid_cons
 
 long long experts_workspace_bytes(long long tokens, long long top, long long ffn)
 {
-    return tokens * top * ((ffn + 63) / 64 * 64) * 4;
+    return tokens * top * ((ffn + 127) / 128 * 128) * 4;
 }
 
 cudaError_t launch_experts_any(const ExpertsParams &p, cudaStream_t stream)

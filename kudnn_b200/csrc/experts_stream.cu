@@ -1,22 +1,26 @@
 // The block of experts for few tokens in two kernels that stream the weights once (experts.cuh).
 //
 // What bounds it is reading the chosen experts' weights; everything here serves to keep as many bytes in flight as HBM wants, without pauses:
-//   * Both products are cut by weight rows alone: the rows (gate and up rows in pairs) of all chosen experts are dealt out evenly, one CTA per SM,
-//     so that every SM streams the same number of bytes; nothing is added up across CTAs, no atomics, and the same call gives the same bits.
-//   * The 8 warps of a CTA stream on their own, without barriers.  First kernel: as many groups of warps as the CTA has tiles of rows, up to 8;
-//     a group's warps split K and add up at the end of a tile (with a tile per warp, what large batches have, nothing is added up).  Second
-//     kernel: each warp an eighth of all steps of all experts at the CTA's rows, with sums of y of its own, added up at the end.
-//   * A step of a warp is 128 bytes of up to 32 rows: up to four TMA boxes of eight rows, into a ring of the warp's own, some steps ahead.  Rows and
-//     columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their products are dropped).  (Copies by every lane,
-//     cp.async or straight into registers, took three to five times the instructions of the products, and their latency bound the whole.)
+//   * Both products are cut by weight rows: the rows (gate and up rows in pairs) of all chosen experts are dealt out evenly, one CTA of eight warps
+//     per SM.  No atomics; sums are added in a fixed order, so that the same call gives the same bits.
+//   * The warps stream on their own.  First kernel: tiles of up to 16 pairs of rows go to warps, or to groups of warps that take turns along K
+//     and add up at the end of a tile (plan_tiles).  Second kernel: the CTA's rows times all experts' steps along K are dealt out to groups
+//     of warps; each warp keeps sums of y of its own, added up once at the end.  Where a CTA would have 16 rows or fewer, two CTAs of a cluster
+//     share twice as many, half of the steps each.
+//   * A step of a warp is 128 bytes of up to 32 rows, up to four TMA boxes of eight rows, and as much of the first eight tokens' rows, into a ring
+//     of the warp's own, some steps ahead.  Rows and columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their
+//     products are dropped).  Copies by every lane (cp.async) or loads into registers took three to five times the instructions of the
+//     products and were bound by their latency; tokens loaded one step ahead were bound by L2's latency.
 //   * 16 bytes per lane, as they lie in the ring, are operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on
-//     that of 8.  The tokens' fragments are read from L1 and L2 in the same permutation, one step ahead.
-//   * The second kernel starts its copies of `down` while the first one ends (its CTAs take the place of the first one's as those leave) and
-//     waits only before it reads h.
+//     that of 8, read in the same permutation.
+//   * For few tokens the CTAs take at most half of an SM's shared memory, so that the second kernel's are there while the first one runs: they make
+//     their lists, fill their rings, and wait only before they read h.
 // h is kept as the tensor cores take it without loss: two bf16 halves (of bf16 and e4m3 weights), or fp32 that the second kernel splits into two
 // tf32 halves (of fp16 weights: halves of fp16 would overflow beyond 65504 and lose small values).
 #include "experts.cuh"
 #include "sm100_ptx.cuh"
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <atomic>
@@ -25,9 +29,17 @@ namespace kb {
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMostPairs = kMostExpertTokens * kMostExpertTop;
+constexpr int kRows = 32;                  // of a tile of weights; a step has 128 bytes of each
+constexpr int kMostTilePairs = kRows / 2;  // of a gate's and an up's row
+constexpr int kBoxRows = 8;
+constexpr int kBoxBytes = kBoxRows * 128;
+constexpr int kStageBytes = kRows * 128;
+constexpr int kMostStages = 8;
+constexpr int kPad = 128;  // h's rows are multiples of this many elements, zeros behind the last one
 
 enum Weights { kBf16, kF16, kE4m3 };
 
@@ -36,29 +48,55 @@ __device__ DeviceStatus experts_status;
 
 struct Waits {
     long long limit;  // in cycles
-    int skip_step;    // test hook: from which step of K on nothing is copied, -1 off
+    int skip_step;    // test hook: from which step of K on no weights are copied, -1 off
 };
 std::atomic<long long> wait_limit{0};
 std::atomic<int> wait_skip{-1};
 
+// Shared memory of a launch: [ring of weights][ring of tokens][sums][lists]
+struct Shape {
+    int stages;
+    int token_rows;   // of a stage: as many as an expert has, at most eight
+    int token_bytes;  // of a stage
+    int cluster;      // CTAs that share rows of y
+};
 
 // Which tokens the experts have: pairs in order of experts and tokens.
 struct Lists {
-    unsigned long long tokens[kMostExperts];  // bit t: token t is the expert's
-    short start[kMostExperts];                // of its pairs
-    short expert[kMostExperts];               // the active experts; what follows is by their rank
-    short first[kMostExperts];
-    short count[kMostExperts];
-    unsigned char token[kMostPairs];
-    float p[kMostPairs];
-    int ids[kMostPairs];  // as given, and the weights
-    float given[kMostPairs];
-    int active;
-    // first kernel: how many warps share a tile, how many tiles an expert's rows are cut into
-    // of at least tile_pairs pairs of rows, the first `longer` of one more
-    int group_warps, tiles, tile_pairs, longer;
-    int abort;  // some wait of the CTA gave up
-    unsigned long long full[kWarps][8];
+    unsigned long long *tokens;  // of each expert; bit t: token t is the expert's
+    short *start;                // of its pairs
+    short *expert;               // the active experts; what follows is by their rank
+    short *first;
+    short *count;
+    unsigned char *token;        // of each pair
+    float *p;
+    int *ids;                    // as given, and the weights
+    float *given;
+    // first kernel: how many warps share a tile, how many tiles an expert's rows are cut into, of at least tile_pairs pairs of rows, the first
+    // `longer` of one more
+    int &active, &group_warps, &tiles, &tile_pairs, &longer;
+    static constexpr int kCounts = 32;
+    static __host__ __device__ __forceinline__ int bytes(int experts, int pairs)
+    {
+        return kCounts + experts * 16 + (pairs * 13 + 15) / 16 * 16;
+    }
+    __device__ __forceinline__ Lists(unsigned char *at, int experts, int pairs)
+        : tokens(reinterpret_cast<unsigned long long *>(at + kCounts)),
+          start(reinterpret_cast<short *>(at + kCounts + experts * 8)),
+          expert(start + experts),
+          first(expert + experts),
+          count(first + experts),
+          token(at + kCounts + experts * 16 + pairs * 12),
+          p(reinterpret_cast<float *>(at + kCounts + experts * 16)),
+          ids(reinterpret_cast<int *>(p + pairs)),
+          given(p + 2 * pairs),
+          active(reinterpret_cast<int *>(at)[0]),
+          group_warps(reinterpret_cast<int *>(at)[1]),
+          tiles(reinterpret_cast<int *>(at)[2]),
+          tile_pairs(reinterpret_cast<int *>(at)[3]),
+          longer(reinterpret_cast<int *>(at)[4])
+    {
+    }
 };
 
 template <bool kBf>
@@ -102,6 +140,14 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t w, bool upper)
     return *reinterpret_cast<const uint32_t *>(&b);
 }
 
+// 16 bytes multiples from global to shared memory, on 16-byte boundaries both
+__device__ __forceinline__ void bulk_copy(void *to, const void *from, int bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // The first `left` of 8 values of 16 bits (a loop: it is seldom run, and must not become instructions of the path beside it)
 __device__ __forceinline__ uint4 load_some(const unsigned short *at, int left)
 {
@@ -110,17 +156,6 @@ __device__ __forceinline__ uint4 load_some(const unsigned short *at, int left)
     for (int i = min(left, 8) - 1; i >= 0; --i) {
         hi = hi << 16 | lo >> 48;
         lo = lo << 16 | at[i];
-    }
-    return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
-}
-// The first `left` of 4 values of fp32
-__device__ __forceinline__ uint4 load_some(const float *at, int left)
-{
-    unsigned long long lo = 0ull, hi = 0ull;
-#pragma unroll 1
-    for (int i = min(left, 4) - 1; i >= 0; --i) {
-        hi = hi << 32 | lo >> 32;
-        lo = lo << 32 | __float_as_uint(at[i]);
     }
     return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
 }
@@ -133,27 +168,10 @@ __device__ __forceinline__ float2 split_tf32(float v)
 }
 
 // h in the workspace, a row per pair in the lists' order: bf16 upper halves, then lower ones, or fp32.
-__device__ __forceinline__ long long h_pitch(const ExpertsParams &p)
+__host__ __device__ __forceinline__ long long h_pitch(int ffn)
 {
-    return (p.ffn + 63) / 64 * 64;
+    return static_cast<long long>((ffn + kPad - 1) / kPad) * kPad;
 }
-
-// A tile has 32 rows of weights, a step 128 bytes of each.
-constexpr int kRows = 32;
-constexpr int kMostTilePairs = kRows / 2;  // of a gate's and an up's row
-constexpr int kBoxRows = 8;
-constexpr int kBoxBytes = kBoxRows * 128;
-constexpr int kStageBytes = kRows * 128;
-
-// The kernels for experts of up to 8 kTokens tokens: the ring, and behind it the warps' sums.
-template <bool kDown, int kTokens>
-struct Layout {
-    static constexpr int kStages = kTokens == 8 && kDown ? 4 : 5;
-    static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-    // up: the sums of 8 tokens of every warp, in two buffers; down: each warp's sums of y
-    static constexpr int kSumBytes = kDown ? kWarps * 8 * kTokens * kRows * 4 : 2 * kWarps * 1024;
-    static constexpr size_t kBytes = kRingBytes + kSumBytes + sizeof(Lists) + 1024;  // the ring begins on a multiple of 1024
-};
 
 // A warp's way through the weights, piece by piece: steps of K of a tile of one expert's rows.  32 bits hold every count (see the launcher).
 template <bool kDown>
@@ -188,16 +206,17 @@ struct Cursor {
         return true;
     }
     // Down: the steps of all experts at the same rows go to groups of warps, as many to each, and a group's warps take turns, so that they read
-    // what lies side by side; groups of as many warps as leave each eight steps of an expert.
-    __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int warp, int depth_steps)
+    // what lies side by side; groups of as many warps as leave each four steps of an expert.
+    __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int warp, int depth_steps, int cluster)
     {
-        at = static_cast<int>(static_cast<unsigned>(p.hidden) * blockIdx.x / gridDim.x);
-        end = static_cast<int>(static_cast<unsigned>(p.hidden) * (blockIdx.x + 1) / gridDim.x);
+        const unsigned shares = gridDim.x / cluster, share = blockIdx.x / cluster;
+        at = static_cast<int>(static_cast<unsigned>(p.hidden) * share / shares);
+        end = static_cast<int>(static_cast<unsigned>(p.hidden) * (share + 1) / shares);
         depth = depth_steps;
-        stride = depth >= 64 ? 8 : depth >= 32 ? 4 : depth >= 16 ? 2 : 1;
-        const int groups = kWarps / stride, group = warp / stride, all = l.active * depth;
-        begin = all * group / groups;
-        until = all * (group + 1) / groups;
+        stride = depth >= 32 ? 8 : depth >= 16 ? 4 : depth >= 8 ? 2 : 1;
+        const int per_cta = kWarps / stride, groups = per_cta * cluster, group = blockIdx.x % cluster * per_cta + warp / stride, all = l.active * depth;
+        begin = all / groups * group + min(group, all % groups);
+        until = begin + all / groups + (group < all % groups ? 1 : 0);
         begin_rank = begin / depth;
         offset = warp & (stride - 1);
         rows = 0;
@@ -326,46 +345,56 @@ __device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p, int
     __syncthreads();
 }
 
-// kTokens: an expert's most, in eights.
+// kTokens: an expert's most, in eights.  One of eight (and fewer) leaves room for a second CTA per SM.
 template <Weights kW, bool kBf, bool kDown, int kTokens>
-__global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __grid_constant__ ExpertsParams p, const __grid_constant__ CUtensorMap map,
-                                                                     const __grid_constant__ Waits waits)
+__global__ void __launch_bounds__(kThreads, kTokens == 1 ? 2 : 1)
+    experts_stream_kernel(const __grid_constant__ ExpertsParams p, const __grid_constant__ CUtensorMap map, const __grid_constant__ Shape shape,
+                          const __grid_constant__ Waits waits)
 {
-    using L = Layout<kDown, kTokens>;
-    constexpr int kStages = L::kStages;
     constexpr int kElem = kW == kE4m3 ? 1 : 2;
     constexpr int kStep = 128 / kElem;                // of K
     constexpr int kPiece = 16 / kElem;                // of a lane, twice in a step
     constexpr bool kTf32 = kDown && kW == kF16;       // h in fp32, products of tf32
     constexpr bool kBfMma = kW == kBf16 || (kW == kE4m3 && (kBf || kDown));
-    constexpr int kPlanes = kDown ? 2 : 1, kLoads = kPiece / 8;
+    constexpr int kPlanes = kDown && !kTf32 ? 2 : 1;  // of the tokens' rows
+    constexpr int kTokenElem = kTf32 ? 4 : 2;
+    constexpr int kTokenRow = kStep * kTokenElem;     // bytes of a token's row in a step
+    constexpr int kTokenPitch = kTokenRow + 64;       // so that two rows' fragments lie in different banks
+    constexpr int kLoads = kPiece * kTokenElem / 16;  // 16-byte pieces of a lane's fragment
     extern __shared__ unsigned char raw[];
+    __shared__ uint64_t barriers[kWarps][kMostStages];
+    __shared__ int abort_word;
     unsigned char *shared = raw + (1024u - (smem_u32(raw) & 1023u)) % 1024u;
     const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    unsigned char *ring = shared + warp * kStages * kStageBytes;
-    float4 *sums = reinterpret_cast<float4 *>(shared + L::kRingBytes);  // up: [2][kWarps][2][32]
-    float *y_sums = reinterpret_cast<float *>(shared + L::kRingBytes);  // down: [kWarps][tokens][kRows]
-    Lists &lists = *reinterpret_cast<Lists *>(shared + L::kRingBytes + L::kSumBytes);
+    const int stages = shape.stages;
+    unsigned char *ring = shared + warp * stages * kStageBytes;
+    unsigned char *token_ring = shared + kWarps * stages * kStageBytes + warp * stages * shape.token_bytes;
+    unsigned char *behind = shared + kWarps * stages * (kStageBytes + shape.token_bytes);
+    float4 *sums = reinterpret_cast<float4 *>(behind);  // up: [kWarps][2][32]
+    float *y_sums = reinterpret_cast<float *>(behind);  // down: [kWarps][tokens][kRows]
+    Lists lists(behind + (kDown ? kWarps * p.tokens * kRows * 4 : kWarps * 1024), p.experts, p.tokens * p.top);
     const int depth = kDown ? p.ffn : p.hidden;  // K
-    uint64_t *full = reinterpret_cast<uint64_t *>(lists.full[warp]);  // a barrier per stage of the warp's ring
-    volatile int *abort_flag = &lists.abort;
+    const int depth_steps = (depth + kStep - 1) / kStep;
+    uint64_t *full = barriers[warp];  // a barrier per stage of the warp's ring
+    volatile int *abort_flag = &abort_word;
     if (tid == 0) {
-        lists.abort = 0;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+        abort_word = 0;
     }
-    if (lane < kStages) {
+    if (lane < stages) {
         mbar_init(full + lane, 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-
-    if (warp == 0 && lane == 0) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
-    }
     for (int e = tid; e < p.experts; e += kThreads) {
         lists.tokens[e] = 0ull;
     }
+    if (kDown) {
+        for (int i = tid; i < kWarps * p.tokens * kRows; i += kThreads) {
+            y_sums[i] = 0.0f;
+        }
+    }
     __syncthreads();
-    const int depth_steps = (depth + kStep - 1) / kStep;
     if (!kDown) {
         pdl_wait();
         pdl_launch_dependents();  // behind the wait: what the second kernel reads ahead of its own is older than this one
@@ -374,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     using Place = Cursor<kDown>;
     auto start = [&](Place &c) {
         if (kDown) {
-            c.start_down(p, lists, warp, depth_steps);
+            c.start_down(p, lists, warp, depth_steps, shape.cluster);
         } else {
             c.start_up(lists, warp, depth_steps);
         }
@@ -395,8 +424,23 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
         return true;
     };
 
-    // ---- the stream: lane i < 4 brings eight rows (up: of the gate, of the up, and the next eight of both)
-    int box_row = 0, boxes = 0;
+    // ---- the stream: lane i < 4 brings eight rows of weights (up: of the gate, of the up, and the next eight of both), lane 8 + 8 plane + i the
+    // row of an expert's i-th token, where those lie on 16-byte boundaries
+    const long long pitch = h_pitch(p.ffn);
+    const long long plane_step = static_cast<long long>(p.tokens) * p.top * pitch;
+    const bool staged = kDown || ((reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && p.x_ld % 8 == 0);
+    // the row of x or h of a pair, in bytes
+    auto token_row = [&](int pair, int plane) -> const unsigned char * {
+        if (kDown) {
+            return static_cast<const unsigned char *>(p.h) + (pair * pitch + plane * plane_step) * kTokenElem;
+        }
+        return static_cast<const unsigned char *>(p.x) + lists.token[pair] * p.x_ld * kTokenElem;
+    };
+    const int copy_plane = (lane - 8) >> 3, copy_row = lane & 7;
+    unsigned char *const copy_to = token_ring + (copy_plane * shape.token_rows + copy_row) * kTokenPitch;
+    const unsigned char *copy_from = nullptr;
+    bool copies = false;
+    int box_row = 0, boxes = 0, token_copies = 0;
     int ahead_k = 0, ahead_left = 0, ahead_stage = 0, ahead_expert = 0;
     Place ahead;
     start(ahead);
@@ -408,126 +452,117 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
             ahead_expert = lists.expert[ahead.rank];
             boxes = kDown ? (ahead.rows + 7) / 8 : ahead.rows > 8 ? 4 : 2;
             box_row = ahead.row + (kDown ? lane * 8 : (lane >> 1) * 8 + (lane & 1) * p.ffn);
+            const int rows = min(static_cast<int>(lists.count[ahead.rank]), 8);
+            token_copies = staged ? rows * kPlanes : 0;
+            copies = staged && lane >= 8 && copy_plane < kPlanes && copy_row < rows;
+            copy_from = token_row(lists.first[ahead.rank] + min(copy_row, rows - 1), copies ? copy_plane : 0);
         }
     };
     aim();
     bool gave_up = false;
+    // weights: those of the step; tokens: theirs
+    auto copy_weights = [&](int stage, int k) {
+        if (lane < boxes && (waits.skip_step < 0 || k / kStep < waits.skip_step)) {
+            tma_load_3d(ring + stage * kStageBytes + lane * kBoxBytes, &map, full + stage, k, box_row, ahead_expert);
+        }
+    };
+    auto copy_tokens = [&](int stage, int k, int bytes) {
+        if (copies) {
+            bulk_copy(copy_to + stage * shape.token_bytes, copy_from + static_cast<long long>(k) * kTokenElem, bytes, full + stage);
+        }
+    };
+    // h's rows are whole; x's last step ends at the last 16 bytes that hold elements
+    auto token_bytes = [&](int k) { return kDown ? kTokenRow : min(kTokenRow, (depth - k + 7) / 8 * 16); };
     auto issue = [&]() {
         if (ahead_left > 0) {
-            if (lane < boxes && !gave_up) {
+            const int bytes = token_bytes(ahead_k);
+            if (!gave_up) {
                 if (lane == 0) {
-                    mbar_expect_tx(full + ahead_stage, boxes * kBoxBytes);
+                    mbar_expect_tx(full + ahead_stage, boxes * kBoxBytes + token_copies * bytes);
                 }
-                if (waits.skip_step < 0 || ahead_k / kStep < waits.skip_step) {
-                    tma_load_3d(ring + ahead_stage * kStageBytes + lane * kBoxBytes, &map, full + ahead_stage, ahead_k, box_row, ahead_expert);
-                }
+                copy_weights(ahead_stage, ahead_k);
+                copy_tokens(ahead_stage, ahead_k, bytes);
             }
+            ahead_k += ahead.stride * kStep;
+            ahead_stage = ahead_stage + 1 == stages ? 0 : ahead_stage + 1;
+            if (--ahead_left == 0) {
+                aim();
+            }
+        }
+    };
+    if (kDown) {
+        // the first round's weights, ahead of the wait for h, whose rows follow
+        const Place from = ahead;
+        const int from_k = ahead_k, from_left = ahead_left, from_expert = ahead_expert, from_boxes = boxes, from_row = box_row, from_copies = token_copies;
+        const unsigned char *from_copy = copy_from;
+        const bool from_any = copies;
+#pragma unroll 1
+        for (int i = 0; i < stages && ahead_left > 0; ++i) {
+            if (lane == 0) {
+                mbar_expect_tx(full + i, boxes * kBoxBytes + token_copies * kTokenRow);
+            }
+            copy_weights(i, ahead_k);
             ahead_k += ahead.stride * kStep;
             if (--ahead_left == 0) {
                 aim();
             }
-            ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
-        }
-    };
-#pragma unroll 1
-    for (int i = 0; i < kStages; ++i) {
-        issue();
-    }
-    if (kDown) {
-        for (int i = tid; i < kWarps * p.tokens * kRows; i += kThreads) {
-            y_sums[i] = 0.0f;
         }
         pdl_wait();
         pdl_launch_dependents();
-        __syncthreads();
+        ahead = from;
+        ahead_k = from_k;
+        ahead_left = from_left;
+        ahead_expert = from_expert;
+        boxes = from_boxes;
+        box_row = from_row;
+        token_copies = from_copies;
+        copy_from = from_copy;
+        copies = from_any;
+#pragma unroll 1
+        for (int i = 0; i < stages && ahead_left > 0; ++i) {
+            copy_tokens(i, ahead_k, kTokenRow);
+            ahead_k += ahead.stride * kStep;
+            ahead_stage = ahead_stage + 1 == stages ? 0 : ahead_stage + 1;
+            if (--ahead_left == 0) {
+                aim();
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < stages; ++i) {
+            issue();
+        }
     }
 
-    // ---- the tokens' fragments of a step, and its scales: the first eight tokens' are fetched one step ahead
-    const long long pitch = h_pitch(p);
-    const long long plane_step = static_cast<long long>(p.tokens) * p.top * pitch;
-    const bool vector = kDown || ((reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && p.x_ld % 8 == 0);
-    const float *scale = kDown ? p.down_scale : p.gate_up_scale;
-    const long long ss_e = kDown ? p.ds_se : p.gus_se, ss_n = kDown ? p.ds_sn : p.gus_sn, ss_k = kDown ? p.ds_sk : p.gus_sk;
+    // ---- the products
     struct Tokens {
-        uint4 q[2][kPlanes][kLoads];  // [which 64 bytes of weights]; kTf32: [..][which four][0]
+        uint4 q[2][kPlanes][kLoads];  // [which 64 bytes of weights]
     };
-    // at: the row of x or h of this lane's token (of lanes without one: of any, their sums are dropped); from element k on; whole: all of the
-    // step's elements exist, on 16-byte boundaries
-    auto load_tokens = [&](Tokens &b, const void *at, int k, bool whole) {
+    // the fragments of tokens that do not come through the ring; whole: all of the step's elements exist, on 16-byte boundaries
+    auto load_tokens = [&](Tokens &b, int pair, int k, bool whole) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int from_k = k + u * 4 * kPiece, some = depth - from_k;
+            const int from_k = k + u * 4 * kPiece;
 #pragma unroll
             for (int plane = 0; plane < kPlanes; ++plane) {
-                if (kTf32) {
-                    const float *from = static_cast<const float *>(at) + from_k + plane * 4;
-                    if (whole) {
-                        b.q[u][plane][0] = *reinterpret_cast<const uint4 *>(from);
+                const unsigned char *from = token_row(pair, plane) + static_cast<long long>(from_k) * kTokenElem;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    if (kDown || whole) {
+                        b.q[u][plane][i] = reinterpret_cast<const uint4 *>(from)[i];
                     } else {
-                        b.q[u][plane][0] = load_some(from, some - plane * 4);
-                    }
-                } else {
-                    const unsigned short *from = static_cast<const unsigned short *>(at) + plane * plane_step + from_k;
-#pragma unroll
-                    for (int i = 0; i < kLoads; ++i) {
-                        if (whole) {
-                            b.q[u][plane][i] = reinterpret_cast<const uint4 *>(from)[i];
-                        } else {
-                            b.q[u][plane][i] = load_some(from + i * 8, some - i * 8);
-                        }
+                        b.q[u][plane][i] = load_some(reinterpret_cast<const unsigned short *>(from) + i * 8, depth - from_k - i * 8);
                     }
                 }
             }
         }
     };
-    auto token_row = [&](int pair) -> const void * {
-        if (kTf32) {
-            return static_cast<const float *>(p.h) + pair * pitch;
-        }
-        return kDown ? static_cast<const unsigned short *>(p.h) + pair * pitch
-                     : static_cast<const unsigned short *>(p.x) + lists.token[pair] * p.x_ld;
-    };
-    Tokens next;
-    float next_scale[4];
-    Place soon;
-    start(soon);
-    int soon_left = 0, soon_step = 0;
-    const void *soon_row = nullptr;
-    const float *soon_scale[4];
-    auto fetch = [&]() {
-        if (soon_left == 0) {
-            if (!advance(soon)) {
-                return;
-            }
-            soon_left = soon.steps;
-            soon_step = soon.step;
-            const int first = lists.first[soon.rank];
-            soon_row = token_row(first + min(g, lists.count[soon.rank] - 1));
-            if (kW == kE4m3) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {  // rows g + 8 i, or g and g of the up, then 8 on
-                    const int r = min(kDown ? i * 8 + g : (i >> 1) * 8 + g, soon.rows - 1);
-                    soon_scale[i] = scale + lists.expert[soon.rank] * ss_e + (soon.row + r + (!kDown && (i & 1) != 0 ? p.ffn : 0)) / 128 * ss_n;
-                }
-            }
-        }
-        load_tokens(next, soon_row, soon_step * kStep + t * kPiece, vector && (soon_step + 1) * kStep <= depth);
-        if (kW == kE4m3) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                next_scale[i] = soon_scale[i][soon_step * ss_k];
-            }
-        }
-        soon_step += soon.stride;
-        --soon_left;
-    };
-    fetch();
-
-    // ---- the products
+    const float *scale = kDown ? p.down_scale : p.gate_up_scale;
+    const long long ss_e = kDown ? p.ds_se : p.gus_se, ss_n = kDown ? p.ds_sn : p.gus_sn, ss_k = kDown ? p.ds_sk : p.gus_sk;
     // where this lane's fragments of row g lie: chunks t and t + 4, which the copies put in place t ^ g and so on
     const unsigned char *fragment = ring + g * 128 + (t ^ g) * 16;
     const int other = (g & 4) != 0 ? -64 : 64;
-    int stage = 0, turn = 0;
+    int stage = 0;
     uint32_t parity = 0;
 
     // a piece for experts of up to 8 kN tokens: sums in c
@@ -542,10 +577,40 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 c[n][m][0] = c[n][m][1] = c[n][m][2] = c[n][m][3] = 0.0f;
             }
         }
+        const float *scale_at[4];
+        if (kW == kE4m3) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // rows g + 8 i, or g and g of the up, then 8 on
+                const int r = min(kDown ? i * 8 + g : (i >> 1) * 8 + g, now.rows - 1);
+                scale_at[i] = scale + lists.expert[now.rank] * ss_e + (now.row + r + (!kDown && (i & 1) != 0 ? p.ffn : 0)) / 128 * ss_n;
+            }
+        }
+        const unsigned char *token_fragment = token_ring + min(g, count - 1) * kTokenPitch + t * 16 * kLoads;
         int step = now.step;
 #pragma unroll 1
         for (int s = 0; s < now.steps; ++s, step += now.stride) {
+            float of_block[4];
+            if (kW == kE4m3) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    of_block[i] = scale_at[i][step * ss_k];
+                }
+            }
             gave_up = gave_up || !mbar_wait(full + stage, parity, abort_flag, &experts_status, kDown ? 2 : 1, waits.limit);
+            const int k = step * kStep + t * kPiece;
+            const bool whole = kDown || (staged && (step + 1) * kStep <= depth);
+            if (!kDown && staged && !whole) {
+                // x's last step: zeros behind the last element, where the copy brought what follows or nothing
+                const int left = depth - step * kStep;
+#pragma unroll 1
+                for (int i = lane; i < min(count, 8) * kStep; i += 32) {
+                    if (i % kStep >= left) {
+                        reinterpret_cast<unsigned short *>(token_ring + stage * shape.token_bytes + i / kStep * kTokenPitch)[i % kStep] = 0;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
             uint4 a[2][4];  // [which 64 bytes][row g + 8 i of the tile's 32]
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -553,9 +618,26 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 a[0][r] = *reinterpret_cast<const uint4 *>(at);
                 a[1][r] = *reinterpret_cast<const uint4 *>(at + other);
             }
+            Tokens b0;
+            if (staged) {
+                const unsigned char *at = token_fragment + stage * shape.token_bytes;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int plane = 0; plane < kPlanes; ++plane) {
+#pragma unroll
+                        for (int i = 0; i < kLoads; ++i) {
+                            b0.q[u][plane][i] =
+                                reinterpret_cast<const uint4 *>(at + plane * shape.token_rows * kTokenPitch + u * 64 * kLoads)[i];
+                        }
+                    }
+                }
+            } else {
+                load_tokens(b0, first + min(g, count - 1), k, false);
+            }
             __syncwarp();
             issue();  // into the stage that has just been read
-            if (++stage == kStages) {
+            if (++stage == stages) {
                 stage = 0;
                 parity ^= 1u;
             }
@@ -572,13 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                     }
                 }
             }
-            float of_block[4];
-            if (kW == kE4m3) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    of_block[i] = next_scale[i];
-                }
-            }
             // sums of the tokens `b`, in two chains in turn: the matrix instructions of one wait for one another
             auto add = [&](float(&sum)[2][4], const Tokens &b) {
                 float part[2][4];
@@ -592,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                     if (kTf32) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const uint4 &q = b.q[u][kPlanes * (j / 2) / 2][0];
+                            const uint4 &q = b.q[u][0][j / 2 % kLoads];
                             const float2 b0 = split_tf32(__uint_as_float(word(q, j % 2 * 2)));
                             const float2 b1 = split_tf32(__uint_as_float(word(q, j % 2 * 2 + 1)));
                             float2 f[4];
@@ -644,16 +719,12 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                     }
                 }
             };
-            add(c[0], next);
-            fetch();
-            if (kN > 1) {
-                const bool whole = vector && (step + 1) * kStep <= depth;
+            add(c[0], b0);
 #pragma unroll
-                for (int n = 1; n < kN; ++n) {
-                    Tokens b;
-                    load_tokens(b, token_row(first + min(n * 8 + g, count - 1)), step * kStep + t * kPiece, whole);
-                    add(c[n], b);
-                }
+            for (int n = 1; n < kN; ++n) {
+                Tokens b;
+                load_tokens(b, first + min(n * 8 + g, count - 1), k, whole);
+                add(c[n], b);
             }
         }
     };
@@ -678,8 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
     Place now;
     start(now);
     if (!kDown) {
-        auto store_h = [&](long long to, float gate, float up) {
-            const float v = expert_gate(gate, up);
+        auto put = [&](long long to, float v) {
             if (kW == kF16) {
                 static_cast<float *>(p.h)[to] = v;
             } else {
@@ -704,21 +774,19 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                             for (int j = 0; j < 2; ++j) {
                                 const int r = m * 8 + g, column = n * 8 + 2 * t + j;
                                 if (r < now.rows && column < count) {
-                                    store_h((first + column) * pitch + now.row + r, c[n][m][j], c[n][m][2 + j]);
+                                    put((first + column) * pitch + now.row + r, expert_gate(c[n][m][j], c[n][m][2 + j]));
                                 }
                             }
                         }
                     } else {
-                        // the group's sums, eight tokens at a time; two buffers take turns, so that one barrier does
-                        float4 *buffer = sums + turn * kWarps * 64;
-                        turn ^= 1;
+                        // the group's sums, eight tokens at a time
+                        const int group = warp / group_warps, threads = group_warps * 32;
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
-                            buffer[warp * 64 + m * 32 + lane] = make_float4(c[n][m][0], c[n][m][1], c[n][m][2], c[n][m][3]);
+                            sums[warp * 64 + m * 32 + lane] = make_float4(c[n][m][0], c[n][m][1], c[n][m][2], c[n][m][3]);
                         }
-                        const int group = warp / group_warps, threads = group_warps * 32;
                         asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
-                        const float *from = reinterpret_cast<const float *>(buffer + group * group_warps * 64);
+                        const float *from = reinterpret_cast<const float *>(sums + group * group_warps * 64);
                         for (int i = tid & (threads - 1); i < 128; i += threads) {
                             const int m = i >> 6, of = i >> 1 & 31, j = i & 1;  // element j of lane `of`, and the one of the up's row
                             float gate = 0.0f, up = 0.0f;
@@ -729,14 +797,22 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                             }
                             const int r = m * 8 + (of >> 2), column = n * 8 + (of & 3) * 2 + j;
                             if (r < now.rows && column < count) {
-                                store_h((first + column) * pitch + now.row + r, gate, up);
+                                put((first + column) * pitch + now.row + r, expert_gate(gate, up));
                             }
                         }
+                        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
+                    }
+                }
+                if (now.row + now.rows == p.ffn && now.offset == 0) {
+                    const int some = static_cast<int>(pitch) - p.ffn;
+                    for (int i = lane; i < some * count; i += 32) {
+                        put((first + i / some) * pitch + p.ffn + i % some, 0.0f);
                     }
                 }
             });
         }
     } else {
+        cg::cluster_group cluster = cg::this_cluster();
         float *mine = y_sums + warp * p.tokens * kRows;
         while (now.next_rows()) {
             while (now.next_down()) {
@@ -763,46 +839,81 @@ __global__ void __launch_bounds__(kThreads, 1) experts_stream_kernel(const __gri
                 });
                 __syncwarp();  // the next expert's columns may be other lanes' tokens
             }
-            __syncthreads();
-            for (int i = tid; i < p.tokens * kRows; i += kThreads) {
+            if (shape.cluster > 1) {
+                cluster.sync();
+            } else {
+                __syncthreads();
+            }
+            // the CTAs of a cluster take turns at the results, all add in the same order
+            const int items = p.tokens * kRows;
+            for (int i = tid * shape.cluster + static_cast<int>(blockIdx.x) % shape.cluster; i < items; i += kThreads * shape.cluster) {
                 float y = 0.0f;
-                for (int w = 0; w < kWarps; ++w) {
-                    y += y_sums[w * p.tokens * kRows + i];
-                    y_sums[w * p.tokens * kRows + i] = 0.0f;
+                for (int cta = 0; cta < shape.cluster; ++cta) {
+                    const float *from = shape.cluster > 1 ? cluster.map_shared_rank(y_sums, cta) : y_sums;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        y += from[w * items + i];
+                    }
                 }
                 const int token = i / kRows, r = i % kRows;
                 if (r < now.rows) {
                     store_exact(p.y, p.x_dtype, token * p.y_ld + now.row + r, round_rne(y, p.x_dtype));
                 }
             }
-            __syncthreads();
+            if (shape.cluster > 1) {
+                cluster.sync();
+            } else {
+                __syncthreads();
+            }
+            if (now.row + now.rows < now.end) {
+                for (int i = tid; i < kWarps * items; i += kThreads) {
+                    y_sums[i] = 0.0f;
+                }
+                __syncthreads();
+            }
         }
     }
     if (gave_up) {
         // the copies that are still on their way, each for a moment
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < stages; ++i) {
             for (int spin = 0; spin < 100000 && !mbar_try_wait(full + i, parity ^ (i < stage ? 1u : 0u)); ++spin) {
             }
         }
     }
 }
 
+constexpr int kMostShared = 227 * 1024 - 1024;           // of a CTA, beside its static part
+constexpr int kHalfShared = (228 * 1024) / 2 - 2 * 1024;  // where two CTAs are to fit
+
 template <Weights kW, bool kBf, bool kDown, int kTokens>
 cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream)
 {
-    constexpr size_t kShared = Layout<kDown, kTokens>::kBytes;
-    static_assert(kShared <= 227 * 1024, "shared memory");
+    constexpr int kStep = kW == kE4m3 ? 128 : 64;
+    constexpr int kTokenPitch = kStep * (kDown && kW == kF16 ? 4 : 2) + 64;
+    Shape shape;
+    shape.token_rows = std::min(8, p.tokens);
+    shape.token_bytes = shape.token_rows * (kDown && kW != kF16 ? 2 : 1) * kTokenPitch;
+    shape.cluster = kDown && p.hidden <= 16 * sm_count ? 2 : 1;
+    const int fixed = 1024 + (kDown ? kWarps * p.tokens * kRows * 4 : kWarps * 1024) + Lists::bytes(p.experts, p.tokens * p.top);
+    const int stage = kWarps * (kStageBytes + shape.token_bytes);
+    // half of the SM, if that gives a ring of three stages and the registers suffice
+    shape.stages = kTokens == 1 ? (kHalfShared - fixed) / stage : 0;
+    if (shape.stages < 3) {
+        shape.stages = (kMostShared - fixed) / stage;
+    }
+    shape.stages = std::min(shape.stages, kMostStages);
+    const size_t shared = static_cast<size_t>(fixed) + static_cast<size_t>(shape.stages) * stage;
     alignas(64) CUtensorMap map;
     cudaError_t e = tc_encode_groups(&map, kDown ? p.down : p.gate_up, p.w_dtype, p.experts, kDown ? p.hidden : 2ll * p.ffn, kDown ? p.ffn : p.hidden,
                                      std::max(kDown ? p.d_se : p.gu_se, 16ll), kDown ? p.d_sn : p.gu_sn, kBoxRows);
     if (e == cudaSuccess) {
-        e = cudaFuncSetAttribute(experts_stream_kernel<kW, kBf, kDown, kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kShared));
+        e = cudaFuncSetAttribute(experts_stream_kernel<kW, kBf, kDown, kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     }
     const long long limit = wait_limit.load();
     const Waits waits = {limit > 0 ? limit : kDefaultWaitLimitCycles, wait_skip.load()};
-    return e != cudaSuccess
-               ? e
-               : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count), dim3(kThreads), kShared, stream, 1u, p, map, waits);
+    return e != cudaSuccess ? e
+                            : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count / shape.cluster * shape.cluster), dim3(kThreads),
+                                             shared, stream, shape.cluster, p, map, shape, waits);
 }
 
 template <Weights kW, bool kBf, int kTokens>
