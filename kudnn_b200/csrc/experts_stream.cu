@@ -1,11 +1,11 @@
 // The block of experts for few tokens in two kernels that stream the weights once (experts.cuh).
 //
 // What bounds it is reading the chosen experts' weights; everything here serves to keep as many bytes in flight as HBM wants, without pauses:
-//   * Both products are cut by weight rows: the rows (gate and up rows in pairs) of all chosen experts are dealt out evenly, one CTA of eight warps
-//     per SM.  No atomics; sums are added in a fixed order, so that the same call gives the same bits.
+//   * Both products are cut by weight rows: the rows (gate and up rows in pairs) of all chosen experts are dealt out evenly, one CTA of 8 to 16
+//     warps per SM.  No atomics; sums are added in a fixed order, so that the same call gives the same bits.
 //   * The warps stream on their own.  First kernel: tiles of up to 16 pairs of rows go to warps, or to groups of warps that take turns along K
-//     and add up at the end of a tile (plan_tiles).  Second kernel: the CTA's rows times all experts' steps along K are dealt out to groups
-//     of warps; each warp keeps sums of y of its own, added up once at the end.  Where a CTA would have 16 rows or fewer, two CTAs of a cluster
+//     and add up at the end of a tile (plan_tiles).  Second kernel: the CTA's rows times all experts' steps along K are dealt out to the
+//     warps; each keeps sums of y of its own, added up once at the end.  Where a CTA would have 16 rows or fewer, two CTAs of a cluster
 //     share twice as many, half of the steps each.
 //   * A step of a warp is 128 bytes of up to 32 rows, up to four TMA boxes of eight rows, and as much of the first eight tokens' rows, into a ring
 //     of the warp's own, some steps ahead.  Rows and columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their
@@ -13,7 +13,7 @@
 //     products and were bound by their latency; tokens loaded one step ahead were bound by L2's latency.
 //   * 16 bytes per lane, as they lie in the ring, are operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on
 //     that of 8, read in the same permutation.
-//   * For few tokens the CTAs take at most half of an SM's shared memory, so that the second kernel's are there while the first one runs: they make
+//   * For few tokens and 16-bit weights the CTAs take at most half of an SM's shared memory, so that the second kernel's are there while the first one runs: they make
 //     their lists, fill their rings, and wait only before they read h.
 // h is kept as the tensor cores take it without loss: two bf16 halves (of bf16 and e4m3 weights), or fp32 that the second kernel splits into two
 // tf32 halves (of fp16 weights: halves of fp16 would overflow beyond 65504 and lose small values).
@@ -31,8 +31,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kRows = 32;                  // of a tile of weights; a step has 128 bytes of each
 constexpr int kMostTilePairs = kRows / 2;  // of a gate's and an up's row
 constexpr int kBoxRows = 8;
@@ -42,6 +40,11 @@ constexpr int kMostStages = 8;
 constexpr int kPad = 128;  // h's rows are multiples of this many elements, zeros behind the last one
 
 enum Weights { kBf16, kF16, kE4m3 };
+
+// Warps of a CTA for experts of up to 8 kTokens tokens.  e4m3 weights take four instructions for every two to become bf16: with two warps per
+// scheduler their latency is the bound (16 tokens, 50 experts 4096 x 2048: 375 us), so as many as their registers leave room for.
+template <Weights kW, int kTokens>
+constexpr int kWarpsOf = kW != kE4m3 || kTokens > 2 ? 8 : kTokens == 2 ? 12 : 16;
 
 // Waits that gave up, on this device since the last look.
 __device__ DeviceStatus experts_status;
@@ -174,14 +177,14 @@ __host__ __device__ __forceinline__ long long h_pitch(int ffn)
 }
 
 // A warp's way through the weights, piece by piece: steps of K of a tile of one expert's rows.  32 bits hold every count (see the launcher).
-template <bool kDown>
+template <bool kDown, int kWarps>
 struct Cursor {
     int rank, row, rows;       // the expert, its first row (of the gate, or of down), how many
     int step, steps, stride;   // of K
     int depth;                 // steps of an expert
     int at, end;               // up: tiles of all active experts, one after the other; down: rows of y
-    int offset;                // of the warp in its group
-    int begin, until, begin_rank, position;  // down: the group's steps of all experts, one after the other
+    int offset;                // up: of the warp in its group
+    int begin, until, begin_rank, position;  // down: the warp's steps of all experts, one after the other
     __device__ __forceinline__ void start_up(const Lists &l, int warp, int depth_steps)
     {
         // consecutive tiles go to different SMs; next_up() adds a whole round
@@ -205,34 +208,31 @@ struct Cursor {
         rows = l.tile_pairs + (tile < l.longer ? 1 : 0);
         return true;
     }
-    // Down: the steps of all experts at the same rows go to groups of warps, as many to each, and a group's warps take turns, so that they read
-    // what lies side by side; groups of as many warps as leave each four steps of an expert.
+    // Down: the steps of all experts at the same rows are dealt out to the warps, as many to each.
     __device__ __forceinline__ void start_down(const ExpertsParams &p, const Lists &l, int warp, int depth_steps, int cluster)
     {
         const unsigned shares = gridDim.x / cluster, share = blockIdx.x / cluster;
         at = static_cast<int>(static_cast<unsigned>(p.hidden) * share / shares);
         end = static_cast<int>(static_cast<unsigned>(p.hidden) * (share + 1) / shares);
         depth = depth_steps;
-        stride = depth >= 32 ? 8 : depth >= 16 ? 4 : depth >= 8 ? 2 : 1;
-        const int per_cta = kWarps / stride, groups = per_cta * cluster, group = blockIdx.x % cluster * per_cta + warp / stride, all = l.active * depth;
-        begin = all / groups * group + min(group, all % groups);
-        until = begin + all / groups + (group < all % groups ? 1 : 0);
+        stride = 1;
+        const int warps = kWarps * cluster, number = blockIdx.x % cluster * kWarps + warp, all = l.active * depth;
+        begin = all / warps * number + min(number, all % warps);
+        until = begin + all / warps + (number < all % warps ? 1 : 0);
         begin_rank = begin / depth;
-        offset = warp & (stride - 1);
         rows = 0;
         position = until;
     }
-    // true while the group has steps at the present rows
+    // true while the warp has steps at the present rows
     __device__ __forceinline__ bool next_down()
     {
         if (position >= until) {
             return false;
         }
         ++rank;
-        const int from = position - rank * depth, to = min(depth, until - rank * depth);
-        step = from + offset;
-        steps = to > step ? (to - step + stride - 1) / stride : 0;
-        position += to - from;
+        step = position - rank * depth;
+        steps = min(depth - step, until - position);
+        position += steps;
         return true;
     }
     __device__ __forceinline__ bool next_rows()
@@ -251,8 +251,10 @@ struct Cursor {
 };
 
 // How the first kernel's tiles are cut, by one warp: with kWarps / w groups of w warps per SM and r rounds of tiles, an expert's rows are cut into
-// as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (24 a cycle; a tenth more
-// where no warps read side by side), or the steps of a warp at what one takes in latency where HBM waits (800 cycles), and the sums of a group.
+// as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (23 a cycle), or the steps of a
+// warp at what one takes in latency where HBM waits (800 cycles), and the sums of a group, which its stream does not outlast (64 tokens, 120
+// experts 2048 x 768, first kernel: 134 us with tiles per warp, 144, 197 and 178 for groups of 2, 4 and 8).
+template <int kWarps>
 __device__ __forceinline__ void plan_tiles(Lists &l, int active, int ffn, int depth_steps, int lane)
 {
     const int w = 1 << (lane & 3), extra = lane >> 2, some = max(active, 1);
@@ -263,7 +265,10 @@ __device__ __forceinline__ void plan_tiles(Lists &l, int active, int ffn, int de
     const int pairs = (ffn + tiles - 1) / tiles;
     const float steps = static_cast<float>((depth_steps + w - 1) / w);
     const float bytes = static_cast<float>(kWarps / w * pairs) * 256.0f * static_cast<float>(depth_steps);
-    float cost = static_cast<float>(rounds) * (fmaxf(bytes / (w > 2 ? 24.0f : w > 1 ? 23.0f : 21.5f), 800.0f * steps) + (w > 1 ? 600.0f : 300.0f));
+    float cost = static_cast<float>(rounds) * (fmaxf(bytes / 23.0f, 800.0f * steps) + (w > 1 ? 3000.0f : 500.0f));
+    if (kWarps % w != 0) {
+        cost = 3e38f;
+    }
     int best = lane;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -283,9 +288,10 @@ __device__ __forceinline__ void plan_tiles(Lists &l, int active, int ffn, int de
 }
 
 // All threads of the CTA; l.tokens is zero.  An id that a token names twice counts once, with both weights.
-template <bool kPlan>
+template <bool kPlan, int kWarps>
 __device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p, int depth_steps)
 {
+    constexpr int kThreads = kWarps * 32;
     const int pairs = p.tokens * p.top, tid = static_cast<int>(threadIdx.x);
     for (int i = tid; i < pairs; i += kThreads) {
         const int e = p.ids[i];
@@ -321,7 +327,7 @@ __device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p, int
             l.active = active;
         }
         if (kPlan) {
-            plan_tiles(l, active, p.ffn, depth_steps, tid);
+            plan_tiles<kWarps>(l, active, p.ffn, depth_steps, tid);
         }
     }
     __syncthreads();
@@ -345,12 +351,13 @@ __device__ __forceinline__ void make_lists(Lists &l, const ExpertsParams &p, int
     __syncthreads();
 }
 
-// kTokens: an expert's most, in eights.  One of eight (and fewer) leaves room for a second CTA per SM.
+// kTokens: an expert's most, in eights.
 template <Weights kW, bool kBf, bool kDown, int kTokens>
-__global__ void __launch_bounds__(kThreads, kTokens == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW != kE4m3 ? 2 : 1)
     experts_stream_kernel(const __grid_constant__ ExpertsParams p, const __grid_constant__ CUtensorMap map, const __grid_constant__ Shape shape,
                           const __grid_constant__ Waits waits)
 {
+    constexpr int kWarps = kWarpsOf<kW, kTokens>, kThreads = kWarps * 32;
     constexpr int kElem = kW == kE4m3 ? 1 : 2;
     constexpr int kStep = 128 / kElem;                // of K
     constexpr int kPiece = 16 / kElem;                // of a lane, twice in a step
@@ -399,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, kTokens == 1 ? 2 : 1)
         pdl_wait();
         pdl_launch_dependents();  // behind the wait: what the second kernel reads ahead of its own is older than this one
     }
-    make_lists<!kDown>(lists, p, depth_steps);
-    using Place = Cursor<kDown>;
+    make_lists<!kDown, kWarps>(lists, p, depth_steps);
+    using Place = Cursor<kDown, kWarps>;
     auto start = [&](Place &c) {
         if (kDown) {
             c.start_down(p, lists, warp, depth_steps, shape.cluster);
@@ -882,13 +889,13 @@ __global__ void __launch_bounds__(kThreads, kTokens == 1 ? 2 : 1)
     }
 }
 
-constexpr int kMostShared = 227 * 1024 - 1024;           // of a CTA, beside its static part
+constexpr int kMostShared = 227 * 1024 - 2048;            // of a CTA, beside its static part
 constexpr int kHalfShared = (228 * 1024) / 2 - 2 * 1024;  // where two CTAs are to fit
 
 template <Weights kW, bool kBf, bool kDown, int kTokens>
 cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream)
 {
-    constexpr int kStep = kW == kE4m3 ? 128 : 64;
+    constexpr int kWarps = kWarpsOf<kW, kTokens>, kStep = kW == kE4m3 ? 128 : 64;
     constexpr int kTokenPitch = kStep * (kDown && kW == kF16 ? 4 : 2) + 64;
     Shape shape;
     shape.token_rows = std::min(8, p.tokens);
@@ -896,8 +903,8 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
     shape.cluster = kDown && p.hidden <= 16 * sm_count ? 2 : 1;
     const int fixed = 1024 + (kDown ? kWarps * p.tokens * kRows * 4 : kWarps * 1024) + Lists::bytes(p.experts, p.tokens * p.top);
     const int stage = kWarps * (kStageBytes + shape.token_bytes);
-    // half of the SM, if that gives a ring of three stages and the registers suffice
-    shape.stages = kTokens == 1 ? (kHalfShared - fixed) / stage : 0;
+    // half of the SM, if that gives rings of three stages and the registers suffice
+    shape.stages = kTokens == 1 && kW != kE4m3 ? (kHalfShared - fixed) / stage : 0;
     if (shape.stages < 3) {
         shape.stages = (kMostShared - fixed) / stage;
     }
@@ -912,7 +919,7 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
     const long long limit = wait_limit.load();
     const Waits waits = {limit > 0 ? limit : kDefaultWaitLimitCycles, wait_skip.load()};
     return e != cudaSuccess ? e
-                            : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count / shape.cluster * shape.cluster), dim3(kThreads),
+                            : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count / shape.cluster * shape.cluster), dim3(kWarps * 32),
                                              shared, stream, shape.cluster, p, map, shape, waits);
 }
 
