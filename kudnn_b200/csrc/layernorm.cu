@@ -1,9 +1,9 @@
-// Kernels of layer normalisation (layernorm.cuh).  Both directions read every input once and write every output once: a row stays in registers
-// between the reduction and the result.  The variance is taken about the mean that is already known, not as a difference of two sums.
+// Kernels of layer normalisation (layernorm.cuh).  Both directions read every input once and write every output once.  The variance is taken about the
+// mean that is already known, not as a difference of two sums.
 //
-// Rows are read and written in pieces of 16 bytes that begin on 16-byte boundaries, whatever the row's own address: its first and last piece
-// are then partly its neighbours' (read, never written).  All rows of a CTA are a multiple of `period` rows apart, so that they begin equally far
-// into a piece and one copy of scale and shift in shared memory, moved by as much, serves all of them.
+// Rows are read and written in pieces of 16 bytes that begin on 16-byte boundaries, whatever the row's own address.  All rows of a CTA are a multiple
+// of `period` rows apart, so that they begin equally far into a piece and one copy of scale and shift in shared memory, moved by as much, serves
+// all of them.
 #include "layernorm.cuh"
 
 #include <algorithm>
@@ -14,8 +14,7 @@ namespace kb {
 namespace {
 
 constexpr int kMostThreads = 512;
-constexpr int kMostShared = 160 * 1024;
-constexpr int kRowWarps = 4;     // rows of a CTA at a time where a warp takes a row
+constexpr int kMostShared = 200 * 1024;
 constexpr int kMostParts = 592;  // CTAs of a backward pass, each with sums of its own: four per SM
 
 template <typename T>
@@ -56,57 +55,101 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v)
 template <typename T>
 constexpr int kPer = 16 / sizeof(T);  // elements of a piece
 
+// Two fp32 values in one 64-bit register pair, for the instructions that take both at once
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float lo, float hi)
+{
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 both(Two v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ Two add(Two a, Two b)
+{
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b)
+{
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c)
+{
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 template <typename T>
-__device__ __forceinline__ void unpack(const uint4 &q, float (&v)[kPer<T>])
+__device__ __forceinline__ void unpack(const uint4 &q, Two (&v)[kPer<T> / 2])
 {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kPer<T> / 2; ++j) {
         if (sizeof(T) == 4) {
-            v[j] = __uint_as_float(w[j]);
+            v[j] = two(__uint_as_float(w[2 * j % 4]), __uint_as_float(w[(2 * j + 1) % 4]));
         } else if (std::is_same<T, __nv_bfloat16>::value) {
-            v[2 * j] = __uint_as_float(w[j] << 16);
-            v[(2 * j + 1) % kPer<T>] = __uint_as_float(w[j] & 0xffff0000u);
+            v[j] = two(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
         } else {
             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
-            v[2 * j] = f.x;
-            v[(2 * j + 1) % kPer<T>] = f.y;
+            v[j] = two(f.x, f.y);
         }
     }
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 pack(const float (&v)[kPer<T>])
+__device__ __forceinline__ uint4 pack(const Two (&v)[kPer<T> / 2])
 {
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kPer<T> / 2; ++j) {
+        const float2 f = both(v[j]);
         if (sizeof(T) == 4) {
-            w[j] = __float_as_uint(v[j]);
+            w[2 * j % 4] = __float_as_uint(f.x);
+            w[(2 * j + 1) % 4] = __float_as_uint(f.y);
         } else if (std::is_same<T, __nv_bfloat16>::value) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[(2 * j + 1) % kPer<T>]);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
             w[j] = *reinterpret_cast<const uint32_t *>(&h);
         } else {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[(2 * j + 1) % kPer<T>]);
+            const __half2 h = __floats2half2_rn(f.x, f.y);
             w[j] = *reinterpret_cast<const uint32_t *>(&h);
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Sums of two values over the threads of a row: a warp, or the CTA.  Consecutive calls take turns between two buffers, so that one barrier
-// does: who writes a buffer again has passed the barrier of the call in between, which nobody reached before reading it.  Fixed order.
-template <bool kWarp>
-__device__ __forceinline__ float2 row_sum(float a, float b, float2 (*scratch)[kMostThreads / 32], int &turn)
+// Sum over a warp, in all its lanes.
+__device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
+        v += __shfl_xor_sync(0xffffffffu, v, o);
     }
-    if (kWarp) {
-        return make_float2(a, b);
-    }
+    return v;
+}
+
+// 1 / sqrt(v): the hardware's and a step of Newton's iteration, 2^-23 off at most; the zero and the infinity of the hardware's stay
+__device__ __forceinline__ float inverse_root(float v)
+{
+    const float r = rsqrtf(v);
+    const float better = fmaf(r * 0.5f, fmaf(-v * r, r, 1.0f), r);
+    return r > 0.0f && r < 3e38f ? better : r;
+}
+
+// Sums of two values over the CTA, in a fixed order.  Consecutive calls take turns between two buffers, so that one barrier does: who writes a
+// buffer again has passed the barrier of the call in between, which nobody reached before reading it.
+__device__ __forceinline__ float2 block_sum(float a, float b, float2 (*scratch)[kMostThreads / 32], int &turn)
+{
+    a = warp_sum(a);
+    b = warp_sum(b);
     float2 *buffer = scratch[turn];
     turn ^= 1;
     if ((threadIdx.x & 31) == 0) {
@@ -114,235 +157,207 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (*scratch)[kM
     }
     __syncthreads();
     const int warps = static_cast<int>(blockDim.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
-    float2 s = lane < warps ? buffer[lane] : make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int o = kMostThreads / 64; o > 0; o >>= 1) {
-        s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
-        s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
-    }
-    s.x = __shfl_sync(0xffffffffu, s.x, 0);
-    s.y = __shfl_sync(0xffffffffu, s.y, 0);
-    return s;
-}
-
-// The piece `c` of a row that begins `skew` elements into its first piece: elements [lo, hi) of it are the row's.
-template <typename T>
-struct Span {
-    int lo, hi;
-    __device__ __forceinline__ Span(int c, int skew, int axis)
-        : lo(c == 0 ? skew : 0), hi(min(kPer<T>, axis + skew - c * kPer<T>))
-    {
-    }
-    __device__ __forceinline__ bool whole() const { return lo == 0 && hi == kPer<T>; }
-};
-
-template <typename T>
-__device__ __forceinline__ void store_piece(T *row, int c, const Span<T> &s, bool whole, const float (&v)[kPer<T>])
-{
-    if (whole) {
-        reinterpret_cast<uint4 *>(row)[c] = pack<T>(v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kPer<T>; ++j) {
-            if (j >= s.lo && j < s.hi) {
-                row[c * kPer<T> + j] = narrow<T>(v[j]);
-            }
-        }
-    }
-}
-
-// elements in the pieces of a row wherever it begins
-template <typename T>
-__host__ __device__ __forceinline__ int most_slots(int axis)
-{
-    return (axis + 2 * kPer<T> - 2) / kPer<T> * kPer<T>;
-}
-
-// Scale or shift, moved by the skew, into shared memory (nothing given: `none`).
-template <typename P>
-__device__ __forceinline__ void stage(P *to, const void *from, int skew, int axis, int slots, float none, int lane, int lanes)
-{
-    for (int i = lane; i < slots; i += lanes) {
-        const int e = i - skew;
-        to[i] = from != nullptr && e >= 0 && e < axis ? static_cast<const P *>(from)[e] : narrow<P>(none);
-    }
+    const float2 s = lane < warps ? buffer[lane] : make_float2(0.0f, 0.0f);
+    return make_float2(warp_sum(s.x), warp_sum(s.y));
 }
 
 // kPer<T> values of P from shared memory, 16 bytes at a time
 template <typename T, typename P>
-__device__ __forceinline__ void fetch(const P *from, int c, float (&v)[kPer<T>])
+__device__ __forceinline__ void fetch(const P *from, int c, Two (&v)[kPer<T> / 2])
 {
-    constexpr int kReads = kPer<T> / kPer<P>;
+    constexpr int kReads = kPer<T> / kPer<P>, kPairs = kPer<P> / 2;
 #pragma unroll
     for (int i = 0; i < kReads; ++i) {
-        float part[kPer<P>];
+        Two part[kPairs];
         unpack<P>(reinterpret_cast<const uint4 *>(from)[c * kReads + i], part);
 #pragma unroll
-        for (int j = 0; j < kPer<P>; ++j) {
-            v[(i * kPer<P> + j) % kPer<T>] = part[j];
+        for (int j = 0; j < kPairs; ++j) {
+            v[(i * kPairs + j) % (kPer<T> / 2)] = part[j];
         }
     }
 }
 
-// Who takes a row: a warp of kRowWarps, or the CTA.
-template <bool kWarp>
-struct Team {
-    int lane, lanes, index;
-    long long first, step;
-    __device__ __forceinline__ Team()
-        : lane(static_cast<int>(threadIdx.x) & (kWarp ? 31 : 0x3ff)),
-          lanes(kWarp ? 32 : static_cast<int>(blockDim.x)),
-          index(kWarp ? static_cast<int>(threadIdx.x) >> 5 : 0),
-          first(kWarp ? blockIdx.x * static_cast<long long>(kRowWarps) + index : blockIdx.x),
-          step(kWarp ? gridDim.x * static_cast<long long>(kRowWarps) : gridDim.x)
+// How rows are dealt out.  A team of `warps` warps takes a row, a CTA has `teams` of them.  CTA b takes rows of the class b % period, so that all
+// of its rows begin equally far into a piece.
+struct Teams {
+    int warps, teams, period;
+    int row_bytes;  // of shared memory per row: its whole pieces
+    int stages;     // backward: rows of a team in shared memory
+};
+
+// A thread's place in them.
+template <typename T, bool kEdge>
+struct Place {
+    int lanes, team, lane;
+    long long row, step;    // first row, and from one to the next
+    int head, whole, tail;  // elements in front of the first whole piece, whole pieces, elements behind
+    bool single;            // this lane has one of those elements: number `at`
+    int at;
+    __device__ __forceinline__ Place(const LayernormParams &p, const Teams &of)
+        : lanes(of.warps * 32), team(static_cast<int>(threadIdx.x) / lanes), lane(static_cast<int>(threadIdx.x) - team * lanes)
     {
-    }
-    __device__ __forceinline__ void sync() const
-    {
-        if (kWarp) {
-            __syncwarp();
-        } else {
-            __syncthreads();
-        }
+        constexpr int kV = kPer<T>;
+        const int in_class = static_cast<int>(blockIdx.x) % of.period;
+        step = static_cast<long long>(gridDim.x) * of.teams;  // gridDim.x is a multiple of the period
+        row = in_class + static_cast<long long>(of.period) * (static_cast<long long>(blockIdx.x) / of.period * of.teams + team);
+        const int skew =
+            kEdge ? static_cast<int>(reinterpret_cast<uintptr_t>(static_cast<const T *>(p.x) + in_class * p.x_ld) & 15u) / static_cast<int>(sizeof(T)) : 0;
+        head = min(p.axis, (kV - skew) % kV);
+        whole = (p.axis - head) / kV;
+        tail = p.axis - head - whole * kV;
+        single = kEdge && (lane < head || (lane >= 16 && lane - 16 < tail));
+        at = lane < 16 ? lane : p.axis - tail + lane - 16;
     }
 };
 
-// kWarp: a warp per row, otherwise a CTA; kN pieces per thread.  Two rows at a time: twice the bytes in flight, and scale and shift are read from
-// shared memory once for both.  kEdge: some row has pieces that are only partly its own.
-template <typename T, typename P, int kN, bool kEdge, bool kWarp>
-__global__ void __launch_bounds__(kMostThreads) layernorm_kernel(const __grid_constant__ LayernormParams p)
+// Sum over a team's warps, in a fixed order; consecutive calls take turns between two buffers (see block_sum).
+__device__ __forceinline__ float2 team_sum(float a, float b, const Teams &of, int team, float2 (*scratch)[kMostThreads / 32], int &turn)
+{
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (of.warps == 1) {
+        return make_float2(a, b);
+    }
+    float2 *buffer = scratch[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+        buffer[threadIdx.x >> 5] = make_float2(a, b);
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(of.warps * 32) : "memory");
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < of.warps; ++w) {
+        const float2 v = buffer[team * of.warps + w];
+        s.x += v.x;
+        s.y += v.y;
+    }
+    return s;
+}
+
+__device__ __forceinline__ void copy_piece(unsigned char *to, const void *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+
+// A row lies in shared memory (cp.async, the next one on its way meanwhile; each thread reads back only what it copied itself) and is gone through
+// three times: mean, squares about it, result.  What bounds it is instructions: the fewer threads a row has, the fewer of them compute the
+// row's statistics, so a team is as small as 256 bytes per lane allow.  kEdge: the elements in front of the first whole piece and behind the
+// last one are single lanes' own, in registers.
+template <typename T, typename P, bool kEdge>
+__global__ void __launch_bounds__(kMostThreads, 2) layernorm_kernel(const __grid_constant__ LayernormParams p, const __grid_constant__ Teams of)
 {
     extern __shared__ uint4 shared[];
     __shared__ float2 scratch[2][kMostThreads / 32];
     constexpr int kV = kPer<T>;
-    const Team<kWarp> team;
-    const int lane = team.lane, lanes = team.lanes;
-    const long long step = team.step;
-    long long row = team.first;
+    const Place<T, kEdge> place(p, of);
+    const int lanes = place.lanes, lane = place.lane, head = place.head, whole = place.whole, at = place.at, slots = whole * kV;
+    const bool single = place.single;
+    const long long step = place.step;
+    long long row = place.row;
     const T *x0 = static_cast<const T *>(p.x);
     T *y0 = static_cast<T *>(p.y);
-    const int skew = kEdge ? static_cast<int>(reinterpret_cast<uintptr_t>(x0 + row * p.x_ld) & 15u) / static_cast<int>(sizeof(T)) : 0;
-    const int pieces = (p.axis + skew + kV - 1) / kV, slots = pieces * kV;
-    // teams of a CTA have copies of their own where their rows may begin elsewhere
-    P *scale = reinterpret_cast<P *>(shared) + (kWarp && kEdge ? team.index * 2ll * most_slots<T>(p.axis) : 0);
-    P *shift = scale + slots;
-    int turn = 0;
+    P *scale = reinterpret_cast<P *>(shared), *shift = scale + slots;
+    unsigned char *ring = reinterpret_cast<unsigned char *>(shared) + (2ll * slots * sizeof(P) + 15) / 16 * 16 + place.team * 2ll * of.row_bytes;
     pdl_launch_dependents();
     pdl_wait();
-    uint4 q[2][kN];
-    auto load = [&](long long r, uint4(&to)[kN]) {
-        const uint4 *from = reinterpret_cast<const uint4 *>(x0 + r * p.x_ld - skew);
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int c = lane + i * lanes;
-            to[i] = c < pieces ? from[c] : make_uint4(0u, 0u, 0u, 0u);
+    auto load = [&](long long r, int stage) {
+        if (r < p.rows) {
+            const uint4 *from = reinterpret_cast<const uint4 *>(x0 + r * p.x_ld + head);
+            unsigned char *to = ring + stage * of.row_bytes;
+            for (int c = lane; c < whole; c += lanes) {
+                copy_piece(to + c * 16, from + c);
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    bool staged = false;
+    load(row, 0);
+    load(row + step, 1);
+    float own = 0.0f, own_next = 0.0f, own_scale = 1.0f, own_shift = 0.0f;
+    if (single) {
+        own_next = row < p.rows ? widen<T>(x0[row * p.x_ld + at]) : 0.0f;
+        own_scale = p.scale != nullptr ? widen<P>(static_cast<const P *>(p.scale)[at]) : 1.0f;
+        own_shift = p.shift != nullptr ? widen<P>(static_cast<const P *>(p.shift)[at]) : 0.0f;
+    }
+    for (int i = static_cast<int>(threadIdx.x); i < slots; i += static_cast<int>(blockDim.x)) {
+        scale[i] = p.scale != nullptr ? static_cast<const P *>(p.scale)[head + i] : narrow<P>(1.0f);
+        shift[i] = p.shift != nullptr ? static_cast<const P *>(p.shift)[head + i] : narrow<P>(0.0f);
+    }
+    __syncthreads();
+    int turn = 0;
     const float inv_axis = 1.0f / static_cast<float>(p.axis);
-    for (; row < p.rows; row += 2 * step) {
-        const bool two = row + step < p.rows;
-        load(row, q[0]);
-        if (two) {
-            load(row + step, q[1]);
+    int stage = 0;
+    for (; row < p.rows; row += step) {
+        if (kEdge) {
+            own = own_next;
+            own_next = single && row + step < p.rows ? widen<T>(x0[(row + step) * p.x_ld + at]) : 0.0f;
         }
-        if (!staged) {
-            stage(scale, p.scale, skew, p.axis, slots, 1.0f, lane, lanes);
-            stage(shift, p.shift, skew, p.axis, slots, 0.0f, lane, lanes);
-            staged = true;
-            team.sync();
-        }
-        float mean[2], var[2];
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        const uint4 *x = reinterpret_cast<const uint4 *>(ring + stage * of.row_bytes);
+        float mean, var;
         if (p.given != 0) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                mean[k] = k == 0 || two ? p.mean[row + k * step] : 0.0f;
-                var[k] = k == 0 || two ? p.variance[row + k * step] : 0.0f;
-            }
+            mean = p.mean[row];
+            var = p.variance[row];
         } else {
-            float s[2] = {0.0f, 0.0f};
+            Two s = two(kEdge ? own : 0.0f, 0.0f);
+#pragma unroll 4
+            for (int c = lane; c < whole; c += lanes) {
+                Two v[kV / 2];
+                unpack<T>(x[c], v);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (k == 0 || two) {
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) {
-                        float v[kV];
-                        unpack<T>(q[k][i], v);
-                        const Span<T> span(lane + i * lanes, skew, p.axis);
-                        const bool whole = !kEdge || span.whole();
-#pragma unroll
-                        for (int j = 0; j < kV; ++j) {
-                            s[k] += whole || (j >= span.lo && j < span.hi) ? v[j] : 0.0f;
-                        }
-                    }
+                for (int j = 0; j < kV / 2; ++j) {
+                    s = add(s, v[j]);
                 }
             }
-            float2 total = row_sum<kWarp>(s[0], s[1], scratch, turn);
-            mean[0] = total.x * inv_axis;
-            mean[1] = total.y * inv_axis;
-            s[0] = s[1] = 0.0f;
+            float2 halves = both(s);
+            mean = team_sum(halves.x + halves.y, 0.0f, of, place.team, scratch, turn).x * inv_axis;
+            const float d = single ? own - mean : 0.0f;
+            const Two less = two(-mean, -mean);
+            s = two(d * d, 0.0f);
+#pragma unroll 4
+            for (int c = lane; c < whole; c += lanes) {
+                Two v[kV / 2];
+                unpack<T>(x[c], v);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (k == 0 || two) {
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) {
-                        float v[kV];
-                        unpack<T>(q[k][i], v);
-                        const int c = lane + i * lanes;
-                        const Span<T> span(c, skew, p.axis);
-                        const bool whole = kEdge ? span.whole() : c < pieces;
-#pragma unroll
-                        for (int j = 0; j < kV; ++j) {
-                            const float d = v[j] - mean[k];
-                            const bool mine = whole || (kEdge && j >= span.lo && j < span.hi);
-                            s[k] = mine ? fmaf(d, d, s[k]) : s[k];
-                        }
-                    }
+                for (int j = 0; j < kV / 2; ++j) {
+                    const Two e = add(v[j], less);
+                    s = fma(e, e, s);
                 }
             }
-            total = row_sum<kWarp>(s[0], s[1], scratch, turn);
-            var[0] = total.x * inv_axis;
-            var[1] = total.y * inv_axis;
+            halves = both(s);
+            var = team_sum(halves.x + halves.y, 0.0f, of, place.team, scratch, turn).x * inv_axis;
             if (lane == 0) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if ((k == 0 || two) && p.mean != nullptr) {
-                        p.mean[row + k * step] = mean[k];
-                    }
-                    if ((k == 0 || two) && p.variance != nullptr) {
-                        p.variance[row + k * step] = var[k];
-                    }
+                if (p.mean != nullptr) {
+                    p.mean[row] = mean;
+                }
+                if (p.variance != nullptr) {
+                    p.variance[row] = var;
                 }
             }
         }
-        const float r[2] = {1.0f / sqrtf(var[0] + p.eps), 1.0f / sqrtf(var[1] + p.eps)};
+        const float r = inverse_root(var + p.eps);
+        T *y = y0 + row * p.y_ld;
+        uint4 *to = reinterpret_cast<uint4 *>(y + head);
+        const Two less = two(-mean, -mean), times = two(r, r);
+#pragma unroll 2
+        for (int c = lane; c < whole; c += lanes) {
+            Two v[kV / 2], a[kV / 2], b[kV / 2];
+            unpack<T>(x[c], v);
+            fetch<T, P>(scale, c, a);
+            fetch<T, P>(shift, c, b);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int c = lane + i * lanes;
-            if (c < pieces) {
-                float a[kV], b[kV];
-                fetch<T, P>(scale, c, a);
-                fetch<T, P>(shift, c, b);
-                const Span<T> span(c, skew, p.axis);
-                const bool whole = !kEdge || span.whole();
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (k == 0 || two) {
-                        float v[kV];
-                        unpack<T>(q[k][i], v);
-#pragma unroll
-                        for (int j = 0; j < kV; ++j) {
-                            v[j] = fmaf((v[j] - mean[k]) * r[k], a[j], b[j]);
-                        }
-                        store_piece<T>(y0 + (row + k * step) * p.y_ld - skew, c, span, whole, v);
-                    }
-                }
+            for (int j = 0; j < kV / 2; ++j) {
+                v[j] = fma(mul(add(v[j], less), times), a[j], b[j]);
             }
+            to[c] = pack<T>(v);
         }
+        if (single) {
+            y[at] = narrow<T>(fmaf((own - mean) * r, own_scale, own_shift));
+        }
+        load(row + 2 * step, stage);
+        stage ^= 1;
     }
 }
 
-// Rows longer than the registers of a CTA hold, or whose x and y do not begin equally far into a piece: element by element, x read three times.
+// Rows longer than shared memory holds, or whose x and y do not begin equally far into a piece: element by element, x read three times.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kMostThreads) layernorm_any_kernel(const __grid_constant__ LayernormParams p)
 {
@@ -362,13 +377,13 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_any_kernel(const __gri
             for (int i = static_cast<int>(threadIdx.x); i < p.axis; i += static_cast<int>(blockDim.x)) {
                 s += widen<T>(x[i]);
             }
-            mean = row_sum<false>(s, 0.0f, scratch, turn).x / static_cast<float>(p.axis);
+            mean = block_sum(s, 0.0f, scratch, turn).x / static_cast<float>(p.axis);
             s = 0.0f;
             for (int i = static_cast<int>(threadIdx.x); i < p.axis; i += static_cast<int>(blockDim.x)) {
                 const float d = widen<T>(x[i]) - mean;
                 s = fmaf(d, d, s);
             }
-            var = row_sum<false>(s, 0.0f, scratch, turn).x / static_cast<float>(p.axis);
+            var = block_sum(s, 0.0f, scratch, turn).x / static_cast<float>(p.axis);
             if (threadIdx.x == 0) {
                 if (p.mean != nullptr) {
                     p.mean[row] = mean;
@@ -387,141 +402,195 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_any_kernel(const __gri
     }
 }
 
-// The gradient: a row at a time per CTA or warp, the next row's x and dy on their way while this one is summed.  The sums over rows of dscale and dshift
-// stay in registers, each thread its own columns; every CTA leaves one set of them, added up in a fixed order by column_sums_kernel.
-template <typename T, typename P, int kN, bool kEdge, bool kWarp>
-__global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const __grid_constant__ LayernormParams p)
+// The gradient, rows as in the forward pass: a thread's kN pieces of x and dy come by way of shared memory, are widened once and kept as xh and g
+// between the row's sums and dx (kKeep), unless that takes too many registers.  The sums over rows of dscale and dshift stay in registers, each
+// thread its own columns; every CTA leaves one set of them, added up in a fixed order by column_sums_kernel.
+template <typename T, typename P, int kN, bool kEdge>
+__global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const __grid_constant__ LayernormParams p, const __grid_constant__ Teams of)
 {
     extern __shared__ uint4 shared[];
     __shared__ float2 scratch[2][kMostThreads / 32];
-    constexpr int kV = kPer<T>;
-    const Team<kWarp> team;
-    const int lane = team.lane, lanes = team.lanes;
-    const long long step = team.step;
-    long long row = team.first;
+    constexpr int kV = kPer<T>, kH = kV / 2;
+    constexpr bool kKeep = kN * kV <= 16;
+    const Place<T, kEdge> place(p, of);
+    const int lanes = place.lanes, lane = place.lane, head = place.head, whole = place.whole, at = place.at, slots = whole * kV;
+    const bool single = place.single;
+    const long long step = place.step;
+    long long row = place.row;
     const T *x0 = static_cast<const T *>(p.x), *dy0 = static_cast<const T *>(p.dy);
-    const int skew = kEdge ? static_cast<int>(reinterpret_cast<uintptr_t>(x0 + row * p.x_ld) & 15u) / static_cast<int>(sizeof(T)) : 0;
-    const int pieces = (p.axis + skew + kV - 1) / kV, slots = pieces * kV;
-    P *scale = reinterpret_cast<P *>(shared) + (kWarp && kEdge ? static_cast<long long>(team.index) * most_slots<T>(p.axis) : 0);
-    int turn = 0;
+    P *scale = reinterpret_cast<P *>(shared);
+    unsigned char *ring = reinterpret_cast<unsigned char *>(shared) + (static_cast<long long>(slots) * sizeof(P) + 15) / 16 * 16 +
+                          place.team * 2ll * of.stages * of.row_bytes;  // [stage][x, dy]
     pdl_launch_dependents();
     pdl_wait();
-    uint4 x_next[kN], dy_next[kN];
-    float mean_next = 0.0f, var_next = 0.0f;
-    auto load = [&](long long r) {
-        const uint4 *x = reinterpret_cast<const uint4 *>(x0 + r * p.x_ld - skew), *dy = reinterpret_cast<const uint4 *>(dy0 + r * p.dy_ld - skew);
+    auto load = [&](long long r, int stage) {
+        if (r < p.rows) {
+            const uint4 *x = reinterpret_cast<const uint4 *>(x0 + r * p.x_ld + head), *dy = reinterpret_cast<const uint4 *>(dy0 + r * p.dy_ld + head);
+            unsigned char *to = ring + stage * 2 * of.row_bytes;
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int c = lane + i * lanes;
-            x_next[i] = c < pieces ? x[c] : make_uint4(0u, 0u, 0u, 0u);
-            dy_next[i] = c < pieces ? dy[c] : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < kN; ++i) {
+                const int c = lane + i * lanes;
+                if (c < whole) {
+                    copy_piece(to + c * 16, x + c);
+                    copy_piece(to + of.row_bytes + c * 16, dy + c);
+                }
+            }
         }
-        mean_next = p.mean[r];
-        var_next = p.variance[r];
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    float sum_scale[kN][kV], sum_shift[kN][kV];
+    load(row, 0);
+    if (of.stages > 1) {
+        load(row + step, 1);
+    }
+    float mean_next = 0.0f, var_next = 0.0f, x_next = 0.0f, dy_next = 0.0f;
+    auto ahead = [&](long long r) {
+        if (r < p.rows) {
+            mean_next = p.mean[r];
+            var_next = p.variance[r];
+            if (single) {
+                x_next = widen<T>(x0[r * p.x_ld + at]);
+                dy_next = widen<T>(dy0[r * p.dy_ld + at]);
+            }
+        }
+    };
+    ahead(row);
+    const float own_scale = single && p.scale != nullptr ? widen<P>(static_cast<const P *>(p.scale)[at]) : 1.0f;
+    float own_sum_scale = 0.0f, own_sum_shift = 0.0f;
+    Two sum_scale[kN][kH], sum_shift[kN][kH];
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
 #pragma unroll
-        for (int j = 0; j < kV; ++j) {
-            sum_scale[i][j] = sum_shift[i][j] = 0.0f;
+        for (int j = 0; j < kH; ++j) {
+            sum_scale[i][j] = sum_shift[i][j] = 0ull;
         }
     }
-    if (row < p.rows) {
-        load(row);
+    for (int i = static_cast<int>(threadIdx.x); i < slots; i += static_cast<int>(blockDim.x)) {
+        scale[i] = p.scale != nullptr ? static_cast<const P *>(p.scale)[head + i] : narrow<P>(1.0f);
     }
-    stage(scale, p.scale, skew, p.axis, slots, 1.0f, lane, lanes);
-    team.sync();
+    __syncthreads();
     const float inv_axis = 1.0f / static_cast<float>(p.axis);
+    int turn = 0, stage = 0;
     for (; row < p.rows; row += step) {
-        uint4 x[kN], dy[kN];
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            x[i] = x_next[i];
-            dy[i] = dy_next[i];
+        const float mean = mean_next, r = inverse_root(var_next + p.eps), own_xh = single ? (x_next - mean) * r : 0.0f, own_dy = single ? dy_next : 0.0f;
+        const Two less = two(-mean, -mean), times = two(r, r);
+        ahead(row + step);
+        if (of.stages > 1) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
-        const float mean = mean_next, r = 1.0f / sqrtf(var_next + p.eps);
-        if (row + step < p.rows) {
-            load(row + step);
+        const uint4 *x = reinterpret_cast<const uint4 *>(ring + stage * 2 * of.row_bytes), *dy = x + of.row_bytes / 16;
+        Two kept_xh[kKeep ? kN : 1][kH], kept_g[kKeep ? kN : 1][kH];
+        const float own_g = own_dy * own_scale;
+        Two of_g = two(own_g, 0.0f), of_gx = two(own_g * own_xh, 0.0f);
+        if (kEdge) {
+            own_sum_scale = fmaf(own_dy, own_xh, own_sum_scale);
+            own_sum_shift += own_dy;
         }
-        float of_g = 0.0f, of_gx = 0.0f;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const int c = lane + i * lanes;
-            const Span<T> span(c, skew, p.axis);
-            const bool whole = kEdge ? span.whole() : c < pieces;
-            if (whole || (kEdge && span.lo < span.hi)) {
-                float xv[kV], dv[kV], a[kV];
-                unpack<T>(x[i], xv);
-                unpack<T>(dy[i], dv);
+            if (c < whole) {
+                Two xh[kH], d[kH], a[kH];
+                unpack<T>(x[c], xh);
+                unpack<T>(dy[c], d);
                 fetch<T, P>(scale, c, a);
 #pragma unroll
-                for (int j = 0; j < kV; ++j) {
-                    const bool mine = whole || (j >= span.lo && j < span.hi);
-                    const float d = mine ? dv[j] : 0.0f, xh = mine ? (xv[j] - mean) * r : 0.0f, g = d * a[j];
-                    of_g += g;
-                    of_gx = fmaf(g, xh, of_gx);
-                    sum_scale[i][j] = fmaf(d, xh, sum_scale[i][j]);
-                    sum_shift[i][j] += d;
+                for (int j = 0; j < kH; ++j) {
+                    xh[j] = mul(add(xh[j], less), times);
+                    sum_scale[i][j] = fma(d[j], xh[j], sum_scale[i][j]);
+                    sum_shift[i][j] = add(sum_shift[i][j], d[j]);
+                    const Two g = mul(d[j], a[j]);
+                    of_g = add(of_g, g);
+                    of_gx = fma(g, xh[j], of_gx);
+                    if (kKeep) {
+                        kept_xh[kKeep ? i : 0][j] = xh[j];
+                        kept_g[kKeep ? i : 0][j] = g;
+                    }
                 }
             }
         }
         if (p.y != nullptr) {
+            float along = 0.0f, level = 0.0f;
             if (p.given == 0) {
-                const float2 total = row_sum<kWarp>(of_g, of_gx, scratch, turn);
-                of_g = total.x * inv_axis;
-                of_gx = total.y * inv_axis;
-            } else {
-                of_g = of_gx = 0.0f;
+                const float2 g = both(of_g), gx = both(of_gx);
+                const float2 total = team_sum(g.x + g.y, gx.x + gx.y, of, place.team, scratch, turn);
+                level = total.x * inv_axis;
+                along = total.y * inv_axis;
             }
-            T *to = static_cast<T *>(p.y) + row * p.y_ld - skew;
+            const Two no_level = two(-level, -level), no_along = two(-along, -along);
+            T *dx = static_cast<T *>(p.y) + row * p.y_ld;
+            uint4 *to = reinterpret_cast<uint4 *>(dx + head);
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 const int c = lane + i * lanes;
-                if (c < pieces) {
-                    float xv[kV], dv[kV], a[kV];
-                    unpack<T>(x[i], xv);
-                    unpack<T>(dy[i], dv);
-                    fetch<T, P>(scale, c, a);
-                    const Span<T> span(c, skew, p.axis);
+                if (c < whole) {
+                    Two xh[kH], g[kH];
+                    if (kKeep) {
 #pragma unroll
-                    for (int j = 0; j < kV; ++j) {
-                        const float xh = (xv[j] - mean) * r, g = dv[j] * a[j];
-                        dv[j] = p.given != 0 ? r * g : r * (g - of_g - xh * of_gx);
+                        for (int j = 0; j < kH; ++j) {
+                            xh[j] = kept_xh[kKeep ? i : 0][j];
+                            g[j] = kept_g[kKeep ? i : 0][j];
+                        }
+                    } else {
+                        Two a[kH];
+                        unpack<T>(x[c], xh);
+                        unpack<T>(dy[c], g);
+                        fetch<T, P>(scale, c, a);
+#pragma unroll
+                        for (int j = 0; j < kH; ++j) {
+                            xh[j] = mul(add(xh[j], less), times);
+                            g[j] = mul(g[j], a[j]);
+                        }
                     }
-                    store_piece<T>(to, c, span, !kEdge || span.whole(), dv);
+#pragma unroll
+                    for (int j = 0; j < kH; ++j) {
+                        g[j] = mul(p.given != 0 ? g[j] : fma(xh[j], no_along, add(g[j], no_level)), times);
+                    }
+                    to[c] = pack<T>(g);
                 }
             }
+            if (single) {
+                dx[at] = narrow<T>((p.given != 0 ? own_g : fmaf(-own_xh, along, own_g - level)) * r);
+            }
         }
+        load(row + of.stages * step, stage);
+        stage = of.stages > 1 ? stage ^ 1 : 0;
     }
     if (p.partial == nullptr) {
         return;
     }
+    // the teams' sums, one after the other
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     float *to = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.axis;
-    float *sums = kWarp ? reinterpret_cast<float *>(shared) : to;  // the warps' sums are added up one after the other
-#pragma unroll 1
-    for (int turn_of = 0; turn_of < (kWarp ? kRowWarps : 1); ++turn_of) {
-        if (kWarp) {
+    float *sums = of.teams > 1 ? reinterpret_cast<float *>(shared) : to;
+    for (int k = 0; k < of.teams; ++k) {
+        if (of.teams > 1) {
             __syncthreads();
         }
-        if (team.index == turn_of) {
+        if (place.team == k) {
+            auto put = [&](int e, float of_scale, float of_shift) {
+                sums[e] = of_scale + (k == 0 ? 0.0f : sums[e]);
+                sums[p.axis + e] = of_shift + (k == 0 ? 0.0f : sums[p.axis + e]);
+            };
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 const int c = lane + i * lanes;
-                if (c < pieces) {
+                if (c < whole) {
 #pragma unroll
-                    for (int j = 0; j < kV; ++j) {
-                        const int e = c * kV + j - skew;
-                        if (e >= 0 && e < p.axis) {
-                            sums[e] = sum_scale[i][j] + (turn_of == 0 ? 0.0f : sums[e]);
-                            sums[p.axis + e] = sum_shift[i][j] + (turn_of == 0 ? 0.0f : sums[p.axis + e]);
-                        }
+                    for (int j = 0; j < kH; ++j) {
+                        const float2 of_scale = both(sum_scale[i][j]), of_shift = both(sum_shift[i][j]);
+                        put(head + c * kV + 2 * j, of_scale.x, of_shift.x);
+                        put(head + c * kV + 2 * j + 1, of_scale.y, of_shift.y);
                     }
                 }
             }
+            if (single) {
+                put(at, own_sum_scale, own_sum_shift);
+            }
         }
     }
-    if (kWarp) {
+    if (of.teams > 1) {
         __syncthreads();
         for (int e = static_cast<int>(threadIdx.x); e < 2 * p.axis; e += static_cast<int>(blockDim.x)) {
             to[e] = sums[e];
@@ -564,7 +633,7 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_backward_any_kernel(co
                     of_g += g;
                     of_gx = fmaf(g, (widen<T>(x[i]) - mean) * r, of_gx);
                 }
-                const float2 total = row_sum<false>(of_g, of_gx, scratch, turn);
+                const float2 total = block_sum(of_g, of_gx, scratch, turn);
                 of_g = total.x / static_cast<float>(p.axis);
                 of_gx = total.y / static_cast<float>(p.axis);
             }
@@ -625,84 +694,144 @@ int period_of(const LayernormParams &p, int elem, bool backward)
     return period;
 }
 
-struct Shape {
-    int threads, pieces, grid;
-    size_t shared;
-    bool edge, warp;
-};
+// CTAs that give every row to a team of its own, none of them without rows (in the last round of the classes, fewer than the period).
+long long ctas_for(long long rows, int teams, int period)
+{
+    const long long round = static_cast<long long>(teams) * period, before = (rows - 1) / round;
+    return before * period + std::min<long long>(period, rows - before * round);
+}
 
 // false: the general kernel
-bool shape_of(const LayernormParams &p, int elem, int param_elem, bool backward, int sm_count, Shape *s)
+bool teams_of(const LayernormParams &p, int elem, int param_elem, int sm_count, Teams *t, int *grid, size_t *shared)
 {
-    const int period = period_of(p, elem, backward);
+    const int period = period_of(p, elem, false);
     if (period == 0) {
         return false;
     }
-    const int per = 16 / elem;
-    s->edge = period != 1 || (reinterpret_cast<uintptr_t>(p.x) & 15u) != 0 || p.axis % per != 0;
-    const long long most = (static_cast<long long>(p.axis) + (s->edge ? 2 * per - 2 : per - 1)) / per;  // pieces of a row
-    s->warp = most <= 128;
-    s->pieces = most <= 32 ? 1 : most <= 64 ? 2 : s->warp ? 4 : most <= 512 ? 2 : 4;
-    const long long threads = s->warp ? 32 * kRowWarps : ((most + s->pieces - 1) / s->pieces + 31) / 32 * 32;
-    long long shared = most * per * param_elem * (backward ? 1 : 2) * (s->warp && s->edge ? kRowWarps : 1);
-    if (backward && s->warp) {
-        shared = std::max<long long>(shared, 8ll * p.axis);
-    }
-    if (threads > kMostThreads || shared > kMostShared) {
+    const long long bytes = (static_cast<long long>(p.axis) * elem + 15) / 16 * 16;
+    const long long params = 2ll * p.axis * param_elem;
+    const long long most = kMostShared - (params + 15) / 16 * 16;
+    if (2 * bytes > most) {
         return false;
     }
-    s->threads = static_cast<int>(threads);
-    s->shared = static_cast<size_t>(shared);
-    const int rows = s->warp ? kRowWarps : 1;
-    const long long per_sm = std::min<long long>(std::min<long long>((backward ? 512 : 1536) / threads, (200 * 1024) / (shared + 1024)), 24);
-    long long grid = std::max<long long>(1, per_sm) * sm_count;
-    if (backward) {
-        grid = std::min<long long>(grid, kMostParts);
+    int warps = 1;
+    while (warps < 16 && (bytes > warps * 8192ll || (p.rows <= 2ll * sm_count && bytes > warps * 512ll))) {
+        warps *= 2;  // 256 bytes per lane, or with few rows one piece
     }
-    grid = grid / period * period;
-    s->grid = static_cast<int>(std::min<long long>(grid, (p.rows + rows - 1) / rows));
+    int teams = static_cast<int>(std::max<long long>(1, std::min<long long>(16 / warps, most / (2 * bytes))));
+    const long long need = (p.rows + sm_count - 1) / sm_count;
+    while (teams > 1 && teams / 2 >= need) {
+        teams /= 2;
+    }
+    *shared = static_cast<size_t>((params + 15) / 16 * 16 + 2 * bytes * teams);
+    const int threads = teams * warps * 32;
+    const long long per_sm = std::max<long long>(1, std::min<long long>({1024 / threads, static_cast<long long>(226 * 1024 / (*shared + 1280)), 16ll}));
+    const long long enough = ctas_for(p.rows, teams, period);
+    *grid = static_cast<int>(std::min<long long>(per_sm * sm_count / period * period, enough));
+    *t = {warps, teams, period, static_cast<int>(bytes), 2};
     return true;
 }
 
-template <typename T, typename P, int kN, bool kEdge, bool kWarp>
-cudaError_t launch_shape(const LayernormParams &p, const Shape &s, bool backward, cudaStream_t stream)
+// The same for the gradient, kN pieces per thread.
+bool backward_teams_of(const LayernormParams &p, int elem, int param_elem, int sm_count, Teams *t, int *pieces, int *grid, size_t *shared)
 {
-    void (*kernel)(LayernormParams) = backward ? layernorm_backward_kernel<T, P, kN, kEdge, kWarp> : layernorm_kernel<T, P, kN, kEdge, kWarp>;
-    if (s.shared > 40 * 1024) {
+    const int period = period_of(p, elem, true);
+    if (period == 0) {
+        return false;
+    }
+    const long long bytes = (static_cast<long long>(p.axis) * elem + 15) / 16 * 16, whole = bytes / 16;
+    const long long params = (static_cast<long long>(p.axis) * param_elem + 15) / 16 * 16;
+    const int usual = elem == 4 ? 4 : 2;  // 16 elements per thread
+    *pieces = whole <= 32 ? 1 : whole <= 64 ? 2 : whole <= usual * kMostThreads ? usual : 2 * usual;
+    const long long warps = (whole + *pieces * 32 - 1) / (*pieces * 32);
+    if (warps * 32 > kMostThreads) {
+        return false;
+    }
+    const int stages = params + 4 * bytes <= kMostShared ? 2 : 1;
+    if (params + 2 * stages * bytes > kMostShared) {
+        return false;
+    }
+    int teams = static_cast<int>(std::max<long long>(1, std::min<long long>(8 / warps, (kMostShared - params) / (2 * stages * bytes))));
+    const long long need = (p.rows + sm_count - 1) / sm_count;
+    while (teams > 1 && teams / 2 >= need) {
+        teams /= 2;
+    }
+    *shared = static_cast<size_t>(std::max(params + 2 * stages * bytes * teams, teams > 1 ? 8ll * p.axis : 0ll));
+    const int threads = static_cast<int>(teams * warps * 32);
+    const long long per_sm = std::max<long long>(1, std::min<long long>(512 / threads, static_cast<long long>(226 * 1024 / (*shared + 1280))));
+    const long long enough = ctas_for(p.rows, teams, period);
+    *grid = static_cast<int>(std::min<long long>({per_sm * sm_count / period * period, kMostParts / period * period, enough}));
+    *t = {static_cast<int>(warps), teams, period, static_cast<int>(bytes), stages};
+    return true;
+}
+
+// Raises the kernel's limit of shared memory and launches it.
+cudaError_t launch_teams(void (*kernel)(LayernormParams, Teams), const LayernormParams &p, const Teams &t, int grid, size_t shared, cudaStream_t stream)
+{
+    if (shared > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
         if (e != cudaSuccess) {
             return e;
         }
     }
-    return launch_chained(kernel, dim3(s.grid), dim3(s.threads), s.shared, stream, 1u, p);
+    return launch_chained(kernel, dim3(grid), dim3(t.teams * t.warps * 32), shared, stream, 1u, p, t);
 }
 
-template <typename T, typename P, bool kEdge>
-cudaError_t launch_edge(const LayernormParams &p, const Shape &s, bool backward, cudaStream_t stream)
+// Whether some row has elements that are not in whole pieces.
+template <typename T>
+bool has_edges(const LayernormParams &p, const Teams &t)
 {
-    if (s.warp) {
-        return s.pieces == 1   ? launch_shape<T, P, 1, kEdge, true>(p, s, backward, stream)
-               : s.pieces == 2 ? launch_shape<T, P, 2, kEdge, true>(p, s, backward, stream)
-                               : launch_shape<T, P, 4, kEdge, true>(p, s, backward, stream);
+    return t.period != 1 || (reinterpret_cast<uintptr_t>(p.x) & 15u) != 0 || p.axis % kPer<T> != 0;
+}
+
+template <typename T, typename P>
+cudaError_t launch_forward(const LayernormParams &p, int sm_count, cudaStream_t stream)
+{
+    Teams t;
+    int grid;
+    size_t shared;
+    if (!teams_of(p, sizeof(T), sizeof(P), sm_count, &t, &grid, &shared)) {
+        return launch_chained(layernorm_any_kernel<T, P>, dim3(static_cast<unsigned>(std::min<long long>(p.rows, 4ll * sm_count))), dim3(kMostThreads), 0,
+                              stream, 1u, p);
     }
-    return s.pieces == 2 ? launch_shape<T, P, 2, kEdge, false>(p, s, backward, stream) : launch_shape<T, P, 4, kEdge, false>(p, s, backward, stream);
+    return launch_teams(has_edges<T>(p, t) ? layernorm_kernel<T, P, true> : layernorm_kernel<T, P, false>, p, t, grid, shared, stream);
+}
+
+template <typename T, typename P>
+cudaError_t launch_backward(const LayernormParams &p, int sm_count, cudaStream_t stream)
+{
+    Teams t;
+    int pieces, grid;
+    size_t shared;
+    cudaError_t e;
+    if (backward_teams_of(p, sizeof(T), sizeof(P), sm_count, &t, &pieces, &grid, &shared)) {
+        const bool edges = has_edges<T>(p, t);
+        void (*kernel)(LayernormParams, Teams) = edges ? layernorm_backward_kernel<T, P, 4, true> : layernorm_backward_kernel<T, P, 4, false>;
+        if (pieces == 1) {
+            kernel = edges ? layernorm_backward_kernel<T, P, 1, true> : layernorm_backward_kernel<T, P, 1, false>;
+        } else if (pieces == 2) {
+            kernel = edges ? layernorm_backward_kernel<T, P, 2, true> : layernorm_backward_kernel<T, P, 2, false>;
+        }
+        if constexpr (sizeof(T) == 4) {
+            if (pieces == 8) {
+                kernel = edges ? layernorm_backward_kernel<T, P, 8, true> : layernorm_backward_kernel<T, P, 8, false>;
+            }
+        }
+        e = launch_teams(kernel, p, t, grid, shared, stream);
+    } else {
+        grid = static_cast<int>(std::min<long long>(p.rows, kMostParts));
+        e = launch_chained(layernorm_backward_any_kernel<T, P>, dim3(grid), dim3(kMostThreads), 0, stream, 1u, p);
+    }
+    if (e != cudaSuccess || p.partial == nullptr) {
+        return e;
+    }
+    return launch_chained(column_sums_kernel<P>, dim3((p.axis + 31) / 32, 2), dim3(256), 0, stream, 1u, p, grid);
 }
 
 template <typename T, typename P>
 cudaError_t launch_typed(const LayernormParams &p, int sm_count, bool backward, cudaStream_t stream)
 {
-    Shape s;
-    cudaError_t e;
-    if (shape_of(p, sizeof(T), sizeof(P), backward, sm_count, &s)) {
-        e = s.edge ? launch_edge<T, P, true>(p, s, backward, stream) : launch_edge<T, P, false>(p, s, backward, stream);
-    } else {
-        s.grid = static_cast<int>(std::min<long long>(p.rows, kMostParts));
-        e = launch_chained(backward ? layernorm_backward_any_kernel<T, P> : layernorm_any_kernel<T, P>, dim3(s.grid), dim3(kMostThreads), 0, stream, 1u, p);
-    }
-    if (e != cudaSuccess || !backward || p.partial == nullptr) {
-        return e;
-    }
-    return launch_chained(column_sums_kernel<P>, dim3((p.axis + 31) / 32, 2), dim3(256), 0, stream, 1u, p, s.grid);
+    return backward ? launch_backward<T, P>(p, sm_count, stream) : launch_forward<T, P>(p, sm_count, stream);
 }
 
 cudaError_t launch(const LayernormParams &p, int sm_count, bool backward, cudaStream_t stream)

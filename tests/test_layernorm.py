@@ -70,8 +70,10 @@ def backward(x, dy, scale, mean, variance, out=None, wanted=(True, True, True), 
     desc = kb.make_layernorm_desc(rows, axis, CODE[x.dtype], param_dtype=CODE[kind], has_scale=scale is not None, given_stats=given, eps=eps,
                                   x_ld=x.stride(0), dy_ld=dy.stride(0), dx_ld=dx.stride(0))
     size = kb.layernorm_backward_workspace(desc)
-    space = torch.full((max(size, 4) // 4,), float("nan"), device="cuda")
+    space = torch.full((size // 4 + 3 * axis + 64,), float("nan"), device="cuda")
     kb.layernorm_backward(desc, x, dy, scale, mean, variance, *[t if w else None for t, w in zip((dx, dscale, dshift), wanted)], space, size, stream=stream)
+    if stream is None:
+        assert bool(torch.isnan(space[size // 4:]).all()), "written beyond the workspace"
     return dx, dscale, dshift
 
 
