@@ -161,15 +161,32 @@ __device__ __forceinline__ float2 block_sum(float a, float b, float2 (*scratch)[
     return make_float2(warp_sum(s.x), warp_sum(s.y));
 }
 
-// kPer<T> values of P from shared memory, 16 bytes at a time
+// Scale and shift in shared memory: where 16 bytes of a row's type hold more elements than 16 bytes of theirs, the first halves of all pieces'
+// worth and behind them the second ones, so that a warp reads 16 bytes per lane side by side.
 template <typename T, typename P>
-__device__ __forceinline__ void fetch(const P *from, int c, Two (&v)[kPer<T> / 2])
+__device__ __forceinline__ int param_slot(int i, int whole)
+{
+    constexpr int kReads = kPer<T> / kPer<P>;
+    return kReads == 1 ? i : i % kPer<T> / kPer<P> * (whole * kPer<P>) + i / kPer<T> * kPer<P> + i % kPer<P>;
+}
+
+template <typename T, typename P>
+__device__ __forceinline__ void stage_params(P *to, const void *from, int head, int whole, float none)
+{
+    for (int i = static_cast<int>(threadIdx.x); i < whole * kPer<T>; i += static_cast<int>(blockDim.x)) {
+        to[param_slot<T, P>(i, whole)] = from != nullptr ? static_cast<const P *>(from)[head + i] : narrow<P>(none);
+    }
+}
+
+// kPer<T> values of P, those of piece c
+template <typename T, typename P>
+__device__ __forceinline__ void fetch(const P *from, int c, int whole, Two (&v)[kPer<T> / 2])
 {
     constexpr int kReads = kPer<T> / kPer<P>, kPairs = kPer<P> / 2;
 #pragma unroll
     for (int i = 0; i < kReads; ++i) {
         Two part[kPairs];
-        unpack<P>(reinterpret_cast<const uint4 *>(from)[c * kReads + i], part);
+        unpack<P>(reinterpret_cast<const uint4 *>(from)[i * whole + c], part);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
             v[(i * kPairs + j) % (kPer<T> / 2)] = part[j];
@@ -277,10 +294,8 @@ __global__ void __launch_bounds__(kMostThreads, 2) layernorm_kernel(const __grid
         own_scale = p.scale != nullptr ? widen<P>(static_cast<const P *>(p.scale)[at]) : 1.0f;
         own_shift = p.shift != nullptr ? widen<P>(static_cast<const P *>(p.shift)[at]) : 0.0f;
     }
-    for (int i = static_cast<int>(threadIdx.x); i < slots; i += static_cast<int>(blockDim.x)) {
-        scale[i] = p.scale != nullptr ? static_cast<const P *>(p.scale)[head + i] : narrow<P>(1.0f);
-        shift[i] = p.shift != nullptr ? static_cast<const P *>(p.shift)[head + i] : narrow<P>(0.0f);
-    }
+    stage_params<T, P>(scale, p.scale, head, whole, 1.0f);
+    stage_params<T, P>(shift, p.shift, head, whole, 0.0f);
     __syncthreads();
     int turn = 0;
     const float inv_axis = 1.0f / static_cast<float>(p.axis);
@@ -341,8 +356,8 @@ __global__ void __launch_bounds__(kMostThreads, 2) layernorm_kernel(const __grid
         for (int c = lane; c < whole; c += lanes) {
             Two v[kV / 2], a[kV / 2], b[kV / 2];
             unpack<T>(x[c], v);
-            fetch<T, P>(scale, c, a);
-            fetch<T, P>(shift, c, b);
+            fetch<T, P>(scale, c, whole, a);
+            fetch<T, P>(shift, c, whole, b);
 #pragma unroll
             for (int j = 0; j < kV / 2; ++j) {
                 v[j] = fma(mul(add(v[j], less), times), a[j], b[j]);
@@ -464,9 +479,7 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const 
             sum_scale[i][j] = sum_shift[i][j] = 0ull;
         }
     }
-    for (int i = static_cast<int>(threadIdx.x); i < slots; i += static_cast<int>(blockDim.x)) {
-        scale[i] = p.scale != nullptr ? static_cast<const P *>(p.scale)[head + i] : narrow<P>(1.0f);
-    }
+    stage_params<T, P>(scale, p.scale, head, whole, 1.0f);
     __syncthreads();
     const float inv_axis = 1.0f / static_cast<float>(p.axis);
     int turn = 0, stage = 0;
@@ -494,7 +507,7 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const 
                 Two xh[kH], d[kH], a[kH];
                 unpack<T>(x[c], xh);
                 unpack<T>(dy[c], d);
-                fetch<T, P>(scale, c, a);
+                fetch<T, P>(scale, c, whole, a);
 #pragma unroll
                 for (int j = 0; j < kH; ++j) {
                     xh[j] = mul(add(xh[j], less), times);
@@ -536,7 +549,7 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const 
                         Two a[kH];
                         unpack<T>(x[c], xh);
                         unpack<T>(dy[c], g);
-                        fetch<T, P>(scale, c, a);
+                        fetch<T, P>(scale, c, whole, a);
 #pragma unroll
                         for (int j = 0; j < kH; ++j) {
                             xh[j] = mul(add(xh[j], less), times);
@@ -714,11 +727,13 @@ bool teams_of(const LayernormParams &p, int elem, int param_elem, int sm_count, 
     if (2 * bytes > most) {
         return false;
     }
+    // sixteen warps per CTA with as many teams as shared memory has room for; with few rows, a piece per lane
+    const long long room = std::max<long long>(1, most / (2 * bytes));
     int warps = 1;
-    while (warps < 16 && (bytes > warps * 8192ll || (p.rows <= 2ll * sm_count && bytes > warps * 512ll))) {
-        warps *= 2;  // 256 bytes per lane, or with few rows one piece
+    while (warps < 16 && (warps * room < 16 || (p.rows <= 2ll * sm_count && bytes > warps * 512ll))) {
+        warps *= 2;
     }
-    int teams = static_cast<int>(std::max<long long>(1, std::min<long long>(16 / warps, most / (2 * bytes))));
+    int teams = static_cast<int>(std::min<long long>(16 / warps, room));
     const long long need = (p.rows + sm_count - 1) / sm_count;
     while (teams > 1 && teams / 2 >= need) {
         teams /= 2;
