@@ -675,7 +675,19 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant_
     float s = 0.0f;
     if (e < p.axis) {
         const float *from = p.partial + static_cast<long long>(blockIdx.y) * p.axis + e;
-        for (int i = warp; i < parts; i += 8) {
+        int i = warp;
+        for (; i + 56 < parts; i += 64) {  // eight loads at a time
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = from[static_cast<long long>(i + 8 * j) * 2 * p.axis];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s += v[j];
+            }
+        }
+        for (; i < parts; i += 8) {
             s += from[static_cast<long long>(i) * 2 * p.axis];
         }
     }
@@ -756,8 +768,7 @@ bool backward_teams_of(const LayernormParams &p, int elem, int param_elem, int s
     }
     const long long bytes = (static_cast<long long>(p.axis) * elem + 15) / 16 * 16, whole = bytes / 16;
     const long long params = (static_cast<long long>(p.axis) * param_elem + 15) / 16 * 16;
-    const int usual = elem == 4 ? 4 : 2;  // 16 elements per thread
-    *pieces = whole <= 32 ? 1 : whole <= 64 ? 2 : whole <= usual * kMostThreads ? usual : 2 * usual;
+    *pieces = whole <= 32 ? 1 : whole <= 64 ? 2 : whole <= 4 * kMostThreads || elem != 4 ? 4 : 8;
     const long long warps = (whole + *pieces * 32 - 1) / (*pieces * 32);
     if (warps * 32 > kMostThreads) {
         return false;
