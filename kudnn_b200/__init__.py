@@ -15,7 +15,7 @@ from .capi import (  # noqa: F401
     NORM_USE_GLOBAL_STATS, NORM_USE_SCALE, SHARD_COLS, SHARD_ROWS,
     SCALE_BLOCK, Grouped, GroupedDesc, QuantizeDesc, make_grouped_desc, make_quantize_desc, quantize,
     LayernormDesc, layernorm, layernorm_backward, layernorm_backward_workspace, make_layernorm_desc,
-    SCORE_SIGMOID, SCORE_SOFTMAX, ExpertsDesc, RouteDesc, experts, experts_workspace, make_experts_desc, make_route_desc, route,
+    SCORE_SIGMOID, SCORE_SOFTMAX, ExpertsDesc, RouteDesc, experts, experts_check, experts_set_wait, experts_workspace, make_experts_desc, make_route_desc, route,
 )
 
 __all__ = [
@@ -28,5 +28,5 @@ __all__ = [
     "NORM_USE_GLOBAL_STATS", "NORM_USE_SCALE", "SHARD_COLS", "SHARD_ROWS",
     "SCALE_BLOCK", "Grouped", "GroupedDesc", "QuantizeDesc", "make_grouped_desc", "make_quantize_desc", "quantize",
     "LayernormDesc", "layernorm", "layernorm_backward", "layernorm_backward_workspace", "make_layernorm_desc",
-    "SCORE_SIGMOID", "SCORE_SOFTMAX", "ExpertsDesc", "RouteDesc", "experts", "experts_workspace", "make_experts_desc", "make_route_desc", "route",
+    "SCORE_SIGMOID", "SCORE_SOFTMAX", "ExpertsDesc", "RouteDesc", "experts", "experts_check", "experts_set_wait", "experts_workspace", "make_experts_desc", "make_route_desc", "route",
 ]

@@ -150,7 +150,7 @@ EXPORTS = [
     "kudnn_b200_layernorm_validate", "kudnn_b200_layernorm_run", "kudnn_b200_layernorm_backward_workspace",
     "kudnn_b200_layernorm_backward_run",
     "kudnn_b200_route_validate", "kudnn_b200_route_run", "kudnn_b200_experts_validate", "kudnn_b200_experts_workspace",
-    "kudnn_b200_experts_run",
+    "kudnn_b200_experts_run", "kudnn_b200_experts_check", "kudnn_b200_experts_set_wait",
 ]
 
 _lib = None
@@ -223,6 +223,8 @@ def library():
     lib.kudnn_b200_experts_validate.argtypes = [ctypes.POINTER(ExpertsDesc)]
     lib.kudnn_b200_experts_workspace.argtypes = [ctypes.POINTER(ExpertsDesc), ctypes.POINTER(i64)]
     lib.kudnn_b200_experts_run.argtypes = [ctypes.POINTER(ExpertsDesc), ctypes.POINTER(ExpertsArgs), vp]
+    lib.kudnn_b200_experts_check.argtypes = [vp]
+    lib.kudnn_b200_experts_set_wait.argtypes = [ctypes.c_longlong, i32]
     lib.kudnn_b200_last_error.restype = ctypes.c_char_p
     lib.kudnn_b200_version.restype = ctypes.c_char_p
     _lib = lib
@@ -509,6 +511,16 @@ def experts(desc, x, weights, ids, gate_up, down, y, workspace, workspace_bytes,
     args = ExpertsArgs(_ptr(x), _ptr(weights), _ptr(ids), _ptr(gate_up), _ptr(down), _ptr(gate_up_scale), _ptr(down_scale), _ptr(y),
                        _ptr(workspace), workspace_bytes)
     _check(library().kudnn_b200_experts_run(ctypes.byref(desc), ctypes.byref(args), stream))
+
+
+def experts_check(stream=None):
+    """Raises KudnnError (TIMEOUT) if a device-side wait of experts has given up on the current device since the last check."""
+    _check(library().kudnn_b200_experts_check(stream))
+
+
+def experts_set_wait(wait_limit_cycles=0, skip_step=-1):
+    """Test hook: limit of the device-side waits in SM cycles, and the step of K from which on no weights are copied."""
+    _check(library().kudnn_b200_experts_set_wait(wait_limit_cycles, skip_step))
 
 
 def debug_fail_allocation(nth):

@@ -238,4 +238,34 @@ int kudnn_b200_experts_run(const kudnn_b200_experts_desc *d, const kudnn_b200_ex
     return e == cudaSuccess ? KUDNN_B200_OK : fail_cuda(e, "experts kernel launch");
 }
 
+int kudnn_b200_experts_check(void *cuda_stream)
+{
+    int sms = 0;
+    const int rc = current_device(&sms);
+    if (rc != KUDNN_B200_OK) {
+        return rc;
+    }
+    kb::DeviceStatus st;
+    cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(cuda_stream));
+    if (e == cudaSuccess) e = kb::experts_take_status(&st);
+    if (e != cudaSuccess) {
+        return fail_cuda(e, "experts: check");
+    }
+    if (st.code != kb::kErrNone) {
+        char text[120];
+        std::snprintf(text, sizeof(text), "device-side wait gave up (site %d, block %d)", st.where, st.block);
+        return fail(KUDNN_B200_TIMEOUT, text);
+    }
+    return KUDNN_B200_OK;
+}
+
+int kudnn_b200_experts_set_wait(long long wait_limit_cycles, int skip_step)
+{
+    if (wait_limit_cycles < 0) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "experts: the limit of a wait is not negative");
+    }
+    kb::experts_set_wait(wait_limit_cycles, skip_step);
+    return KUDNN_B200_OK;
+}
+
 }  // extern "C"

@@ -883,7 +883,7 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
     if (gave_up) {
         // the copies that are still on their way, each for a moment
         for (int i = 0; i < stages; ++i) {
-            for (int spin = 0; spin < 100000 && !mbar_try_wait(full + i, parity ^ (i < stage ? 1u : 0u)); ++spin) {
+            for (int spin = 0; spin < 2000 && !mbar_try_wait(full + i, parity ^ (i < stage ? 1u : 0u)); ++spin) {
             }
         }
     }

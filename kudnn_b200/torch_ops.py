@@ -1,5 +1,5 @@
-"""PyTorch glue over the C ABI: the custom operators ``kudnn_b200::linear``, ``::quantize`` and ``::grouped``, a drop-in module for
-``nn.Linear`` and a feed-forward block of experts.
+"""PyTorch glue over the C ABI: the custom operators ``kudnn_b200::linear``, ``::quantize``, ``::grouped``, ``::layernorm``, ``::route`` and
+``::experts``, drop-in modules for ``nn.Linear`` and ``nn.LayerNorm`` and a feed-forward block of experts.
 
 The reference reaches PyTorch through a patched build in which ``torch._C._set_kdnn_enabled(True)`` routes
 ``torch.nn.Linear`` to KuDNN (docs/zh/KuDNN_development_guide.md:1407-1486, 1748-1775).  Here the same dispatch point
@@ -287,6 +287,88 @@ def _grouped_fake(x, weight, offsets=None, x_scale=None, weight_scale=None, bias
     return x.new_empty((x.shape[0], weight.shape[-2]), dtype=out_dtype)
 
 
+# ---- a router and a block of experts for few tokens
+
+SCORES = {"softmax": capi.SCORE_SOFTMAX, "sigmoid": capi.SCORE_SIGMOID}
+MOST_FEW_TOKENS, MOST_FEW_TOP = 64, 16
+
+
+@torch.library.custom_op("kudnn_b200::route", mutates_args=(), device_types="cuda")
+def route(x: torch.Tensor, router: torch.Tensor, top: int, bias: Optional[torch.Tensor] = None, score: str = "softmax", normalise: bool = True,
+          scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [tokens, hidden], router [experts, hidden] -> (weights [tokens, top] float32, ids [tokens, top] int32), the largest score first.
+
+    Scores are a softmax or a sigmoid of x . router^T, computed in 64 bits.  bias [experts] float32 is added to them for the choice alone; minus
+    infinity takes an expert out.  With `normalise` a token's weights are divided by their sum, then multiplied by `scale`.  Places that no
+    expert is left for have the id -1 and the weight 0."""
+    if x.dtype not in _DTYPES or router.dtype not in _DTYPES:
+        raise TypeError("kudnn_b200::route takes float32 / float16 / bfloat16 tokens and routers")
+    if x.dim() != 2 or router.dim() != 2 or x.shape[1] != router.shape[1] or router.device != x.device:
+        raise ValueError("kudnn_b200::route: x [tokens, hidden] and router [experts, hidden] on one device do not match")
+    if score not in SCORES:
+        raise ValueError("kudnn_b200::route: scores are softmax or sigmoid")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != router.shape[:1] or bias.device != x.device):
+        raise ValueError("kudnn_b200::route: bias is a float32 vector of the experts on the device of x")
+    x, router = [t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous() for t in (x, router)]
+    tokens = x.shape[0]
+    weights = torch.empty((tokens, top), dtype=torch.float32, device=x.device)
+    ids = torch.empty((tokens, top), dtype=torch.int32, device=x.device)
+    desc = capi.make_route_desc(tokens, router.shape[0], x.shape[1], top, _DTYPES[x.dtype], router_dtype=_DTYPES[router.dtype], score=SCORES[score],
+                                normalise=normalise, scale=scale, x_ld=x.stride(0), w_ld=router.stride(0))
+    with _on(x.device):
+        capi.route(desc, x, router, weights, ids, None if bias is None else bias.contiguous(), stream=torch.cuda.current_stream(x.device).cuda_stream)
+    return weights, ids
+
+
+@route.register_fake
+def _route_fake(x, router, top, bias=None, score="softmax", normalise=True, scale=1.0):
+    return x.new_empty((x.shape[0], top), dtype=torch.float32), x.new_empty((x.shape[0], top), dtype=torch.int32)
+
+
+@torch.library.custom_op("kudnn_b200::experts", mutates_args=(), device_types="cuda")
+def experts(x: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
+            gate_up_scale: Optional[torch.Tensor] = None, down_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] = sum over j of weights[t, j] * down[e](silu(gate[e](x[t])) * up[e](x[t])), e = ids[t, j], for at most 64 tokens.
+
+    x [tokens, hidden] float16 or bfloat16; weights float32 and ids int32 [tokens, top] as route gives them; gate_up [experts, 2 ffn, hidden] and
+    down [experts, hidden, ffn] of x's type, or float8_e4m3fn with float32 scales per 128 x 128."""
+    if x.dtype not in (torch.float16, torch.bfloat16) or gate_up.dtype not in (x.dtype, torch.float8_e4m3fn) or down.dtype != gate_up.dtype:
+        raise TypeError("kudnn_b200::experts takes float16 or bfloat16 tokens and weights of that type or of float8_e4m3fn")
+    if x.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[1] % 2 != 0 or \
+            down.shape != (gate_up.shape[0], gate_up.shape[2], gate_up.shape[1] // 2) or x.shape[1] != gate_up.shape[2]:
+        raise ValueError("kudnn_b200::experts: x [tokens, hidden], gate_up [experts, 2 * ffn, hidden] and down [experts, hidden, ffn] do not match")
+    (tokens, hidden), (count, ffn) = x.shape, (gate_up.shape[0], down.shape[2])
+    if weights.dtype != torch.float32 or ids.dtype != torch.int32 or weights.dim() != 2 or weights.shape != ids.shape or ids.shape[0] != tokens:
+        raise ValueError("kudnn_b200::experts: weights float32 and ids int32 are [tokens, top]")
+    inner, outer = -(-ffn // capi.SCALE_BLOCK), -(-hidden // capi.SCALE_BLOCK)
+    shapes = ((count, -(-2 * ffn // capi.SCALE_BLOCK), outer), (count, outer, inner))
+    for scale, shape in zip((gate_up_scale, down_scale), shapes):
+        if (scale is not None) != (gate_up.dtype == torch.float8_e4m3fn) or (scale is not None and (scale.dtype != torch.float32 or scale.shape != shape)):
+            raise ValueError("kudnn_b200::experts: e4m3 weights need float32 scales per 128 x 128, others take none")
+    for other in (weights, ids, gate_up, down, gate_up_scale, down_scale):
+        if other is not None and other.device != x.device:
+            raise ValueError("kudnn_b200::experts: all tensors lie on one device")
+    if x.stride(1) != 1 and hidden > 1:
+        x = x.contiguous()
+    y = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device)
+    desc = capi.make_experts_desc(tokens, hidden, ffn, count, ids.shape[1], _DTYPES[x.dtype], weight_dtype=_OPERANDS[gate_up.dtype],
+                                  x_ld=x.stride(0) if tokens > 1 else hidden, gate_up_strides=gate_up.stride(), down_strides=down.stride(),
+                                  gate_up_scale_strides=None if gate_up_scale is None else gate_up_scale.stride(),
+                                  down_scale_strides=None if down_scale is None else down_scale.stride())
+    size = capi.experts_workspace(desc)
+    # scratch of this call alone: calls on other streams and in graphs have theirs
+    space = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        capi.experts(desc, x, weights.contiguous(), ids.contiguous(), gate_up, down, y, space, size, gate_up_scale, down_scale,
+                     stream=torch.cuda.current_stream(x.device).cuda_stream)
+    return y
+
+
+@experts.register_fake
+def _experts_fake(x, weights, ids, gate_up, down, gate_up_scale=None, down_scale=None):
+    return x.new_empty(x.shape)
+
+
 class Experts(torch.nn.Module):
     """Feed-forward block of experts (inference): every token goes to `top` experts, and what they answer is added up by weight.
 
@@ -294,14 +376,19 @@ class Experts(torch.nn.Module):
 
     p: softmax of the router's logits, the `top` largest made to sum to one.  gate_up [experts, 2 * ffn, hidden] holds gate's rows, then
     up's; down [experts, hidden, ffn].  With eight_bit the weights are kept as e4m3 with a scale per 128 x 128 block, the tokens are
-    quantised on their way to the experts and the gated values between the two products.  Nothing is read back to the host."""
+    quantised on their way to the experts and the gated values between the two products.  Nothing is read back to the host.
 
-    def __init__(self, router, gate_up, down, top, eight_bit=False):
+    few: calls of 16-bit tokens, at most so many (64, and a top of 16, at most), go through ``route`` and ``experts`` instead, three launches in
+    all, which read each chosen expert's weights once and quantise nothing but the weights."""
+
+    def __init__(self, router, gate_up, down, top, eight_bit=False, few=0):
         super().__init__()
         if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[1] != 2 * down.shape[2] or gate_up.shape[2] != down.shape[1] or \
                 router.shape != (gate_up.shape[0], gate_up.shape[2]) or not 1 <= top <= gate_up.shape[0]:
             raise ValueError("Experts: router [experts, hidden], gate_up [experts, 2 * ffn, hidden] and down [experts, hidden, ffn] do not match")
-        self.top, self.eight_bit = top, eight_bit
+        if not 0 <= few <= MOST_FEW_TOKENS or (few > 0 and top > MOST_FEW_TOP):
+            raise ValueError("Experts: few is at most 64, and with it top at most 16")
+        self.top, self.eight_bit, self.few = top, eight_bit, few
         self.register_buffer("router", router.float())
         for name, w in (("gate_up", gate_up), ("down", down)):
             if eight_bit:
@@ -338,6 +425,10 @@ class Experts(torch.nn.Module):
         tokens = x.reshape(-1, x.shape[-1])
         count, experts = tokens.shape[0], self.router.shape[0]
         ops = torch.ops.kudnn_b200
+        if count <= self.few and x.dtype in (torch.float16, torch.bfloat16) and (self.eight_bit or self.gate_up.dtype == x.dtype):
+            p, chosen = ops.route(tokens, self.router, self.top)
+            scales = (self.gate_up_scale, self.down_scale) if self.eight_bit else (None, None)
+            return ops.experts(tokens, p, chosen, self.gate_up, self.down, *scales).view(x.shape)
         p, chosen = torch.topk(torch.softmax(ops.linear(tokens.float(), self.router), dim=1), self.top, dim=1)
         p = p / p.sum(dim=1, keepdim=True)
         # rows sorted by expert; a stable sort keeps the tokens of an expert in order
@@ -357,3 +448,120 @@ class Experts(torch.nn.Module):
         back[order] = torch.arange(order.shape[0], device=x.device)
         y = (y[back].view(count, self.top, tokens.shape[1]).float() * p[:, :, None]).sum(dim=1)
         return y.to(x.dtype).view(x.shape)
+
+
+# ---- layer normalisation
+
+
+def _rows(t):
+    """[..., axis] as rows with contiguous elements."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _layernorm_desc(x, param, has_scale, has_shift, eps, dy=None):
+    rows, axis = x.shape
+
+    def pitch(t):
+        return t.stride(0) if rows > 1 else axis
+
+    return capi.make_layernorm_desc(rows, axis, _DTYPES[x.dtype], param_dtype=_DTYPES[x.dtype if param is None else param.dtype],
+                                    has_scale=has_scale, has_shift=has_shift, eps=eps, x_ld=pitch(x), dy_ld=None if dy is None else pitch(dy))
+
+
+def _check_layernorm(x, scale, shift):
+    if x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] == 0:
+        raise TypeError("kudnn_b200::layernorm takes float32 / float16 / bfloat16 rows")
+    for t in (scale, shift):
+        if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32) or t.device != x.device):
+            raise ValueError("kudnn_b200::layernorm: scale and shift are vectors of the last axis, float32 or of x's type, on its device")
+    if scale is not None and shift is not None and scale.dtype != shift.dtype:
+        raise ValueError("kudnn_b200::layernorm: scale and shift are of one type")
+
+
+@torch.library.custom_op("kudnn_b200::layernorm", mutates_args=(), device_types="cuda")
+def layernorm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
+              eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(x - mean) / sqrt(variance + eps) * scale + shift over the last axis, with the mean and the variance of every row (float32).
+
+    scale, shift: float32 or of x's type.  Differentiable with respect to x, scale and shift (the first result's gradient only)."""
+    _check_layernorm(x, scale, shift)
+    rows = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, variance = [torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2)]
+    desc = _layernorm_desc(rows, scale if scale is not None else shift, scale is not None, shift is not None, eps)
+    with _on(x.device):
+        capi.layernorm(desc, rows, y, None if scale is None else scale.contiguous(), None if shift is None else shift.contiguous(), mean, variance,
+                       stream=torch.cuda.current_stream(x.device).cuda_stream)
+    return y, mean, variance
+
+
+@layernorm.register_fake
+def _layernorm_fake(x, scale=None, shift=None, eps=1e-5):
+    return x.new_empty(x.shape), x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op("kudnn_b200::layernorm_backward", mutates_args=(), device_types="cuda")
+def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, scale: Optional[torch.Tensor], mean: torch.Tensor, variance: torch.Tensor,
+                       eps: float, param_dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of layernorm's x, scale and shift, the latter two of param_dtype."""
+    _check_layernorm(x, scale, None)
+    if dy.shape != x.shape or dy.dtype != x.dtype or mean.shape != x.shape[:-1] or variance.shape != mean.shape or \
+            mean.dtype != torch.float32 or variance.dtype != torch.float32 or (scale is not None and scale.dtype != param_dtype):
+        raise ValueError("kudnn_b200::layernorm_backward: dy, mean and variance do not match x")
+    rows, dy_rows = _rows(x), _rows(dy)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dscale, dshift = [torch.empty(x.shape[-1:], dtype=param_dtype, device=x.device) for _ in range(2)]
+    desc = _layernorm_desc(rows, dscale, scale is not None, False, eps, dy=dy_rows)
+    size = capi.layernorm_backward_workspace(desc)
+    space = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        capi.layernorm_backward(desc, rows, dy_rows, None if scale is None else scale.contiguous(), mean.contiguous(), variance.contiguous(), dx, dscale,
+                                dshift, space, size, stream=torch.cuda.current_stream(x.device).cuda_stream)
+    return dx, dscale, dshift
+
+
+@layernorm_backward.register_fake
+def _layernorm_backward_fake(dy, x, scale, mean, variance, eps, param_dtype):
+    return x.new_empty(x.shape), x.new_empty(x.shape[-1:], dtype=param_dtype), x.new_empty(x.shape[-1:], dtype=param_dtype)
+
+
+def _layernorm_context(ctx, inputs, output):
+    x, scale, shift, eps = inputs
+    _, mean, variance = output
+    ctx.mark_non_differentiable(mean, variance)
+    ctx.save_for_backward(x, scale, mean, variance)
+    ctx.eps, ctx.param_dtype, ctx.with_scale, ctx.with_shift = eps, (scale if scale is not None else shift if shift is not None else x).dtype, \
+        scale is not None, shift is not None
+
+
+def _layernorm_gradient(ctx, dy, _mean, _variance):
+    x, scale, mean, variance = ctx.saved_tensors
+    dx, dscale, dshift = torch.ops.kudnn_b200.layernorm_backward(dy, x, scale, mean, variance, ctx.eps, ctx.param_dtype)
+    return dx, dscale if ctx.with_scale else None, dshift if ctx.with_shift else None, None
+
+
+layernorm.register_autograd(_layernorm_gradient, setup_context=_layernorm_context)
+
+
+class LayerNorm(torch.nn.Module):
+    """``nn.LayerNorm`` over the last axis through ``kudnn_b200::layernorm``, forward and backward:  ``LayerNorm.from_torch(layer)(x)``.
+
+    As with every autograd function of torch: while a backward pass is captured into a CUDA graph, no eager graph of the same parameters may be
+    alive (delete its results first), or torch's own accumulation of gradients waits for a stream that is not captured."""
+
+    def __init__(self, axis, eps=1e-5, bias=True, device=None, dtype=None):
+        super().__init__()
+        self.inner = torch.nn.LayerNorm(axis, eps=eps, bias=bias, device=device, dtype=dtype)
+
+    @classmethod
+    def from_torch(cls, layer):
+        if len(layer.normalized_shape) != 1:
+            raise ValueError("LayerNorm: one axis, the last")
+        mod = cls.__new__(cls)
+        torch.nn.Module.__init__(mod)
+        mod.inner = layer
+        return mod
+
+    def forward(self, x):
+        return torch.ops.kudnn_b200.layernorm(x, self.inner.weight, self.inner.bias, self.inner.eps)[0]
