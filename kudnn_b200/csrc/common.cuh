@@ -316,7 +316,8 @@ __device__ __forceinline__ void epilogue_scalar(const EpiParams &p, float acc, l
 
 // ---- programmatic dependent launch
 // The tensor-core kernels (tc_linear_kernel, tc_wide_kernel, tc_planes_kernel), the streaming kernels, simt_small_kernel,
-// pack_rows_kernel, split_rows_kernel, split_rows_if_kernel, split_half_kernel, grouped_tc_kernel and the quantize kernels let the next kernel
+// pack_rows_kernel, split_rows_kernel, split_rows_if_kernel, split_half_kernel, grouped_tc_kernel, the quantize, layernorm and route kernels
+// and those of the experts for few tokens let the next kernel
 // on their stream be set up while they still run, and wait for their predecessor before they touch memory that it may write;
 // what they do earlier (barriers, tensor memory, descriptors, weights in copies that the handle owns) depends on no kernel.  The
 // other kernels of the library do neither.  Takes 2-4 us off a call that follows another one.

@@ -324,7 +324,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) route_many_kernel(const __gri
 template <typename X, typename W>
 cudaError_t launch_typed(const RouteParams &p, cudaStream_t stream)
 {
-    if (p.tokens > 256) {
+    // x 64 experts x 4096: 64, 256, 512 and 1024 tokens 9, 24, 40 and 71 us by the first kernel, 51 (256) to 57 (1024) by the second; x 128
+    // experts 14, 39, 64, 114 and 99 to 101
+    if (p.tokens > 768) {
         const size_t shared = sizeof(double) * kTile * p.experts;
         const cudaError_t e = cudaFuncSetAttribute(route_many_kernel<X, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    static_cast<int>(sizeof(double)) * kTile * kMostExperts);

@@ -103,7 +103,8 @@ class Block:
 # tokens, experts, top, hidden, ffn
 SIZES = [(1, 1, 1, 8, 8), (1, 4, 2, 64, 32), (2, 3, 3, 16, 1), (3, 8, 2, 40, 24), (5, 6, 2, 300, 200), (1, 8, 8, 1024, 704), (8, 8, 2, 2048, 136),
          (9, 16, 4, 512, 384), (17, 16, 3, 301, 203), (33, 32, 8, 1024, 352), (64, 8, 2, 520, 136), (64, 60, 6, 640, 1408), (2, 128, 8, 4096, 256),
-         (64, 1, 1, 256, 2048), (40, 200, 16, 128, 64), (12, 4, 2, 5120, 96), (4, 1000, 16, 64, 72)]
+         (64, 1, 1, 256, 2048), (40, 200, 16, 128, 64), (12, 4, 2, 5120, 96), (4, 1000, 16, 64, 72),
+         (35, 3, 2, 9536, 16), (3, 2, 1, 4784, 24), (64, 5, 3, 2376, 40), (9, 2, 2, 2360, 64)]
 
 
 @gpu

@@ -55,6 +55,7 @@ def operands(tokens, experts, hidden, dtype, router, seed=0):
 
 SIZES = [(1, 1, 1, 1), (1, 2, 7, 2), (3, 8, 64, 3), (5, 9, 130, 4), (4, 60, 511, 6), (33, 64, 4096, 8), (2, 128, 2050, 64), (130, 33, 1000, 5),
          (257, 5, 33, 2), (300, 64, 1000, 8), (271, 150, 130, 64), (513, 1024, 70, 3),
+         (769, 5, 33, 2), (800, 64, 1000, 8), (783, 150, 130, 64), (801, 1024, 70, 3),
          (1, 256, 7168, 8), (6, 1000, 300, 64), (2, 1024, 128, 33)]
 
 
