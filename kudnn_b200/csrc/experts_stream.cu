@@ -900,15 +900,18 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
     Shape shape;
     shape.token_rows = std::min(8, p.tokens);
     shape.token_bytes = shape.token_rows * (kDown && kW != kF16 ? 2 : 1) * kTokenPitch;
-    shape.cluster = kDown && p.hidden <= 16 * sm_count ? 2 : 1;
-    const int fixed = 1024 + (kDown ? kWarps * p.tokens * kRows * 4 : kWarps * 1024) + Lists::bytes(p.experts, p.tokens * p.top);
+    // Two CTAs fit an SM where the registers suffice and half of its shared memory holds the rings.  With much to read both are this kernel's: 16
+    // warps hide the latency of their instructions better than 8 (1 token, 8 experts 4096 x 2048: 77 us, with 8 warps 86).  With little, the second
+    // place is the next kernel's, which is then set up while this one runs (2 experts 1024 x 704: 12.5 us, otherwise 14.9).
+    constexpr bool kHalves = kTokens == 1 && kW != kE4m3;
+    const long long most = 6ll * std::min(p.experts, p.tokens * p.top) * p.hidden * p.ffn;  // bytes of the experts that can be chosen
     const int stage = kWarps * (kStageBytes + shape.token_bytes);
-    // half of the SM, if that gives rings of three stages and the registers suffice
-    shape.stages = kTokens == 1 && kW != kE4m3 ? (kHalfShared - fixed) / stage : 0;
-    if (shape.stages < 3) {
-        shape.stages = (kMostShared - fixed) / stage;
-    }
-    shape.stages = std::min(shape.stages, kMostStages);
+    const int fixed = 1024 + (kDown ? kWarps * p.tokens * kRows * 4 : kWarps * 1024) + Lists::bytes(p.experts, p.tokens * p.top);
+    const int in_half = kHalves ? (kHalfShared - fixed) / stage : 0;
+    const bool two = most > 64ll << 20 && in_half >= 2;
+    const int ctas = two ? 2 * sm_count : sm_count;
+    shape.cluster = kDown && p.hidden <= 16 * ctas ? 2 : 1;
+    shape.stages = std::min(two || in_half >= 3 ? in_half : (kMostShared - fixed) / stage, kMostStages);
     const size_t shared = static_cast<size_t>(fixed) + static_cast<size_t>(shape.stages) * stage;
     alignas(64) CUtensorMap map;
     cudaError_t e = tc_encode_groups(&map, kDown ? p.down : p.gate_up, p.w_dtype, p.experts, kDown ? p.hidden : 2ll * p.ffn, kDown ? p.ffn : p.hidden,
@@ -919,7 +922,7 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
     const long long limit = wait_limit.load();
     const Waits waits = {limit > 0 ? limit : kDefaultWaitLimitCycles, wait_skip.load()};
     return e != cudaSuccess ? e
-                            : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(sm_count / shape.cluster * shape.cluster), dim3(kWarps * 32),
+                            : launch_chained(experts_stream_kernel<kW, kBf, kDown, kTokens>, dim3(ctas / shape.cluster * shape.cluster), dim3(kWarps * 32),
                                              shared, stream, shape.cluster, p, map, shape, waits);
 }
 
