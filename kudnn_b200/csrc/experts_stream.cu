@@ -13,8 +13,10 @@
 //     products and were bound by their latency; tokens loaded one step ahead were bound by L2's latency.
 //   * 16 bytes per lane, as they lie in the ring, are operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on
 //     that of 8, read in the same permutation.
-//   * For few tokens and 16-bit weights the CTAs take at most half of an SM's shared memory, so that the second kernel's are there while the first one runs: they make
-//     their lists, fill their rings, and wait only before they read h.
+//   * The second kernel's CTAs take the place of the first one's as those leave, or stand beside them where two fit an SM: they make their lists, fill
+//     their rings with weights, and wait only before they read h.
+// 1 token, 8 experts 4096 x 2048 of bf16: 77 us, 5.2 TB/s; 64 tokens, 120 experts 2048 x 768: 264 us, 4.3 TB/s; 14 tokens, 50 experts 4096 x 2048 of e4m3:
+// 310 us, 4.1 TB/s.  What is left is the latency of the instructions of a step (1 of 4 issue slots busy with 8 warps) and 5 us of start.
 // h is kept as the tensor cores take it without loss: two bf16 halves (of bf16 and e4m3 weights), or fp32 that the second kernel splits into two
 // tf32 halves (of fp16 weights: halves of fp16 would overflow beyond 65504 and lose small values).
 #include "experts.cuh"

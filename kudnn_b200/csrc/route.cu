@@ -5,7 +5,8 @@
 // Few tokens: a cluster of eight CTAs takes eight of them, each CTA an eighth of the experts, so that w is read by many SMs, K split between its warps.
 // The logits are gathered through distributed shared memory, and a warp finishes each token.  It is latency throughout: reading w once, two
 // cluster barriers, the choice.
-// Many tokens: a CTA takes sixteen, eight of its warps' and all experts 64 at a time, with K in quarters.
+// Many tokens: a CTA takes sixteen and all experts, 64 at a time, two warps side by side for each quarter of K.
+// 1 token x 64 experts x 4096: 7.8 us; 61 x 128 x 2048: 10.7 us; 4096 x 64 x 4096: 93 us, 23 TFLOP/s in 64 bits.
 #include "experts.cuh"
 
 #include <cooperative_groups.h>
