@@ -266,6 +266,27 @@ def test_streams_and_graphs(cuda_device):
         assert torch.equal(y, want[1])
 
 
+@gpu
+def test_calls_of_all_sizes_side_by_side(cuda_device):
+    """Launches that share SMs with their successors, of CTA pairs and of whole SMs, on four streams at once: the same bits as alone."""
+    sizes = [(1, 16, 8, 2048, 1408, False), (4, 16, 4, 1024, 2048, False), (64, 16, 4, 1024, 512, False), (12, 16, 4, 2048, 512, True)]
+    blocks = [Block(*size[:5], torch.bfloat16, size[5], seed=i) for i, size in enumerate(sizes)]
+    want = [block.run() for block in blocks]
+    for block, y in zip(blocks, want):
+        block.check(y)
+    spaces = [torch.empty(1 << 21, device="cuda") for _ in blocks]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in blocks]
+    for _ in range(15):
+        got = []
+        for block, s, space in zip(blocks, streams, spaces):
+            with torch.cuda.stream(s):
+                got.append([block.run(stream=s.cuda_stream, workspace=space) for _ in range(2)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for pair, w in zip(got, want) for g in pair)
+    kb.experts_check()
+
+
 def desc(**more):
     sizes = [more.pop(name, v) for name, v in (("tokens", 2), ("hidden", 16), ("ffn", 8), ("experts", 4), ("top", 2), ("dtype", kb.BF16))]
     return kb.make_experts_desc(*sizes, **more)
