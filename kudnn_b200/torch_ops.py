@@ -507,8 +507,10 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, scale: Optional[torch.
     """The gradients of layernorm's x, scale and shift, the latter two of param_dtype."""
     _check_layernorm(x, scale, None)
     if dy.shape != x.shape or dy.dtype != x.dtype or mean.shape != x.shape[:-1] or variance.shape != mean.shape or \
-            mean.dtype != torch.float32 or variance.dtype != torch.float32 or (scale is not None and scale.dtype != param_dtype):
-        raise ValueError("kudnn_b200::layernorm_backward: dy, mean and variance do not match x")
+            mean.dtype != torch.float32 or variance.dtype != torch.float32 or any(t.device != x.device for t in (dy, mean, variance)):
+        raise ValueError("kudnn_b200::layernorm_backward: dy, mean and variance do not match x or lie on another device")
+    if param_dtype not in (x.dtype, torch.float32) or (scale is not None and scale.dtype != param_dtype):
+        raise ValueError("kudnn_b200::layernorm_backward: scale and the gradients are of one type, float32 or that of x")
     rows, dy_rows = _rows(x), _rows(dy)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dscale, dshift = [torch.empty(x.shape[-1:], dtype=param_dtype, device=x.device) for _ in range(2)]

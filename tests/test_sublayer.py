@@ -32,6 +32,19 @@ def block(eight_bit, few, hidden=512, ffn=384, count=16, top=4, seed=0, dtype=to
     return torch_ops.Experts(router, gate_up, down, top, eight_bit=eight_bit, few=few), (router, gate_up, down, top)
 
 
+@pytest.mark.parametrize("wrong", [
+    dict(dy=torch.zeros(5, 300, dtype=torch.bfloat16)), dict(mean=torch.zeros(5)), dict(variance=torch.zeros(5)), dict(scale=torch.zeros(300)),
+    dict(x=torch.zeros(5, 300, dtype=torch.bfloat16)), dict(param_dtype=torch.float16), dict(param_dtype=torch.int32), dict(dy=meta(5, 299)),
+    dict(mean=meta(5)), dict(scale=meta(300)),
+])
+def test_gradients_across_devices_or_types_are_refused_before_any_launch(wrong):
+    """The operator's own body, with tensors that have no memory: a host address must not reach a kernel."""
+    given = dict(dy=meta(5, 300), x=meta(5, 300), scale=None, mean=meta(5, dtype=torch.float32), variance=meta(5, dtype=torch.float32), eps=1e-5,
+                 param_dtype=torch.float32)
+    with pytest.raises(ValueError, match="layernorm"):
+        torch_ops.layernorm_backward._init_fn(**{**given, **wrong})
+
+
 @pytest.mark.parametrize("more", [dict(few=65), dict(few=-1), dict(few=4, top=17)])
 def test_experts_refuse_more_tokens_than_the_kernels_take(more):
     with pytest.raises(ValueError):
