@@ -663,14 +663,18 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
                     }
                 }
             }
-            // sums of the tokens `b`, in two chains in turn: the matrix instructions of one wait for one another
+            // sums of the tokens `b`, in chains in turn: the matrix instructions of one wait for one another.  part: of e4m3 weights this step's,
+            // for the scale; of others the products of h's lower half, which count only where they are finite: with an infinite weight the upper
+            // half has the infinity, and the lower one, which may be zero or of the other sign, must not make it NaN.
             auto add = [&](float(&sum)[2][4], const Tokens &b) {
+                constexpr bool kApart = kDown && kW != kE4m3;
                 float part[2][4];
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     part[m][0] = part[m][1] = part[m][2] = part[m][3] = 0.0f;
                 }
                 float(&to)[2][4] = kW == kE4m3 ? part : sum;
+                float(&lower)[2][4] = kApart ? part : to;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     if (kTf32) {
@@ -685,8 +689,8 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
                                 const uint32_t w = word(a[u][r], j);
                                 f[r] = __half22float2(*reinterpret_cast<const __half2 *>(&w));
                             }
-                            mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.y, b1.y);
-                            mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.y, b1.y);
+                            mma_tf32(lower[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.y, b1.y);
+                            mma_tf32(lower[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.y, b1.y);
                             mma_tf32(to[0], f[0].x, f[1].x, f[0].y, f[1].y, b0.x, b1.x);
                             mma_tf32(to[1], f[2].x, f[3].x, f[2].y, f[3].y, b0.x, b1.x);
                         }
@@ -712,7 +716,7 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
                                 const uint4 &q = b.q[u][plane][j / 2];
 #pragma unroll
                                 for (int m = 0; m < 2; ++m) {
-                                    mma_16<kBfMma>(to[m], w[m][0], w[m][1], w[m][2], w[m][3], word(q, j % 2 * 2), word(q, j % 2 * 2 + 1));
+                                    mma_16<kBfMma>(plane > 0 ? lower[m] : to[m], w[m][0], w[m][1], w[m][2], w[m][3], word(q, j % 2 * 2), word(q, j % 2 * 2 + 1));
                                 }
                             }
                         }
@@ -724,6 +728,15 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             sum[m][i] = fmaf(part[m][i], of_block[2 * m + i / 2], sum[m][i]);
+                        }
+                    }
+                }
+                if (kApart) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            sum[m][i] += isfinite(part[m][i]) ? part[m][i] : 0.0f;
                         }
                     }
                 }

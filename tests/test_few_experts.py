@@ -235,6 +235,62 @@ def test_gated_values_beyond_the_range_of_16_bits(cuda_device, dtype, eight, lou
     block.check()
 
 
+def pitched(w, extra, offset=0):
+    """w at a pitch of its rows that is a multiple of 16 bytes where `offset` is 0 and `extra` such a number of elements."""
+    g, n, k = w.shape
+    ld = -(-k // 16) * 16 + extra
+    store = torch.zeros((offset + g * n * ld,), dtype=w.dtype, device="cuda")
+    view = store[offset:].view(g, n, ld)[:, :, :k]
+    view.copy_(w)
+    return view
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 6, 12, 20, 64])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_infinite_weights(cuda_device, dtype, tokens, offset):
+    """As the definition has it, by the kernels that stream (offset 0) and by the general ones: an infinity in down, times values that are not
+    zero, is an infinity of the product's sign; two of unlike signs are NaN; one in up's rows makes h infinite."""
+    block = Block(tokens, 3, 2, 264, 136, dtype, False, seed=tokens)
+    block.ids = torch.tensor([[t % 3, (t + 1) % 3] for t in range(tokens)], dtype=torch.int32, device="cuda")
+    if tokens == 64:
+        block.ids[:, :] = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    block.down[0, 100, 70] = float("inf")
+    block.down[0, 263, 135] = float("-inf")
+    block.down[1, 7, 3], block.down[1, 7, 4] = float("inf"), float("inf")
+    block.gate_up[2, 136 + 50, 9] = float("inf")
+    block.gate_up, block.down = pitched(block.gate_up, 0, offset), pitched(block.down, 0, offset)
+    y, off = block.definition()
+    got = block.run().double()
+    assert bool(torch.isinf(y).any())
+    assert torch.equal(torch.isnan(got), torch.isnan(y))
+    assert torch.equal(torch.isposinf(got), torch.isposinf(y)) and torch.equal(torch.isneginf(got), torch.isneginf(y))
+    finite = torch.isfinite(y)
+    assert bool(finite.any()) or tokens == 1
+    clean = torch.isfinite(off) & finite
+    assert torch.all((got - y)[clean].abs() <= off[clean])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_infinite_weights_times_values_without_a_lower_half(cuda_device, dtype, offset):
+    """h = 64 * 2 exactly: its upper half is all of it, its lower half is zero."""
+    block = Block(1, 1, 1, 8, 8, dtype, False)
+    block.x.fill_(0.0)
+    block.x[0, 0] = 2.0
+    block.gate_up.fill_(0.0)
+    block.gate_up[0, 2, 0], block.gate_up[0, 8 + 2, 0] = 32.0, 1.0
+    block.down.fill_(1.0)
+    block.down[0, 5, 2], block.down[0, 6, 2] = float("inf"), float("-inf")
+    block.p.fill_(0.5)
+    block.gate_up, block.down = pitched(block.gate_up, 0, offset), pitched(block.down, 0, offset)
+    want = torch.full((1, 8), 64.0, device="cuda")
+    want[0, 5], want[0, 6] = float("inf"), float("-inf")
+    assert torch.equal(block.run().float(), want)
+
+
 @gpu
 def test_streams_and_graphs(cuda_device):
     """Two calls at once, each with a workspace; one captured and replayed on other tokens, ids and weights: the same bits as alone."""
