@@ -775,9 +775,11 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
             if (kW == kF16) {
                 static_cast<float *>(p.h)[to] = v;
             } else {
-                const float hi = __bfloat162float(__float2bfloat16_rn(v));
+                // next to fp32's largest value the upper half is cut, not rounded, which would make it infinite; the rest is rounded either way
+                const float nearest = bf16_bits_to_f32(f32_to_bf16_rne_bits(v));
+                const float hi = isfinite(v) && !isfinite(nearest) ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : nearest;
                 unsigned short *planes = static_cast<unsigned short *>(p.h);
-                planes[to] = f32_to_bf16_rne_bits(v);
+                planes[to] = f32_to_bf16_rne_bits(hi);
                 planes[plane_step + to] = f32_to_bf16_rne_bits(isfinite(hi) ? v - hi : 0.0f);
             }
         };

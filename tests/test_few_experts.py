@@ -292,6 +292,26 @@ def test_infinite_weights_times_values_without_a_lower_half(cuda_device, dtype, 
 
 
 @gpu
+@pytest.mark.parametrize("offset", [0, 1])
+def test_gated_values_next_to_the_largest(cuda_device, offset):
+    """h = 2^64 (2^64 - 2^55): below fp32's largest value, but nearer to 2^128 than to bf16's largest.  Times 2^-126 it is 4 - 2^-7, which bf16
+    rounds to 4."""
+    block = Block(1, 1, 1, 8, 8, torch.bfloat16, False)
+    block.x.fill_(0.0)
+    block.x[0, 0], block.x[0, 1] = 2.0 ** 64, 2.0 ** 55
+    block.gate_up.fill_(0.0)
+    block.gate_up[0, 2, 0] = 1.0
+    block.gate_up[0, 8 + 2, 0], block.gate_up[0, 8 + 2, 1] = 1.0, -1.0
+    block.down.fill_(0.0)
+    block.down[0, 5, 2], block.down[0, 6, 2] = 2.0 ** -126, -(2.0 ** -120)
+    block.p.fill_(1.0)
+    block.gate_up, block.down = pitched(block.gate_up, 0, offset), pitched(block.down, 0, offset)
+    want = torch.zeros((1, 8), device="cuda")
+    want[0, 5], want[0, 6] = 4.0, -256.0
+    assert torch.equal(block.run().float(), want)
+
+
+@gpu
 def test_streams_and_graphs(cuda_device):
     """Two calls at once, each with a workspace; one captured and replayed on other tokens, ids and weights: the same bits as alone."""
     blocks = [Block(6, 32, 4, 512, 384, torch.bfloat16, False, seed=s) for s in (1, 2)]
