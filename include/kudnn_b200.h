@@ -321,14 +321,17 @@ KUDNN_B200_API int kudnn_b200_grouped_last_tile(kudnn_b200_grouped_t handle, int
  *   key         = score + bias[e] (without a bias: score)
  * The experts with the largest keys are chosen, largest first, the lower index first among equals.  Their scores (without the bias) become
  * the weights, with `normalise` divided by their sum, then times `scale`; fp32.  An expert whose bias is minus infinity or whose key is NaN
- * takes no part; where fewer than `top` do, the places left over get the id -1 and the weight 0.
+ * takes no part; where fewer than `top` do, the places left over get the id -1 and the weight 0.  A token with a NaN, or whose softmax is NaN
+ * because of an infinite logit, then goes nowhere.  With `nan_first` a NaN key comes before all others, the lower index first, and its weight is
+ * NaN (with `normalise` all of the token's are), so that what follows shows it.
  * x, w: F32 / F16 / BF16 at row pitches; bias fp32; ids int32 and weights fp32 are dense [tokens, top].  At most 1024 experts, top at most 64. */
 #define KUDNN_B200_SCORE_SOFTMAX 0
 #define KUDNN_B200_SCORE_SIGMOID 1
 typedef struct kudnn_b200_route_desc {
     int64_t tokens, hidden, x_ld, w_ld;
     int32_t experts, top, x_dtype, w_dtype, score, normalise;
-    float scale, reserved_f;
+    float scale;
+    int32_t nan_first; /* 0: as above */
 } kudnn_b200_route_desc;
 KUDNN_B200_API int kudnn_b200_route_validate(const kudnn_b200_route_desc *desc);
 KUDNN_B200_API int kudnn_b200_route_run(const kudnn_b200_route_desc *desc, const void *x, const void *w, const float *bias, float *weights,

@@ -107,7 +107,7 @@ class RouteDesc(ctypes.Structure):
     _fields_ = [
         ("tokens", ctypes.c_int64), ("hidden", ctypes.c_int64), ("x_ld", ctypes.c_int64), ("w_ld", ctypes.c_int64),
         ("experts", ctypes.c_int32), ("top", ctypes.c_int32), ("x_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
-        ("score", ctypes.c_int32), ("normalise", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved_f", ctypes.c_float),
+        ("score", ctypes.c_int32), ("normalise", ctypes.c_int32), ("scale", ctypes.c_float), ("nan_first", ctypes.c_int32),
     ]
 
 
@@ -469,11 +469,14 @@ class Grouped:
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 
-def make_route_desc(tokens, experts, hidden, top, dtype, *, router_dtype=F32, score=SCORE_SOFTMAX, normalise=True, scale=1.0, x_ld=None, w_ld=None):
-    """Descriptor of the choice of `top` of `experts` experts for each of x [tokens, hidden] by a router [experts, hidden]; dense by default."""
+def make_route_desc(tokens, experts, hidden, top, dtype, *, router_dtype=F32, score=SCORE_SOFTMAX, normalise=True, scale=1.0, x_ld=None, w_ld=None,
+                    nan_first=False):
+    """Descriptor of the choice of `top` of `experts` experts for each of x [tokens, hidden] by a router [experts, hidden]; dense by default.
+    nan_first: NaN keys come before all others and have weights of NaN; without it they take no part."""
     d = RouteDesc()
     d.tokens, d.experts, d.hidden, d.top = tokens, experts, hidden, top
     d.x_dtype, d.w_dtype, d.score, d.normalise, d.scale = dtype, router_dtype, score, 1 if normalise else 0, scale
+    d.nan_first = 1 if nan_first else 0
     d.x_ld, d.w_ld = hidden if x_ld is None else x_ld, hidden if w_ld is None else w_ld
     return d
 

@@ -19,7 +19,7 @@ struct RouteParams {
     int *ids;
     long long x_ld, w_ld;
     int tokens, experts, hidden, top;
-    int x_dtype, w_dtype, sigmoid, normalise;
+    int x_dtype, w_dtype, sigmoid, normalise, nan_first;
     float scale;
 };
 cudaError_t launch_route(const RouteParams &p, cudaStream_t stream);

@@ -170,9 +170,10 @@ __device__ __forceinline__ void finish_token(const RouteParams &p, int token, in
         if (key[i] != 0ull) {
             const double s = p.sigmoid != 0 ? 1.0 / (1.0 + exp(-v[i])) : v[i] / sum;
             const double k = (p.bias != nullptr ? s + static_cast<double>(p.bias[e]) : s) + 0.0;
-            scores[e] = s;
+            const bool ahead = p.nan_first != 0 && k != k;
+            scores[e] = ahead ? k : s;
             const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(k));
-            key[i] = k > lowest ? ((bits >> 63) != 0ull ? ~bits : bits | 0x8000000000000000ull) : 0ull;
+            key[i] = ahead ? ~0ull : k > lowest ? ((bits >> 63) != 0ull ? ~bits : bits | 0x8000000000000000ull) : 0ull;
         }
     }
     __syncwarp();

@@ -295,12 +295,13 @@ MOST_FEW_TOKENS, MOST_FEW_TOP = 64, 16
 
 @torch.library.custom_op("kudnn_b200::route", mutates_args=(), device_types="cuda")
 def route(x: torch.Tensor, router: torch.Tensor, top: int, bias: Optional[torch.Tensor] = None, score: str = "softmax", normalise: bool = True,
-          scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+          scale: float = 1.0, nan_first: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """x [tokens, hidden], router [experts, hidden] -> (weights [tokens, top] float32, ids [tokens, top] int32), the largest score first.
 
     Scores are a softmax or a sigmoid of x . router^T, computed in 64 bits.  bias [experts] float32 is added to them for the choice alone; minus
     infinity takes an expert out.  With `normalise` a token's weights are divided by their sum, then multiplied by `scale`.  Places that no
-    expert is left for have the id -1 and the weight 0."""
+    expert is left for have the id -1 and the weight 0.  An expert whose score is NaN takes no part, or with `nan_first` comes before all others
+    with a weight of NaN, as in torch.topk."""
     if x.dtype not in _DTYPES or router.dtype not in _DTYPES:
         raise TypeError("kudnn_b200::route takes float32 / float16 / bfloat16 tokens and routers")
     if x.dim() != 2 or router.dim() != 2 or x.shape[1] != router.shape[1] or router.device != x.device:
@@ -314,14 +315,14 @@ def route(x: torch.Tensor, router: torch.Tensor, top: int, bias: Optional[torch.
     weights = torch.empty((tokens, top), dtype=torch.float32, device=x.device)
     ids = torch.empty((tokens, top), dtype=torch.int32, device=x.device)
     desc = capi.make_route_desc(tokens, router.shape[0], x.shape[1], top, _DTYPES[x.dtype], router_dtype=_DTYPES[router.dtype], score=SCORES[score],
-                                normalise=normalise, scale=scale, x_ld=x.stride(0), w_ld=router.stride(0))
+                                normalise=normalise, scale=scale, x_ld=x.stride(0), w_ld=router.stride(0), nan_first=nan_first)
     with _on(x.device):
         capi.route(desc, x, router, weights, ids, None if bias is None else bias.contiguous(), stream=torch.cuda.current_stream(x.device).cuda_stream)
     return weights, ids
 
 
 @route.register_fake
-def _route_fake(x, router, top, bias=None, score="softmax", normalise=True, scale=1.0):
+def _route_fake(x, router, top, bias=None, score="softmax", normalise=True, scale=1.0, nan_first=False):
     return x.new_empty((x.shape[0], top), dtype=torch.float32), x.new_empty((x.shape[0], top), dtype=torch.int32)
 
 
@@ -426,7 +427,7 @@ class Experts(torch.nn.Module):
         count, experts = tokens.shape[0], self.router.shape[0]
         ops = torch.ops.kudnn_b200
         if count <= self.few and x.dtype in (torch.float16, torch.bfloat16) and (self.eight_bit or self.gate_up.dtype == x.dtype):
-            p, chosen = ops.route(tokens, self.router, self.top)
+            p, chosen = ops.route(tokens, self.router, self.top, nan_first=True)  # a token without a softmax stays visible, as below
             scales = (self.gate_up_scale, self.down_scale) if self.eight_bit else (None, None)
             return ops.experts(tokens, p, chosen, self.gate_up, self.down, *scales).view(x.shape)
         p, chosen = torch.topk(torch.softmax(ops.linear(tokens.float(), self.router), dim=1), self.top, dim=1)

@@ -131,6 +131,38 @@ def test_values_that_are_no_numbers(cuda_device):
 
 
 @gpu
+@pytest.mark.parametrize("tokens", [6, 800])
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("normalise", [False, True])
+@pytest.mark.parametrize("taken_out", [[], [3], [3, 7]])
+def test_scores_that_are_no_numbers_come_first_where_asked_for(cuda_device, tokens, sigmoid, normalise, taken_out):
+    """nan_first: a token with a NaN, one with an infinity (whose softmax is NaN), and an expert whose row holds a NaN; an expert that is taken
+    out stays out.  The other tokens' ids and weights are those of the call without it."""
+    x, w = operands(tokens, 12, 64, torch.bfloat16, torch.float32)
+    x[2, 5], x[4, 9] = float("nan"), float("inf")
+    bias = torch.zeros(12, device="cuda")
+    bias[taken_out] = -math.inf
+    for broken in (None, 7):
+        if broken is not None:
+            w[broken, 3] = float("nan")
+        logits = x.double() @ w.double().t()
+        out, nan = torch.isneginf(bias), torch.isnan(logits)
+        score = 1 / (1 + torch.exp(-logits)) if sigmoid else torch.softmax(logits.masked_fill(out | nan, -math.inf), dim=1)
+        score = score.masked_fill(nan, float("nan"))
+        key = torch.where(torch.isnan(score), torch.full_like(score, 9.0), score).masked_fill(out, -math.inf)
+        ids = torch.sort(key, dim=1, descending=True, stable=True)[1][:, :4]
+        p = score.gather(1, ids)
+        p = p / p.sum(dim=1, keepdim=True) if normalise else p
+        desc = kb.make_route_desc(tokens, 12, 64, 4, kb.BF16, normalise=normalise, nan_first=True, score=kb.SCORE_SIGMOID if sigmoid else kb.SCORE_SOFTMAX)
+        weights, names = torch.full((tokens, 4), -7.0, device="cuda"), torch.full((tokens, 4), -7, dtype=torch.int32, device="cuda")
+        kb.route(desc, x, w, weights, names, bias)
+        assert torch.equal(names, ids.int())
+        assert torch.equal(torch.isnan(weights), torch.isnan(p)) and bool(torch.isnan(weights[2]).any())
+        there = ~torch.isnan(p)
+        assert torch.all((weights.double() - p)[there].abs() <= (2.0 ** -24 + 2.0 ** -40) * p[there].abs() + 2.0 ** -149)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("offset,extra", [(0, 0), (1, 0), (2, 3), (4, 4), (3, 1)])
 def test_pitch_and_alignment(cuda_device, dtype, offset, extra):

@@ -87,6 +87,28 @@ def test_many_tokens_and_few_of_zero_take_the_way_they_took(cuda_device):
 
 @gpu
 @pytest.mark.parametrize("eight_bit", [False, True])
+def test_tokens_whose_scores_are_no_numbers_stay_visible_either_way(cuda_device, eight_bit):
+    """A token with a NaN or an infinity has a softmax of NaN, and so its answer is NaN, by the kernels for few tokens as by those for many; the
+    others are as without it but for their rounding, twice 2^-8: with other experts chosen the weights are cut elsewhere, and sums are taken in
+    another order.  A router that holds a NaN has no softmax for any token."""
+    few, _ = block(eight_bit, 64)
+    many, _ = block(eight_bit, 0)
+    x = torch.randn(6, 512, device="cuda").bfloat16()
+    clean = few(x)
+    x[1, 5], x[4, 300] = float("nan"), float("inf")
+    bad = torch.tensor([False, True, False, False, True, False], device="cuda")
+    for experts in (few, many):
+        y = experts(x)
+        assert bool(torch.isnan(y[bad]).all()) and bool(torch.isfinite(y[~bad]).all())
+    got, want = few(x)[~bad].double(), clean[~bad].double()
+    assert torch.linalg.vector_norm(got - want) <= 2.0 ** -7 * torch.linalg.vector_norm(want)
+    for experts in (few, many):
+        experts.router[3, 17] = float("nan")
+        assert bool(torch.isnan(experts(x)).all())
+
+
+@gpu
+@pytest.mark.parametrize("eight_bit", [False, True])
 def test_a_sublayer(cuda_device, eight_bit):
     """x + experts(layernorm(x)) of one to 64 tokens, eager and captured; against 64 bits on the normalised rows as they were rounded."""
     experts, parts = block(eight_bit, 64, hidden=768, ffn=320)
