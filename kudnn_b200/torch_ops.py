@@ -426,7 +426,7 @@ class Experts(torch.nn.Module):
         tokens = x.reshape(-1, x.shape[-1])
         count, experts = tokens.shape[0], self.router.shape[0]
         ops = torch.ops.kudnn_b200
-        if count <= self.few and x.dtype in (torch.float16, torch.bfloat16) and (self.eight_bit or self.gate_up.dtype == x.dtype):
+        if 0 < self.few and count <= self.few and x.dtype in (torch.float16, torch.bfloat16) and (self.eight_bit or self.gate_up.dtype == x.dtype):
             p, chosen = ops.route(tokens, self.router, self.top, nan_first=True)  # a token without a softmax stays visible, as below
             scales = (self.gate_up_scale, self.down_scale) if self.eight_bit else (None, None)
             return ops.experts(tokens, p, chosen, self.gate_up, self.down, *scales).view(x.shape)

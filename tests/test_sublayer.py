@@ -59,6 +59,35 @@ def test_shapes_on_either_side_of_few(eight_bit, shape):
     assert y.shape == shape and y.dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("tokens", [0, 3])
+def test_a_module_without_few_keeps_to_the_way_of_many(eight_bit, tokens):
+    """Not even no tokens go to the kernels for few: without `few` any top is allowed, also one that those refuse."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    called = []
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            called.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    experts = torch_ops.Experts(meta(20, 300, dtype=torch.float32), meta(20, 400, 300), meta(20, 300, 200), 17, eight_bit=eight_bit)
+    with Record():
+        y = experts(meta(tokens, 300))
+    assert y.shape == (tokens, 300) and "kudnn_b200::grouped" in called
+    assert "kudnn_b200::route" not in called and "kudnn_b200::experts" not in called
+
+
+@gpu
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("few,top", [(0, 17), (8, 4)])
+def test_no_tokens(cuda_device, eight_bit, few, top):
+    experts, _ = block(eight_bit, few, count=20, top=top)
+    y = experts(torch.empty((2, 0, 512), dtype=torch.bfloat16, device="cuda"))
+    assert y.shape == (2, 0, 512) and y.dtype == torch.bfloat16
+
+
 @gpu
 @pytest.mark.parametrize("tokens", [1, 7, 64, 65])
 @pytest.mark.parametrize("eight_bit", [False, True])
