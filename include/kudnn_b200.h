@@ -226,7 +226,9 @@ KUDNN_B200_API int kudnn_b200_rmsnorm_run(const void *src, void *dst, const void
  * dy, with the same pitch; other overlaps are not allowed.  What lies between the rows is not written. */
 typedef struct kudnn_b200_layernorm_desc {
     int64_t rows, axis;
-    int64_t x_ld, y_ld, dy_ld, dx_ld; /* row pitches in elements; columns are contiguous */
+    /* row pitches in elements; columns are contiguous.  Those of results are axis at least, or 0 where the call does not write them: dy_ld and
+     * dx_ld do not matter for y, y_ld does not for the gradient, nor dx_ld where dx is NULL. */
+    int64_t x_ld, y_ld, dy_ld, dx_ld;
     int32_t dtype, param_dtype, flags, reserved;
     float eps, reserved_f;
 } kudnn_b200_layernorm_desc;

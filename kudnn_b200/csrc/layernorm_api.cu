@@ -98,7 +98,8 @@ int kudnn_b200_layernorm_validate(const kudnn_b200_layernorm_desc *d)
     if (!(d->eps >= 0.0f) || std::isinf(d->eps)) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: eps is finite and not negative");
     }
-    if (d->rows > 1 && (d->y_ld < d->axis || d->dx_ld < d->axis)) {
+    // 0: not used by this call; whoever writes the result looks again
+    if (d->rows > 1 && ((d->y_ld != 0 && d->y_ld < d->axis) || (d->dx_ld != 0 && d->dx_ld < d->axis))) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: rows of a result overlap");
     }
     return KUDNN_B200_OK;
@@ -119,6 +120,9 @@ int kudnn_b200_layernorm_run(const kudnn_b200_layernorm_desc *d, const void *x, 
     if (y == nullptr || ((d->flags & KUDNN_B200_NORM_USE_SHIFT) != 0) != (shift != nullptr) ||
         (p.given != 0 && (mean == nullptr || variance == nullptr))) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: y, the shift or the given statistics and the descriptor do not agree");
+    }
+    if (d->rows > 1 && d->y_ld < d->axis) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: rows of a result overlap");
     }
     if (misaligned(y, kb::dtype_size(d->dtype)) || misaligned(shift, kb::dtype_size(d->param_dtype))) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: a tensor is not aligned to its elements");
@@ -178,6 +182,9 @@ int kudnn_b200_layernorm_backward_run(const kudnn_b200_layernorm_desc *d, const 
     const bool sums = dscale != nullptr || dshift != nullptr;
     if (sums && (workspace == nullptr || misaligned(workspace, 4) || workspace_bytes < kb::layernorm_backward_floats(d->rows, d->axis) * 4)) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: the workspace is missing, too small or not aligned");
+    }
+    if (dx != nullptr && d->rows > 1 && d->dx_ld < d->axis) {
+        return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: rows of a result overlap");
     }
     if (misaligned(dy, kb::dtype_size(d->dtype)) || misaligned(dx, kb::dtype_size(d->dtype))) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "layernorm: a tensor is not aligned to its elements");

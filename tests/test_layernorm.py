@@ -338,3 +338,41 @@ def test_calls_that_are_refused(call):
 def test_workspace_grows_with_the_rows_up_to_a_bound():
     sizes = [kb.layernorm_backward_workspace(desc(rows=rows, axis=100)) for rows in (0, 1, 7, 592, 10 ** 6)]
     assert sizes == [0, 800, 5600, 473600, 473600]
+
+
+@pytest.mark.parametrize("unused", [dict(dx_ld=0, dy_ld=0), dict(dx_ld=0)])
+def test_pitches_that_a_forward_call_does_not_use_may_be_zero(unused):
+    """On the host: refused for its y (misaligned), not for a dx that it does not write."""
+    with pytest.raises(kb.KudnnError, match="aligned"):
+        kb.layernorm(desc(**unused), 16, 17)
+    with pytest.raises(kb.KudnnError, match="overlap"):
+        kb.layernorm(desc(y_ld=0), 16, 16)
+
+
+def test_pitches_that_a_gradient_does_not_use_may_be_zero():
+    assert kb.layernorm_backward_workspace(desc(y_ld=0)) == 4 * 2 * 8 * 4
+    with pytest.raises(kb.KudnnError, match="aligned"):
+        kb.layernorm_backward(desc(y_ld=0), 16, 16, None, 16, 16, 17)
+    with pytest.raises(kb.KudnnError, match="workspace"):  # dx is not wanted
+        kb.layernorm_backward(desc(y_ld=0, dx_ld=0), 16, 16, None, 16, 16, None, 16)
+    with pytest.raises(kb.KudnnError, match="overlap"):
+        kb.layernorm_backward(desc(dx_ld=0), 16, 16, None, 16, 16, 16)
+
+
+@gpu
+def test_results_with_only_the_pitches_that_they_use(cuda_device):
+    x, dy = values(5, 24, torch.float32), values(5, 24, torch.float32, seed=5)
+    y, mean, variance = forward(x)
+    want = backward(x, dy, None, mean, variance)
+    again, dx, dscale, dshift = torch.empty_like(x), torch.empty_like(x), torch.empty(24, device="cuda"), torch.empty(24, device="cuda")
+    kb.layernorm(kb.make_layernorm_desc(5, 24, kb.F32, eps=EPS, dy_ld=0, dx_ld=0), x, again)
+    assert torch.equal(again, y)
+    d = kb.make_layernorm_desc(5, 24, kb.F32, eps=EPS, y_ld=0)
+    size = kb.layernorm_backward_workspace(d)
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    kb.layernorm_backward(d, x, dy, None, mean, variance, dx, dscale, dshift, space, size)
+    assert all(torch.equal(a, b) for a, b in zip((dx, dscale, dshift), want))
+    d.dx_ld = 0
+    dscale.zero_(), dshift.zero_()
+    kb.layernorm_backward(d, x, dy, None, mean, variance, None, dscale, dshift, space, size)
+    assert torch.equal(dscale, want[1]) and torch.equal(dshift, want[2])
