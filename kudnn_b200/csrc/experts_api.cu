@@ -30,6 +30,7 @@ bool misaligned(const void *p, int size)
 }
 
 constexpr int64_t kMostExtent = 0x7fffffffll - 1024;
+constexpr int64_t kMostRouterDepth = 0x7fffffffll - 4096;  // its kernels look up to 2060 elements ahead, in 32 bits
 
 int current_device(int *sms)
 {
@@ -57,7 +58,7 @@ int kudnn_b200_route_validate(const kudnn_b200_route_desc *d)
     if (d->tokens < 0 || d->x_ld < 0 || d->w_ld < 0) {
         return fail(KUDNN_B200_BAD_ARGUMENTS, "route: negative extents or pitches");
     }
-    if (d->hidden <= 0 || d->hidden > kMostExtent || d->tokens > kMostExtent / 8) {
+    if (d->hidden <= 0 || d->hidden > kMostRouterDepth || d->tokens > kMostExtent / 8) {
         return fail(KUDNN_B200_UNSUPPORTED, "route: rows without elements and extents of 2^28 tokens and more are not supported");
     }
     if (d->experts < 1 || d->experts > kb::kMostExperts) {

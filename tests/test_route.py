@@ -226,3 +226,11 @@ def test_calls_that_are_refused(place, wrong):
     with pytest.raises(kb.KudnnError) as e:
         kb.route(desc(), *operands)
     assert e.value.status == 2
+
+
+def test_the_longest_rows():
+    """Steps of up to 2048 elements are taken while they end within a row, in 32 bits: rows that such a sum could pass 2^31 for are refused."""
+    for hidden, status in ((2 ** 31 - 1025, 1), (2 ** 31 - 2049, 1), (2 ** 31 - 4096, 1), (2 ** 31 - 4097, 2)):
+        with pytest.raises(kb.KudnnError) as e:
+            kb.route(desc(hidden=hidden), None, 16, 16, 16)
+        assert e.value.status == status
