@@ -476,12 +476,12 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
         }
     };
     auto copy_tokens = [&](int stage, int k, int bytes) {
-        if (copies) {
+        if (copies && bytes > 0) {
             bulk_copy(copy_to + stage * shape.token_bytes, copy_from + static_cast<long long>(k) * kTokenElem, bytes, full + stage);
         }
     };
-    // h's rows are whole; x's last step ends at the last 16 bytes that hold elements
-    auto token_bytes = [&](int k) { return kDown ? kTokenRow : min(kTokenRow, (depth - k + 7) / 8 * 16); };
+    // h's rows are whole; of x's last step the whole 16 bytes
+    auto token_bytes = [&](int k) { return kDown ? kTokenRow : min(kTokenRow, (depth - k) / 8 * 16); };
     auto issue = [&]() {
         if (ahead_left > 0) {
             const int bytes = token_bytes(ahead_k);
@@ -609,12 +609,14 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
             const int k = step * kStep + t * kPiece;
             const bool whole = kDown || (staged && (step + 1) * kStep <= depth);
             if (!kDown && staged && !whole) {
-                // x's last step: zeros behind the last element, where the copy brought what follows or nothing
-                const int left = depth - step * kStep;
+                // x's last step: the elements behind the last whole 16 bytes, which the copy did not bring, and zeros behind the last one
+                const int left = depth - step * kStep, copied = left & ~7;
 #pragma unroll 1
                 for (int i = lane; i < min(count, 8) * kStep; i += 32) {
-                    if (i % kStep >= left) {
-                        reinterpret_cast<unsigned short *>(token_ring + stage * shape.token_bytes + i / kStep * kTokenPitch)[i % kStep] = 0;
+                    const int row = i / kStep, column = i % kStep;
+                    if (column >= copied) {
+                        const unsigned short *from = reinterpret_cast<const unsigned short *>(token_row(first + row, 0)) + step * kStep + column;
+                        reinterpret_cast<unsigned short *>(token_ring + stage * shape.token_bytes + row * kTokenPitch)[column] = column < left ? *from : 0;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

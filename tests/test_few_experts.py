@@ -188,6 +188,22 @@ def test_pitch_alignment_and_layout(cuda_device, dtype, eight, hidden, ffn):
 
 @gpu
 @pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("tokens", [1, 3, 8, 13, 40])
+@pytest.mark.parametrize("hidden", [1, 7, 8, 65, 130, 250, 301])
+def test_tokens_that_end_inside_16_bytes(cuda_device, dtype, eight, tokens, hidden):
+    """Rows of x on 16-byte boundaries whose last elements fill a part of 16 bytes only, NaN behind them, the last row at its storage's end;
+    weights that are streamed."""
+    block = Block(tokens, 5, 2, hidden, 72, dtype, eight)
+    block.gate_up, block.down = pitched(block.gate_up, 16), pitched(block.down, 16)
+    ld = -(-hidden // 8) * 8
+    store = torch.full(((tokens - 1) * ld + hidden,), float("nan"), dtype=dtype, device="cuda")
+    x = torch.as_strided(store, (tokens, hidden), (ld, 1))
+    x.copy_(block.x)
+    block.check(block.run(x=x))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
 def test_in_place(cuda_device, dtype, eight):
     block = Block(7, 8, 2, 512, 256, dtype, eight)
     want = block.run()
