@@ -373,9 +373,10 @@ typedef struct kudnn_b200_experts_args {
 KUDNN_B200_API int kudnn_b200_experts_validate(const kudnn_b200_experts_desc *desc);
 KUDNN_B200_API int kudnn_b200_experts_workspace(const kudnn_b200_experts_desc *desc, int64_t *bytes);
 KUDNN_B200_API int kudnn_b200_experts_run(const kudnn_b200_experts_desc *desc, const kudnn_b200_experts_args *args, void *cuda_stream);
-/* After synchronising the stream: whether a device-side wait of a run on the current device has given up since the last check (TIMEOUT; the
- * results of that run are undefined).  set_wait is a test hook for all later runs of the process: the waits' limit in cycles (0: the default,
- * about two seconds), and the step of 128 bytes of K from which on no weights are copied (-1: off). */
+/* After synchronising the stream: whether a device-side wait of any run on the current device has given up since this thread's last check of the
+ * device, before its first one since the program began (TIMEOUT; the results of that run are undefined).  Threads do not take reports from each
+ * other.  set_wait is a test hook for all later runs of the process: the waits' limit in cycles (0: the default, about two seconds), and the step
+ * of 128 bytes of K from which on no weights are copied (-1: off). */
 KUDNN_B200_API int kudnn_b200_experts_check(void *cuda_stream);
 KUDNN_B200_API int kudnn_b200_experts_set_wait(long long wait_limit_cycles, int skip_step);
 

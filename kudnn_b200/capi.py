@@ -517,7 +517,8 @@ def experts(desc, x, weights, ids, gate_up, down, y, workspace, workspace_bytes,
 
 
 def experts_check(stream=None):
-    """Raises KudnnError (TIMEOUT) if a device-side wait of experts has given up on the current device since the last check."""
+    """Raises KudnnError (TIMEOUT) if a device-side wait of experts has given up on the current device since this thread's last check of it.
+    Every thread gets every report."""
     _check(library().kudnn_b200_experts_check(stream))
 
 

@@ -43,7 +43,8 @@ long long experts_workspace_bytes(long long tokens, long long top, long long ffn
 bool experts_stream_takes(const ExpertsParams &p);
 cudaError_t launch_experts_stream(const ExpertsParams &p, int sm_count, cudaStream_t stream);
 void experts_set_wait(long long limit_cycles, int skip_step);
-cudaError_t experts_take_status(DeviceStatus *status);  // of the current device, and clears it
+// Of the current device, since the program began: how many waits gave up, and which was the last
+cudaError_t experts_status_of(unsigned *gave_up, DeviceStatus *last);
 cudaError_t launch_experts_any(const ExpertsParams &p, cudaStream_t stream);
 
 // silu(gate) * up in fp32: e raised to a power below zero, so that the divisor lies in [1, 2]

@@ -3,6 +3,8 @@
 
 #include <cmath>
 #include <cstdio>
+#include <map>
+#include <new>
 
 namespace {
 
@@ -242,18 +244,31 @@ int kudnn_b200_experts_run(const kudnn_b200_experts_desc *d, const kudnn_b200_ex
 
 int kudnn_b200_experts_check(void *cuda_stream)
 {
-    int sms = 0;
+    // What this thread has seen of each device.  Runs of all callers count together: a thread that took another's report away would leave the
+    // other with results that are undefined and a check that says nothing.
+    static thread_local std::map<int, unsigned> seen;
+    int sms = 0, dev = 0;
     const int rc = current_device(&sms);
     if (rc != KUDNN_B200_OK) {
         return rc;
     }
     kb::DeviceStatus st;
-    cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(cuda_stream));
-    if (e == cudaSuccess) e = kb::experts_take_status(&st);
+    unsigned gave_up = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(static_cast<cudaStream_t>(cuda_stream));
+    if (e == cudaSuccess) e = kb::experts_status_of(&gave_up, &st);
     if (e != cudaSuccess) {
         return fail_cuda(e, "experts: check");
     }
-    if (st.code != kb::kErrNone) {
+    bool news = false;
+    try {
+        unsigned &known = seen[dev];
+        news = gave_up != known;
+        known = gave_up;
+    } catch (const std::bad_alloc &) {
+        return fail(KUDNN_B200_ALLOC_FAILED, "experts: check: out of host memory");
+    }
+    if (news) {
         char text[120];
         std::snprintf(text, sizeof(text), "device-side wait gave up (site %d, block %d)", st.where, st.block);
         return fail(KUDNN_B200_TIMEOUT, text);

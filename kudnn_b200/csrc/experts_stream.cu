@@ -48,8 +48,10 @@ enum Weights { kBf16, kF16, kE4m3 };
 template <Weights kW, int kTokens>
 constexpr int kWarpsOf = kW != kE4m3 || kTokens > 2 ? 8 : kTokens == 2 ? 12 : 16;
 
-// Waits that gave up, on this device since the last look.
+// Waits that gave up, on this device: how many lanes had one, ever, and which was the last.  Nothing takes it back, so that no look at it takes
+// another's report away (see experts_api.cu).
 __device__ DeviceStatus experts_status;
+__device__ unsigned experts_gave_up;
 
 struct Waits {
     long long limit;  // in cycles
@@ -900,6 +902,10 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
         }
     }
     if (gave_up) {
+        experts_status.where = kDown ? 2 : 1;
+        experts_status.block = static_cast<int>(blockIdx.x);
+        __threadfence();
+        atomicAdd(&experts_gave_up, 1u);  // every lane: some may have been there in time
         // the copies that are still on their way, each for a moment
         for (int i = 0; i < stages; ++i) {
             for (int spin = 0; spin < 2000 && !mbar_try_wait(full + i, parity ^ (i < stage ? 1u : 0u)); ++spin) {
@@ -984,14 +990,10 @@ void experts_set_wait(long long limit_cycles, int skip_step)
     wait_skip.store(skip_step);
 }
 
-cudaError_t experts_take_status(DeviceStatus *status)
+cudaError_t experts_status_of(unsigned *gave_up, DeviceStatus *last)
 {
-    cudaError_t e = cudaMemcpyFromSymbol(status, experts_status, sizeof(DeviceStatus));
-    if (e == cudaSuccess && status->code != kErrNone) {
-        const DeviceStatus none = {};
-        e = cudaMemcpyToSymbol(experts_status, &none, sizeof(DeviceStatus));
-    }
-    return e;
+    const cudaError_t e = cudaMemcpyFromSymbol(gave_up, experts_gave_up, sizeof(unsigned));
+    return e == cudaSuccess ? cudaMemcpyFromSymbol(last, experts_status, sizeof(DeviceStatus)) : e;
 }
 
 cudaError_t launch_experts_stream(const ExpertsParams &p, int sm_count, cudaStream_t stream)

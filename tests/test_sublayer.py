@@ -263,3 +263,46 @@ def test_a_wait_that_runs_out_is_reported(cuda_device):
         kb.experts_set_wait()
     assert torch.equal(experts(x), want)
     kb.experts_check(torch.cuda.current_stream().cuda_stream)
+
+
+@gpu
+def test_no_thread_takes_a_report_from_another(cuda_device):
+    """Two threads whose waits ran out: each learns of it, once, whichever looks first."""
+    import threading
+
+    experts, _ = block(False, 64)
+    x = torch.randn(3, 512, device="cuda").bfloat16()
+    ran, looked, seen = threading.Barrier(2), threading.Barrier(2), {}
+
+    def work(name):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(stream):
+            experts(x)
+            stream.synchronize()
+            ran.wait(60)
+            for turn in range(2):
+                if name == "second":
+                    looked.wait(60)
+                try:
+                    kb.experts_check(stream.cuda_stream)
+                    seen[name, turn] = 0
+                except kb.KudnnError as e:
+                    seen[name, turn] = e.status
+                if name == "first":
+                    looked.wait(60)
+
+    torch.cuda.synchronize()
+    kb.experts_set_wait(2000000, 1)
+    try:
+        threads = [threading.Thread(target=work, args=(name,)) for name in ("first", "second")]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(120)
+    finally:
+        kb.experts_set_wait()
+    assert seen == {("first", 0): 5, ("first", 1): 0, ("second", 0): 5, ("second", 1): 0}
+    with pytest.raises(kb.KudnnError):
+        kb.experts_check()
+    kb.experts_check()
