@@ -83,7 +83,7 @@ struct Lists {
     // `longer` of one more
     int &active, &group_warps, &tiles, &tile_pairs, &longer;
     static constexpr int kCounts = 32;
-    static __host__ __device__ __forceinline__ int bytes(int experts, int pairs)
+    static constexpr __host__ __device__ __forceinline__ int bytes(int experts, int pairs)
     {
         return kCounts + experts * 16 + (pairs * 13 + 15) / 16 * 16;
     }
@@ -932,6 +932,10 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
     const long long most = 6ll * std::min(p.experts, p.tokens * p.top) * p.hidden * p.ffn;  // bytes of the experts that can be chosen
     const int stage = kWarps * (kStageBytes + shape.token_bytes);
     const int fixed = 1024 + (kDown ? kWarps * p.tokens * kRows * 4 : kWarps * 1024) + Lists::bytes(p.experts, p.tokens * p.top);
+    // A ring of one step at least, whatever the call (a kernel without a ring would wait for copies that nobody makes)
+    constexpr int kMostFixed = 1024 + kWarps * (kDown ? 8 * kTokens * kRows * 4 : 1024) + Lists::bytes(kMostExperts, 8 * kTokens * kMostExpertTop);
+    constexpr int kMostStage = kWarps * (kStageBytes + 8 * (kDown && kW != kF16 ? 2 : 1) * kTokenPitch);
+    static_assert(8 * kTokens <= kMostExpertTokens && kMostFixed + kMostStage <= kMostShared, "shared memory holds no ring");
     const int in_half = kHalves ? (kHalfShared - fixed) / stage : 0;
     const bool two = most > 64ll << 20 && in_half >= 2;
     const int ctas = two ? 2 * sm_count : sm_count;
