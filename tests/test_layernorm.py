@@ -376,3 +376,31 @@ def test_results_with_only_the_pitches_that_they_use(cuda_device):
     dscale.zero_(), dshift.zero_()
     kb.layernorm_backward(d, x, dy, None, mean, variance, None, dscale, dshift, space, size)
     assert torch.equal(dscale, want[1]) and torch.equal(dshift, want[2])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,axis", [(5, 130), (40, 4096), (3, 8195), (2, 40000)])
+def test_means_far_above_the_deviation(cuda_device, dtype, rows, axis):
+    x = values(rows, axis, dtype, mean=1000.0)
+    scale, shift = params(axis, torch.float32)
+    got = forward(x, scale, shift)
+    check_forward(got, x, scale, shift)
+    dy = values(rows, axis, dtype, seed=5, mean=0.1)
+    check_backward(backward(x, dy, scale, got[1], got[2]), x, dy, scale, got[1], got[2])
+
+
+@gpu
+def test_elements_beyond_2_to_the_31(cuda_device):
+    """Two rows further apart than 32 bits count: x, y, dy and dx."""
+    ld, axis = 2 ** 31 + 9, 1027
+    near = values(2, axis, torch.float16)
+    store, out = [torch.empty(ld + axis, dtype=torch.float16, device="cuda") for _ in range(2)]
+    x, y = [torch.as_strided(t, (2, axis), (ld, 1)) for t in (store, out)]
+    x.copy_(near)
+    scale, shift = params(axis, torch.float32)
+    _, mean, variance = got = forward(x, scale, shift, out=y)
+    check_forward(got, near, scale, shift)
+    dy = values(2, axis, torch.float16, seed=5)
+    y.copy_(dy)
+    check_backward(backward(x, y, scale, mean, variance, out=y), near, dy, scale, mean, variance)

@@ -234,3 +234,11 @@ def test_the_longest_rows():
         with pytest.raises(kb.KudnnError) as e:
             kb.route(desc(hidden=hidden), None, 16, 16, 16)
         assert e.value.status == status
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [768, 769, 2000])
+@pytest.mark.parametrize("experts,top", [(1, 1), (8, 2), (16, 4), (32, 8), (96, 6)])
+def test_prompts_with_few_experts(cuda_device, tokens, experts, top):
+    x, w = operands(tokens, experts, 264, torch.bfloat16, torch.float32)
+    check(route(x, w, top), definition(x, w, top))

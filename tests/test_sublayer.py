@@ -306,3 +306,52 @@ def test_no_thread_takes_a_report_from_another(cuda_device):
     with pytest.raises(kb.KudnnError):
         kb.experts_check()
     kb.experts_check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,kind", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+def test_operators_of_layer_normalisation_meet_the_contract_of_custom_operators(cuda_device, dtype, kind):
+    x, w, b = torch.randn(3, 5, 72, device="cuda").to(dtype), torch.randn(72, device="cuda").to(kind), torch.randn(72, device="cuda").to(kind)
+    _, mean, variance = ops.layernorm(x, w, b)
+    torch.library.opcheck(ops.layernorm.default, [t.clone().requires_grad_() for t in (x, w, b)] + [1e-5])
+    torch.library.opcheck(ops.layernorm.default, (x.transpose(0, 1)[..., :-1], None, b[:-1], 1e-5))
+    torch.library.opcheck(ops.layernorm_backward.default, (torch.randn_like(x), x, w, mean, variance, 1e-5, kind))
+
+
+@gpu
+def test_operators_of_experts_meet_the_contract_of_custom_operators(cuda_device):
+    x, r = torch.randn(5, 64, device="cuda").bfloat16(), torch.randn(8, 64, device="cuda")
+    u, d = torch.randn(8, 64, 64, device="cuda").bfloat16(), torch.randn(8, 64, 32, device="cuda").bfloat16()
+    torch.library.opcheck(ops.route.default, (x, r, 3, None, "sigmoid", False, 2.0, True))
+    p, ids = ops.route(x, r, 3)
+    for t in (x, torch.randn(64, 5, device="cuda").bfloat16().t()):
+        torch.library.opcheck(ops.experts.default, (t, p, ids, u, d))
+
+
+@gpu
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_a_sublayer_traces_as_one_graph(cuda_device, eight_bit):
+    experts, _ = block(eight_bit, 64)
+    norm = torch_ops.LayerNorm(512, device="cuda", dtype=torch.bfloat16)
+
+    def run(x):
+        return x + experts(norm(x))
+
+    with torch.no_grad():
+        for tokens in (1, 5, 64):
+            x = torch.randn(tokens, 512, device="cuda").bfloat16()
+            assert torch.equal(torch.compile(run, backend="aot_eager", fullgraph=True)(x), run(x))
+
+
+@gpu
+@pytest.mark.parametrize("frozen", range(7))
+def test_gradients_beside_frozen_tensors(cuda_device, frozen):
+    """Bit i of `frozen`: x, the scale, the shift take no gradient; the others' are those of the call with all three."""
+    made = [torch.randn(7, 40, device="cuda"), torch.randn(40, device="cuda"), torch.randn(40, device="cuda")]
+    dy = torch.randn(7, 40, device="cuda")
+    every = [t.clone().requires_grad_() for t in made]
+    some = [t.clone().requires_grad_((frozen >> i & 1) == 0) for i, t in enumerate(made)]
+    for tensors in (every, some):
+        ops.layernorm(*tensors)[0].backward(dy)
+    for i, (a, b) in enumerate(zip(every, some)):
+        assert b.grad is None if (frozen >> i & 1) != 0 else torch.equal(a.grad, b.grad)
