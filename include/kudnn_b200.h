@@ -333,7 +333,7 @@ typedef struct kudnn_b200_route_desc {
     int64_t tokens, hidden, x_ld, w_ld;
     int32_t experts, top, x_dtype, w_dtype, score, normalise;
     float scale;
-    int32_t nan_first; /* 0: as above */
+    int32_t nan_first; /* 1, or as above */
 } kudnn_b200_route_desc;
 KUDNN_B200_API int kudnn_b200_route_validate(const kudnn_b200_route_desc *desc);
 KUDNN_B200_API int kudnn_b200_route_run(const kudnn_b200_route_desc *desc, const void *x, const void *w, const float *bias, float *weights,

@@ -119,7 +119,7 @@ int kudnn_b200_route_run(const kudnn_b200_route_desc *d, const void *x, const vo
     p.w_dtype = d->w_dtype;
     p.sigmoid = d->score == KUDNN_B200_SCORE_SIGMOID ? 1 : 0;
     p.normalise = d->normalise != 0 ? 1 : 0;
-    p.nan_first = d->nan_first != 0 ? 1 : 0;
+    p.nan_first = d->nan_first == 1 ? 1 : 0;  // the place of a field that had no meaning
     p.scale = d->scale;
     const cudaError_t e = kb::launch_route(p, static_cast<cudaStream_t>(cuda_stream));
     return e == cudaSuccess ? KUDNN_B200_OK : fail_cuda(e, "route kernel launch");
