@@ -219,7 +219,8 @@ KUDNN_B200_API int kudnn_b200_rmsnorm_run(const void *src, void *dst, const void
  *   m = mean(x), v = mean((x - m)^2), r = 1 / sqrt(v + eps), y = (x - m) r * scale + shift
  * and, with g = dy * scale and xh = (x - m) r,
  *   dx = r (g - mean(g) - xh mean(g xh)), dscale = sum over rows of dy xh, dshift = sum over rows of dy.
- * All arithmetic is fp32; each result is rounded once, to nearest even.  The same call gives the same bits every time.
+ * All arithmetic is fp32; each result is rounded once, to nearest even.  The same call gives the same bits every time; the same rows elsewhere in
+ * memory, or as part of other calls, may differ in the last bits of fp32, where sums are taken in another order.
  * flags: USE_SCALE, USE_SHIFT (without them 1 and 0); USE_GLOBAL_STATS: mean and variance (fp32, one per row) are given, and constants for the
  * gradient (dx = r g).  Otherwise a run writes them unless they are NULL; the gradient always reads them.
  * scale, shift and their gradients are of param_dtype: F32 or dtype.  dx, dscale and dshift may each be NULL.  y may be x and dx may be x or
@@ -348,7 +349,7 @@ KUDNN_B200_API int kudnn_b200_route_run(const kudnn_b200_route_desc *desc, const
  * type or E4M3 with fp32 scales per 128 x 128 block of [2 ffn, hidden] and [hidden, ffn], as kudnn_b200_quantize_run writes them: x and h are
  * not quantised.  Sums and h are held in 32 bits or as two 16-bit halves of them; y is rounded once.  The same call gives the same bits.
  * y may be x.  Weights whose rows are K-contiguous, 16-byte aligned and 16 bytes apart or a multiple of it are streamed by the fast kernels;
- * other strides take general ones, many times slower.
+ * other strides take general ones, 2 to 11 times slower (1028 x 708 against 1024 x 704, 8 experts: 1 and 64 tokens).
  * The workspace: as many bytes of device memory as experts_workspace says (host arithmetic), on a 16-byte boundary, contents irrelevant, used by
  * one run at a time. */
 typedef struct kudnn_b200_experts_desc {

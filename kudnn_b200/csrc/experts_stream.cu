@@ -2,21 +2,22 @@
 //
 // What bounds it is reading the chosen experts' weights; everything here serves to keep as many bytes in flight as HBM wants, without pauses:
 //   * Both products are cut by weight rows: the rows (gate and up rows in pairs) of all chosen experts are dealt out evenly, one CTA of 8 to 16
-//     warps per SM.  No atomics; sums are added in a fixed order, so that the same call gives the same bits.
+//     warps per SM or two of 8.  No atomics; sums are added in a fixed order, so that the same call gives the same bits.
 //   * The warps stream on their own.  First kernel: tiles of up to 16 pairs of rows go to warps, or to groups of warps that take turns along K
 //     and add up at the end of a tile (plan_tiles).  Second kernel: the CTA's rows times all experts' steps along K are dealt out to the
 //     warps; each keeps sums of y of its own, added up once at the end.  Where a CTA would have 16 rows or fewer, two CTAs of a cluster
 //     share twice as many, half of the steps each.
 //   * A step of a warp is 128 bytes of up to 32 rows, up to four TMA boxes of eight rows, and as much of the first eight tokens' rows, into a ring
-//     of the warp's own, some steps ahead.  Rows and columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their
+//     of the warp's own, of as many steps as shared memory has room for (launch_one).  Rows and columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their
 //     products are dropped).  Copies by every lane (cp.async) or loads into registers took three to five times the instructions of the
 //     products and were bound by their latency; tokens loaded one step ahead were bound by L2's latency.
 //   * 16 bytes per lane, as they lie in the ring, are operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on
 //     that of 8, read in the same permutation.
 //   * The second kernel's CTAs take the place of the first one's as those leave, or stand beside them where two fit an SM: they make their lists, fill
 //     their rings with weights, and wait only before they read h.
-// 1 token, 8 experts 4096 x 2048 of bf16: 77 us, 5.2 TB/s; 64 tokens, 120 experts 2048 x 768: 264 us, 4.3 TB/s; 14 tokens, 50 experts 4096 x 2048 of e4m3:
-// 310 us, 4.1 TB/s.  What is left is the latency of the instructions of a step (1 of 4 issue slots busy with 8 warps) and 5 us of start.
+// 1 token, 8 experts 4096 x 2048 of bf16: 74 to 78 us, 5.2 to 5.5 TB/s; 64 tokens, 120 experts 2048 x 768: 261 to 270 us, 4.2 to 4.4 TB/s; 14 tokens, 50
+// experts 4096 x 2048 of e4m3: 307 to 320 us, 4 TB/s.  What is left is latency: of the instructions of a step (1 of 4 issue slots busy with 8 warps), of
+// the next step's copies where a ring has one step only, and 5 us of start.
 // h is kept as the tensor cores take it without loss: two bf16 halves (of bf16 and e4m3 weights), or fp32 that the second kernel splits into two
 // tf32 halves (of fp16 weights: halves of fp16 would overflow beyond 65504 and lose small values).
 #include "experts.cuh"
@@ -257,7 +258,8 @@ struct Cursor {
 // How the first kernel's tiles are cut, by one warp: with kWarps / w groups of w warps per SM and r rounds of tiles, an expert's rows are cut into
 // as many tiles as that has room for.  What a round costs: the bytes of the SM's tiles at its share of HBM's rate (23 a cycle), or the steps of a
 // warp at what one takes in latency where HBM waits (800 cycles), and the sums of a group, which its stream does not outlast (64 tokens, 120
-// experts 2048 x 768, first kernel: 134 us with tiles per warp, 144, 197 and 178 for groups of 2, 4 and 8).
+// experts 2048 x 768, first kernel: 134 us with tiles per warp, 144, 197 and 178 for groups of 2, 4 and 8).  The rate is that of one CTA per SM:
+// where two share an SM the bytes count for half of what they take.
 template <int kWarps>
 __device__ __forceinline__ void plan_tiles(Lists &l, int active, int ffn, int depth_steps, int lane)
 {
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(kWarpsOf<kW, kTokens> * 32, kTokens == 1 && kW
     constexpr int kPlanes = kDown && !kTf32 ? 2 : 1;  // of the tokens' rows
     constexpr int kTokenElem = kTf32 ? 4 : 2;
     constexpr int kTokenRow = kStep * kTokenElem;     // bytes of a token's row in a step
-    constexpr int kTokenPitch = kTokenRow + 64;       // so that two rows' fragments lie in different banks
+    constexpr int kTokenPitch = kTokenRow + 64;       // two rows of 128 bytes lie in different banks then, of 256 bytes in the same
     constexpr int kLoads = kPiece * kTokenElem / 16;  // 16-byte pieces of a lane's fragment
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t barriers[kWarps][kMostStages];
@@ -940,6 +942,8 @@ cudaError_t launch_one(const ExpertsParams &p, int sm_count, cudaStream_t stream
     const bool two = most > 64ll << 20 && in_half >= 2;
     const int ctas = two ? 2 * sm_count : sm_count;
     shape.cluster = kDown && p.hidden <= 16 * ctas ? 2 : 1;
+    // For 64 experts: 2 to 4 steps of 16-bit weights; of e4m3 weights, with more warps and tokens' rows of 256 bytes, 2, but 1 for 8 tokens and in the
+    // second kernel for 5 to 16, and 2 to 4 from 17 on
     shape.stages = std::min(two || in_half >= 3 ? in_half : (kMostShared - fixed) / stage, kMostStages);
     const size_t shared = static_cast<size_t>(fixed) + static_cast<size_t>(shape.stages) * stage;
     alignas(64) CUtensorMap map;
@@ -973,8 +977,8 @@ cudaError_t launch_tokens(const ExpertsParams &p, int sm_count, cudaStream_t str
 
 }  // namespace
 
-// K-contiguous rows on 16-byte boundaries; the tokens may begin anywhere.  Sizes whose counts of rows, tiles and steps 32 bits hold: 148 x 2^22
-// rows, 1024 experts x 2^22 / 16 tiles (and a round or eight more).
+// K-contiguous rows on 16-byte boundaries; the tokens may begin anywhere.  Sizes whose counts of rows, tiles and steps 32 bits hold: 2^22 rows x
+// 296 CTAs, 1024 experts x 2^22 / 16 tiles (and a round or eight more).
 bool experts_stream_takes(const ExpertsParams &p)
 {
     if (p.hidden > 1 << 22 || p.ffn > 1 << 22) {

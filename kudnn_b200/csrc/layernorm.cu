@@ -258,8 +258,8 @@ __device__ __forceinline__ void copy_piece(unsigned char *to, const void *from)
 // A row lies in shared memory (cp.async, the next one on its way meanwhile; each thread reads back only what it copied itself) and is gone through
 // three times: mean, squares about it, result.  What bounds it is instructions beside HBM: the fewer threads a row has, the fewer of them compute
 // the row's statistics, so teams are as small as sixteen warps per CTA allow, and sums and products are taken two at a time.
-// 16384 x 8192 bf16: 102 to 107 us, 5.0 to 5.3 TB/s (a CTA per row, one value at a time: 122); 9001 x 4099 f16 with fp32 scale and shift: 44 us, 3.4 TB/s
-// (58); 8 x 4096: 4.3 us.  kEdge: the elements in front of the first whole piece and behind the
+// 16384 x 8192 bf16: 101 to 109 us, 4.9 to 5.3 TB/s (a CTA per row, one value at a time: 122); 9001 x 4099 f16 with fp32 scale and shift: 44 us, 3.4 TB/s
+// (58); 8 x 4096: 4.2 us; 8192 x 8192 fp32: 96 us, 5.6 TB/s.  kEdge: the elements in front of the first whole piece and behind the
 // last one are single lanes' own, in registers.
 template <typename T, typename P, bool kEdge>
 __global__ void __launch_bounds__(kMostThreads, 2) layernorm_kernel(const __grid_constant__ LayernormParams p, const __grid_constant__ Teams of)
@@ -374,7 +374,9 @@ __global__ void __launch_bounds__(kMostThreads, 2) layernorm_kernel(const __grid
     }
 }
 
-// Rows longer than shared memory holds, or whose x and y do not begin equally far into a piece: element by element, x read three times.
+// Rows longer than shared memory holds (fp32 from 12,801 elements on, 16 bit with fp32 parameters from 17,065, 16 bit from 25,601), or whose x and y
+// do not begin equally far into a piece: element by element, x read three times.  4096 x 16384 fp32: 205 us, 2.6 TB/s; rows of a view, 16384 x
+// 4096 bf16: 211 us, 1.3 TB/s.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kMostThreads) layernorm_any_kernel(const __grid_constant__ LayernormParams p)
 {
@@ -422,7 +424,8 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_any_kernel(const __gri
 // The gradient, rows as in the forward pass: a thread's kN pieces of x and dy come by way of shared memory, are widened once and kept as xh and g
 // between the row's sums and dx (kKeep), unless that takes too many registers (then it is widened again).  The sums over rows of dscale and dshift stay in registers, each
 // thread its own columns; every CTA leaves one set of them, added up in a fixed order by column_sums_kernel.
-// 16384 x 4096 bf16: 87 to 91 us, 4.4 to 4.6 TB/s, bound by instructions (the schedulers issue in 56 % of the cycles); 16 elements per thread 94.
+// 16384 x 4096 bf16: 87 to 92 us, 4.4 to 4.7 TB/s; the schedulers issue in 56 % of the cycles and HBM is at 65 %, so that it is the chain of a row
+// (load, sums, exchange, dx), of which a team has one at a time, that bounds it; 16 elements per thread 94.
 template <typename T, typename P, int kN, bool kEdge>
 __global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const __grid_constant__ LayernormParams p, const __grid_constant__ Teams of)
 {
@@ -614,7 +617,8 @@ __global__ void __launch_bounds__(kMostThreads) layernorm_backward_kernel(const 
     }
 }
 
-// As layernorm_any_kernel: the sums over a CTA's rows column by column, then dx of them, which may lie where x or dy does.
+// As layernorm_any_kernel (rows from 16,385 elements on): the sums over a CTA's rows column by column, then dx of them, which may lie where x or
+// dy does.  4096 x 18432 bf16: 715 us, a tenth of HBM's rate.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kMostThreads) layernorm_backward_any_kernel(const __grid_constant__ LayernormParams p)
 {

@@ -6,7 +6,9 @@
 // The logits are gathered through distributed shared memory, and a warp finishes each token.  It is latency throughout: reading w once, two
 // cluster barriers, the choice.
 // Many tokens: a CTA takes sixteen and all experts, 64 at a time, two warps side by side for each quarter of K.
-// 1 token x 64 experts x 4096: 7.8 us; 61 x 128 x 2048: 10.7 us; 4096 x 64 x 4096: 93 us, 23 TFLOP/s in 64 bits.
+// 1 token x 64 experts x 4096: 7.8 us; 61 x 128 x 2048: 10.7 us; 4096 x 64 x 4096: 93 us, 23 TFLOP/s in 64 bits, with
+// 8 experts 96 us (all 64 are computed), with 96 or 128 experts 180.  All registers that ptxas spills (332 to 664 bytes per instance) are those of
+// finish_token for more than 256 experts, 32 keys and scores of 64 bits per lane.
 #include "experts.cuh"
 
 #include <cooperative_groups.h>
