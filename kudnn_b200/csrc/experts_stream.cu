@@ -8,9 +8,9 @@
 //     warps; each keeps sums of y of its own, added up once at the end.  Where a CTA would have 16 rows or fewer, two CTAs of a cluster
 //     share twice as many, half of the steps each.
 //   * A step of a warp is 128 bytes of up to 32 rows, up to four TMA boxes of eight rows, and as much of the first eight tokens' rows, into a ring
-//     of the warp's own, of as many steps as shared memory has room for (launch_one).  Rows and columns beyond the matrix come as zeros, rows beyond the tile are another warp's (their
-//     products are dropped).  Copies by every lane (cp.async) or loads into registers took three to five times the instructions of the
-//     products and were bound by their latency; tokens loaded one step ahead were bound by L2's latency.
+//     of the warp's own, of as many steps as shared memory has room for (launch_one).  Rows and columns beyond the matrix come as zeros, rows
+//     beyond the tile are another warp's (their products are dropped).  Copies by every lane (cp.async) or loads into registers took three to
+//     five times the instructions of the products and were bound by their latency; tokens loaded one step ahead were bound by L2's latency.
 //   * 16 bytes per lane, as they lie in the ring, are operand fragments of mma.m16n8k16 with a permuted k: weights on the side of 16 rows, tokens on
 //     that of 8, read in the same permutation.
 //   * The second kernel's CTAs take the place of the first one's as those leave, or stand beside them where two fit an SM: they make their lists, fill

@@ -380,7 +380,8 @@ class Experts(torch.nn.Module):
     quantised on their way to the experts and the gated values between the two products.  Nothing is read back to the host.
 
     few: calls of 16-bit tokens, at most so many (64, and a top of 16, at most), go through ``route`` and ``experts`` instead, three launches in
-    all, which read each chosen expert's weights once and quantise nothing but the weights."""
+    all, which read each chosen expert's weights once and quantise nothing but the weights.  8 suits large experts (4096 x 2048), up to 64 small ones
+    (1024 x 704).  Whether a wait in those kernels gave up, ``kudnn_b200.experts_check`` tells; the module does not ask."""
 
     def __init__(self, router, gate_up, down, top, eight_bit=False, few=0):
         super().__init__()
